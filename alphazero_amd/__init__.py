@@ -5,4 +5,4 @@ src/model.py live in alphazero_amd.game / .mcts / .model; the compute runs in
 libazamd.so (hand-written gfx950 HIP kernels behind the C ABI of
 include/azamd.h).
 """
-__all__ = ["config", "game", "mcts", "model", "engine", "selfplay"]
+__all__ = ["config", "game", "mcts", "model", "engine", "selfplay", "ops", "optim"]

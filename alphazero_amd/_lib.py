@@ -48,6 +48,28 @@ class SelfplayStats(C.Structure):
     ]
 
 
+class NormArgs(C.Structure):
+    _fields_ = ([("n", C.c_int64)] + [(k, C.c_int32) for k in ("c", "hw", "hidden", "dtype", "channels_last", "training")]
+                + [("eps", C.c_double), ("momentum", C.c_double)]
+                + [(k, C.c_void_p) for k in (
+                    "x", "residual", "weight", "bias", "running_mean", "running_var", "num_batches", "fc1_weight", "fc1_bias",
+                    "fc2_weight", "fc2_bias", "saved", "workspace", "out", "grad", "dx", "dresidual", "dweight", "dbias",
+                    "dfc1_weight", "dfc1_bias", "dfc2_weight", "dfc2_bias")])
+
+
+class LossArgs(C.Structure):
+    _fields_ = ([("n", C.c_int64)] + [(k, C.c_int32) for k in ("actions", "outcomes", "dtype")]
+                + [(k, C.c_void_p) for k in ("policy", "wl", "target_pi", "target_wl", "mask", "losses", "stats", "up_loss",
+                                             "up_pi", "up_wl", "dpolicy", "dwl")])
+
+
+class AdamConfig(C.Structure):
+    _fields_ = ([(k, C.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")]
+                + [("decoupled", C.c_int32), ("state_bits", C.c_int32), ("seed", C.c_uint64), ("capacity", C.c_int64),
+                   ("n_partials", C.c_int64), ("n_slots", C.c_int32)]
+                + [(k, C.c_void_p) for k in ("m", "v", "m_scale", "v_scale", "steps", "partials", "norm", "scratch")])
+
+
 # name -> (argtypes); every entry point returns int unless listed in _RESTYPES
 _VP = C.c_void_p
 _SIGNATURES = {
@@ -94,9 +116,17 @@ _SIGNATURES = {
     "az_engine_drain_packed": [_VP, C.c_int64, _VP, C.POINTER(C.c_int64), _VP],
     "az_unpack_samples": [C.c_int64, _VP, _VP, _VP, _VP, _VP],
     "az_engine_selfplay_stats": [_VP, C.POINTER(SelfplayStats), _VP],
+    "az_norm_sizes": [C.POINTER(NormArgs), C.POINTER(C.c_int64)],
+    "az_norm_forward": [C.POINTER(NormArgs), _VP],
+    "az_norm_backward": [C.POINTER(NormArgs), _VP],
+    "az_policy_value_loss_forward": [C.POINTER(LossArgs), _VP],
+    "az_policy_value_loss_backward": [C.POINTER(LossArgs), _VP],
+    "az_grad_sumsq": [C.c_int32, _VP, _VP, _VP, C.c_int64, _VP],
+    "az_adam_step": [C.POINTER(AdamConfig), C.c_int32, _VP, _VP, _VP, _VP, _VP, _VP],
 }
 _OPTIONAL = {}
 
+OPTIM_CHUNK, OPTIM_PAD = 4096, 256      # AZ_OPTIM_CHUNK, AZ_OPTIM_PAD
 PACKED_SAMPLE_BYTES = 792     # AZ_PACKED_SAMPLE_BYTES
 
 _lib = None

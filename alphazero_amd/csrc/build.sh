@@ -36,6 +36,10 @@ $HIPCC $COMMON -mllvm -amdgpu-mfma-vgpr-form=1 -DAZ_SPLIT_STAMPS=${AZ_SPLIT_STAM
 # (v_accvgpr_*, s_nop 7) after any change to tower16.hip: python tools/tower16_isa_check.py [--agpr].
 $HIPCC $COMMON ${T16_FLAGS--mllvm -amdgpu-mfma-vgpr-form=1} -Rpass-analysis=kernel-resource-usage -c tower16.hip -o $OBJ/tower16.o 2> $OBJ/tower16.remarks & pids+=($!)
 $HIPCC $COMMON -c tower_any.hip -o $OBJ/tower_any.o & pids+=($!)
+# training operators; the optimiser's arithmetic is rounded operation by operation
+$HIPCC $COMMON -c train_norm.hip -o $OBJ/train_norm.o & pids+=($!)
+$HIPCC $COMMON -c train_loss.hip -o $OBJ/train_loss.o & pids+=($!)
+$HIPCC $COMMON -ffp-contract=off -c optim.hip -o $OBJ/optim.o & pids+=($!)
 g++ -O2 -fPIC -std=c++17 ${HOSTSAN:+-fsanitize=undefined -fsanitize-undefined-trap-on-error} -c core.cpp -o $OBJ/core.o & pids+=($!)
 for p in "${pids[@]}"; do wait $p; done
 $HIPCC --offload-arch=gfx950 -shared -fPIC -o $OUT $OBJ/*.o

@@ -1,0 +1,269 @@
+"""Adam and AdamW over all tensors of a model in a few launches (az_grad_sumsq, az_adam_step in include/azamd.h),
+with gradient clipping by the global norm and moments in 32 bits or in 8.  It needs parameters on a GPU; there is
+no CPU fallback."""
+import array
+import ctypes as C
+from operator import is_
+
+import torch
+
+from . import _lib
+
+_PAD, _CHUNK = _lib.OPTIM_PAD, _lib.OPTIM_CHUNK
+
+
+def _dense(t):
+    """Whether t's elements fill one stretch of memory, in whatever order of dimensions."""
+    if t.numel() == 0:
+        return True
+    expected = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _encode(x, positive):
+    """Float32 values -> (e4m3 codes, a power of two per 256), to nearest: exact for values that came out of _decode.
+    positive: what is not zero does not become zero."""
+    x = x.reshape(-1, _PAD)
+    magnitude = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x))
+    mantissa, exponent = torch.frexp(magnitude.amax(1))
+    exponent = torch.where(mantissa > 0, exponent - 9 + (mantissa > 0.875), torch.full_like(exponent, -108)).clamp(min=-108)
+    scale = ((exponent + 127) << 23).view(torch.float32)          # 2 ** exponent, exactly
+    y = x / scale[:, None]
+    if positive:
+        y = torch.where((y > 0) & (y < 2.0 ** -9), torch.full_like(y, 2.0 ** -9), y)
+    return y.to(torch.float8_e4m3fn).reshape(-1), scale
+
+
+def _decode(codes, scale):
+    return (codes.float().reshape(-1, _PAD) * scale[:, None]).reshape(-1)
+
+
+class FusedAdam(torch.optim.Optimizer):
+    """torch.optim.Adam(params, lr, betas, eps, weight_decay), or AdamW with decoupled=True, for float32 parameters on
+    one GPU, as two to four launches for all of them.
+
+    step(max_norm=x) also clips by the norm over the gradients of all parameters: they are scaled by
+    min(1, x / (norm + 1e-6)) on the way into the update (the .grad tensors keep their values; torch's
+    clip_grad_norm_ would overwrite them).  `grad_norm` is the norm of the last such step, a float32 scalar on the GPU.
+
+    state_bits=32 keeps the moments in float32.  state_bits=8 keeps m and sqrt(v) as e4m3 codes with one power of two
+    per 256, rounded at random (reproducibly: by `seed`, the step and the place): 2 bytes per weight instead of 8.
+
+    state_dict() is torch.optim.Adam's: per parameter step, exp_avg, exp_avg_sq (float32, also with 8-bit moments, which
+    a load restores exactly), so checkpoints go both ways.  Step counters live on the GPU; a step can be captured into
+    a HIP graph (learning rate and the other hyper-parameters are constants of the capture).  amsgrad, maximize,
+    sparse gradients and parameter groups added after construction are refused."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled=False, state_bits=32, seed=0):
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
+            raise ValueError(f"betas must lie in [0, 1), got {betas}")
+        if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"lr, eps and weight_decay must not be negative, got {lr}, {eps}, {weight_decay}")
+        self.state_bits, self.seed = state_bits, int(seed)
+        self._built = False
+        # capturable: what torch.optim.Adam calls an optimiser whose step counters are on the GPU
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled=decoupled, capturable=True))
+        self._build()
+
+    # ------------------------------------------------------------------ layout
+    def add_param_group(self, param_group):
+        if self._built:
+            raise RuntimeError("FusedAdam takes all its parameter groups at construction")
+        super().add_param_group(param_group)
+
+    def _build(self):
+        params = [p for g in self.param_groups for p in g["params"]]
+        device = params[0].device
+        if device.type != "cuda":
+            raise ValueError(f"FusedAdam needs parameters on a GPU, got one on {device}")
+        for p in params:
+            if p.dtype != torch.float32:
+                raise TypeError(f"FusedAdam takes float32 parameters, got {p.dtype}")
+            if p.device != device:
+                raise ValueError(f"all parameters must be on one GPU, got {device} and {p.device}")
+            if not _dense(p):
+                raise ValueError(f"a parameter of shape {tuple(p.shape)} and strides {p.stride()} does not fill its memory")
+        self._params, self._device = params, device
+        self._offsets, total = [], 0
+        for p in params:
+            self._offsets.append(total)
+            total += -(-p.numel() // _PAD) * _PAD
+        self._capacity = total
+        self._partials = sum(-(-p.numel() // _CHUNK) for p in params)
+        shape = dict(device=device)
+        self._step = torch.zeros(len(params), dtype=torch.float32, **shape)
+        if self.state_bits == 32:
+            self._flat = {"exp_avg": torch.zeros(total, **shape), "exp_avg_sq": torch.zeros(total, **shape)}
+        else:
+            self._flat = {}
+            for name in ("exp_avg", "exp_rms"):
+                self._flat[name] = torch.zeros(total, dtype=torch.uint8, **shape).view(torch.float8_e4m3fn)
+                self._flat[name + "_scale"] = torch.full((total // _PAD,), 2.0 ** -108, **shape)
+        self.grad_norm = torch.zeros((), **shape)
+        self._pointers = self._strides = None        # of the parameters, when they were last looked at
+        self._grads = []                             # gradients whose strides were last looked at
+        self._groups = []
+        at = 0
+        for g in self.param_groups:
+            k = len(g["params"])
+            self._groups.append(range(at, at + k))
+            at += k
+        self._built = True
+        self._attach()
+
+    def _view(self, flat, i):
+        p, at = self._params[i], self._offsets[i]
+        return flat[at:at + p.numel()].as_strided(p.size(), p.stride())
+
+    def _attach(self):
+        """self.state as torch.optim.Adam has it: views of the flat buffers."""
+        self.state.clear()
+        for i, p in enumerate(self._params):
+            self.state[p] = {"step": self._step[i]}
+            if self.state_bits == 32:
+                self.state[p].update((k, self._view(v, i)) for k, v in self._flat.items())
+
+    def flat_state(self):
+        """The live buffers: `step` (float32, one per parameter) and the moments, parameter after parameter in the order of
+        the groups, each in the parameter's memory order and padded with zeros to a multiple of 256 elements.
+        32 bits: exp_avg, exp_avg_sq.  8 bits: exp_avg and exp_rms (the root of exp_avg_sq) as float8_e4m3fn, and
+        exp_avg_scale, exp_rms_scale, the power of two that each 256 of them are multiplied with."""
+        return {"step": self._step, **self._flat}
+
+    # ------------------------------------------------------------------ checkpoints
+    def __getstate__(self):
+        raise TypeError("FusedAdam is not copied or pickled as a whole: use state_dict()")
+
+    def state_dict(self):
+        sd = super().state_dict()
+        if self.state_bits == 8:
+            m = _decode(self._flat["exp_avg"], self._flat["exp_avg_scale"])
+            v = _decode(self._flat["exp_rms"], self._flat["exp_rms_scale"]).square()
+            sd["state"] = {i: {"step": self._step[i], "exp_avg": self._view(m, i), "exp_avg_sq": self._view(v, i)}
+                           for i in range(len(self._params))}
+        return sd
+
+    def load_state_dict(self, state_dict):
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad") or g.get("maximize"):
+                raise ValueError("FusedAdam has no amsgrad and no maximize")
+        before = self.param_groups
+        super().load_state_dict(state_dict)
+        for g, old in zip(self.param_groups, before):
+            g["decoupled"] = g.get("decoupled", old["decoupled"])
+            g["capturable"] = True
+        moments = {k: torch.zeros(self._capacity, device=self._device) for k in ("exp_avg", "exp_avg_sq")}
+        with torch.no_grad():
+            for i, p in enumerate(self._params):
+                st = self.state.get(p, {})
+                self._step[i] = float(st["step"]) if "step" in st else 0.0
+                for k, flat in moments.items():
+                    if k in st:
+                        self._view(flat, i).copy_(st[k])
+            if self.state_bits == 32:
+                for k, flat in moments.items():
+                    self._flat[k].copy_(flat)
+            else:
+                for name, x in (("exp_avg", moments["exp_avg"]), ("exp_rms", moments["exp_avg_sq"].sqrt())):
+                    codes, scale = _encode(x, name == "exp_rms")
+                    self._flat[name].copy_(codes)
+                    self._flat[name + "_scale"].copy_(scale)
+        self._attach()
+
+    # ------------------------------------------------------------------ the step
+    def zero_grad(self, set_to_none=True):
+        if set_to_none:
+            self._grads = []                 # do not keep them alive
+        super().zero_grad(set_to_none)
+
+    def _look_at_params(self):
+        for p in self._params:
+            if p.dtype != torch.float32 or p.device != self._device:
+                raise ValueError(f"a parameter became {p.dtype} on {p.device} after FusedAdam was built")
+        strides = [p.stride() for p in self._params]
+        if self._strides is not None and strides != self._strides:
+            raise ValueError("a parameter's strides changed after FusedAdam was built: its moments are in the old order")
+        self._strides = strides
+
+    def _look_at_grads(self, grads):
+        """Gradients in their parameter's memory order (autograd makes them so; anything else is copied)."""
+        out = []
+        for p, g in zip(self._params, grads):
+            if g is not None:
+                if g.is_sparse or g.layout != torch.strided:
+                    raise ValueError("FusedAdam takes dense gradients")
+                if g.dtype != torch.float32 or g.device != self._device or g.shape != p.shape:
+                    raise ValueError(f"the gradient of a parameter of shape {tuple(p.shape)} is {g.dtype} {tuple(g.shape)} on {g.device}")
+                if g.stride() != p.stride() and any(a != b and n > 1 for a, b, n in zip(g.stride(), p.stride(), p.shape)):
+                    g = torch.empty_strided(p.size(), p.stride(), dtype=g.dtype, device=g.device).copy_(g)
+            out.append(g)
+        return out
+
+    @torch.no_grad()
+    def step(self, closure=None, max_norm=None):
+        """One update.  max_norm (> 0): clip by the global norm first."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError(f"max_norm must be positive, got {max_norm}")
+        pointers = [p.data_ptr() for p in self._params]
+        if pointers != self._pointers:
+            self._look_at_params()
+            self._pointers = pointers
+        grads = [p.grad for p in self._params]
+        if len(grads) != len(self._grads) or not all(map(is_, grads, self._grads)):
+            seen, grads = grads, self._look_at_grads(grads)
+            self._grads = seen if all(map(is_, seen, grads)) else []
+        with torch.cuda.device(self._device):
+            self._launch(pointers, grads, max_norm)
+        return loss
+
+    def _launch(self, pointers, grads, max_norm):
+        L, params = _lib.lib(), self._params
+        stream = torch.cuda.current_stream(self._device).cuda_stream
+        sizes = [p.numel() for p in params]
+        use = [i for i, g in enumerate(grads) if g is not None and sizes[i]]
+        if not use:
+            return
+        g_ptr = [0 if g is None else g.data_ptr() for g in grads]
+
+        def table(code, values):
+            a = array.array(code, values)
+            return a, a.buffer_info()[0]
+        scratch = torch.empty(4 + 3 * len(params), dtype=torch.float32, device=self._device)
+        partials = None
+        if max_norm is not None:
+            partials = torch.empty(self._partials, dtype=torch.float64, device=self._device)
+            (a, a_at), (b, b_at) = table("Q", [g_ptr[i] for i in use]), table("q", [sizes[i] for i in use])
+            n_partials = sum(-(-sizes[i] // _CHUNK) for i in use)
+            _lib.check(L.az_grad_sumsq(len(use), a_at, b_at, partials.data_ptr(), n_partials, stream))
+        flat = self._flat
+        moments = (flat["exp_avg"], flat["exp_avg_sq"], None, None) if self.state_bits == 32 else (
+            flat["exp_avg"], flat["exp_rms"], flat["exp_avg_scale"], flat["exp_rms_scale"])
+        changed = []
+        for group, members in zip(self.param_groups, self._groups):
+            mine = [i for i in use if i in members]
+            if not mine:
+                continue
+            cfg = _lib.AdamConfig(
+                group["lr"], *group["betas"], group["eps"], group["weight_decay"], max_norm or 0.0, int(group["decoupled"]),
+                self.state_bits, self.seed & 0xFFFFFFFF, self._capacity, 0 if partials is None else n_partials, len(params),
+                *(None if t is None else t.data_ptr() for t in moments), self._step.data_ptr(),
+                None if partials is None else partials.data_ptr(), self.grad_norm.data_ptr() if partials is not None else None,
+                scratch.data_ptr())
+            tables = [table("Q", [pointers[i] for i in mine]), table("Q", [g_ptr[i] for i in mine]), table("q", [sizes[i] for i in mine]),
+                      table("q", [self._offsets[i] for i in mine]), table("i", mine)]
+            _lib.check(L.az_adam_step(C.byref(cfg), len(mine), *(at for _, at in tables), stream))
+            changed += [params[i] for i in mine]
+        if self.state_bits == 32:
+            changed += list(flat.values())
+        # written behind torch's back: whoever watches version counters has to see it
+        torch.autograd.graph.increment_version(changed + [self._step])

@@ -323,6 +323,100 @@ int az_unpack_samples(int64_t n, const void* packed_dev, float* states_dev, floa
                       float* wls_dev, void* stream);
 int az_engine_selfplay_stats(az_engine* e, az_selfplay_stats* out, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Training operators.  The reference trains with torch modules
+ * (src/parallel_trainer.py:225-284: forward, two cross-entropies, gradient
+ * clipping, Adam; src/model.py:56-92: BatchNorm, squeeze-excitation, residual,
+ * ReLU); these are the same operations in a few launches each.  Activations and
+ * logits are float32, bfloat16 or float16, parameters, statistics and sums
+ * float32 or wider.  Nothing is allocated, uploaded or synchronised: every entry
+ * can be captured into a HIP graph.  Outputs do not depend on the scheduling of
+ * workgroups.  Pointers need only their element's alignment unless said otherwise.
+ */
+#define AZ_F32 0
+#define AZ_BF16 1
+#define AZ_F16 2
+
+/* Batch normalisation with ReLU (hidden == 0: relu(bn(x)), src/model.py:82-84), or the end of a
+ * squeeze-excitation residual block (hidden > 0: relu(bn(x) * sigmoid(w) + b + residual) with
+ * (w, b) = fc2(relu(fc1(mean over the board of bn(x)))), src/model.py:40-53, 85-92).
+ * x, residual, out, grad, dx, dresidual: [n][c][hw], or [n][hw][c] with channels_last != 0.
+ * Sizes in bytes of `saved` (kept for the backward pass), of the forward and of the backward
+ * workspace: az_norm_sizes.  These buffers are 16-byte aligned. */
+typedef struct {
+    int64_t n;
+    int32_t c, hw, hidden;       /* hidden > 0: c <= 1024 and hidden <= 1024 */
+    int32_t dtype, channels_last;
+    int32_t training;            /* 1: the batch's statistics, running ones updated; 0: the running statistics */
+    double eps, momentum;
+    const void *x_dev, *residual_dev;
+    const float *weight_dev, *bias_dev;             /* [c] */
+    float *running_mean_dev, *running_var_dev;      /* [c]; may be null in training */
+    int64_t* num_batches_dev;                       /* counts a training call; may be null */
+    const float *fc1_weight_dev, *fc1_bias_dev;     /* [hidden][c], [hidden] */
+    const float *fc2_weight_dev, *fc2_bias_dev;     /* [2c][hidden], [2c] */
+    void* saved_dev;
+    void* workspace_dev;
+    void* out_dev;
+    /* backward only */
+    const void* grad_dev;
+    void *dx_dev, *dresidual_dev;
+    float *dweight_dev, *dbias_dev;
+    float *dfc1_weight_dev, *dfc1_bias_dev, *dfc2_weight_dev, *dfc2_bias_dev;
+} az_norm_args;
+int az_norm_sizes(const az_norm_args* args, int64_t sizes_host[3]);
+int az_norm_forward(const az_norm_args* args, void* stream);
+int az_norm_backward(const az_norm_args* args, void* stream);
+
+/* losses_dev[3] = (sum, policy, outcome): mean over n rows of the soft-target cross-entropy of
+ * policy [n][actions] and wl [n][outcomes] (src/parallel_trainer.py:251-260).  mask_dev
+ * ([n][actions] bytes, may be null): places with 0 take no part, whatever they hold; a row
+ * without any has loss 0.  stats_dev: 8 n floats, 16-byte aligned, filled by the forward call and
+ * read by the backward call.  upstream_dev: gradients of the three losses, null = 0. */
+typedef struct {
+    int64_t n;
+    int32_t actions, outcomes, dtype;
+    const void *policy_dev, *wl_dev;
+    const float *target_pi_dev, *target_wl_dev;
+    const uint8_t* mask_dev;
+    float *losses_dev, *stats_dev;
+    const float* upstream_dev[3];
+    void *dpolicy_dev, *dwl_dev;
+} az_loss_args;
+int az_policy_value_loss_forward(const az_loss_args* args, void* stream);
+int az_policy_value_loss_backward(const az_loss_args* args, void* stream);
+
+/* One Adam (decoupled == 0: weight decay added to the gradient, torch.optim.Adam of
+ * src/parallel_trainer.py:121) or AdamW step over `count` float32 tensors, given as host arrays of
+ * device addresses and sizes in elements.  Tensor i's moments start at element offsets_host[i] (a
+ * multiple of AZ_OPTIM_PAD) of m_dev / v_dev, which hold `capacity` elements; its step counter is
+ * steps_dev[slots_host[i]] (float32, incremented by the call).  A slot appears once.
+ * state_bits 32: m and v as float32.  state_bits 8: m and sqrt(v) as e4m3 codes, one power of
+ * two per AZ_OPTIM_PAD of them in m_scale_dev / v_scale_dev, rounded at random (a hash of seed,
+ * step counter and place).
+ * max_norm > 0: gradients are scaled by min(1, max_norm / (norm + 1e-6)) on the way in, norm being
+ * the root of the sum of partials_dev[0..n_partials) (az_grad_sumsq over every tensor, one partial
+ * sum per AZ_OPTIM_CHUNK elements of a tensor); the gradients themselves are not written.
+ * scratch_dev: 4 + 3 * n_slots floats. */
+#define AZ_OPTIM_CHUNK 4096
+#define AZ_OPTIM_PAD 256
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay, max_norm;
+    int32_t decoupled, state_bits;
+    uint64_t seed;
+    int64_t capacity, n_partials;
+    int32_t n_slots;
+    void *m_dev, *v_dev;
+    float *m_scale_dev, *v_scale_dev, *steps_dev;
+    const double* partials_dev;
+    float* norm_dev;             /* receives the norm; may be null */
+    float* scratch_dev;
+} az_adam_config;
+int az_grad_sumsq(int32_t count, const uint64_t* grads_host, const int64_t* sizes_host, double* partials_dev,
+                  int64_t n_partials, void* stream);
+int az_adam_step(const az_adam_config* cfg, int32_t count, const uint64_t* params_host, const uint64_t* grads_host,
+                 const int64_t* sizes_host, const int64_t* offsets_host, const int32_t* slots_host, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,140 @@
+"""CPU: what the training operators refuse before anything reaches a GPU - the Python entry points' checks of
+types, shapes and devices, and the C entries' checks of their arguments."""
+import ctypes as C
+
+import pytest
+import torch
+
+from alphazero_amd import _lib, ops
+from alphazero_amd.optim import FusedAdam, _decode, _dense, _encode
+
+
+def test_structures_match_the_header(tmp_path):
+    """The ctypes mirrors have the C structures' sizes (compiled from include/azamd.h)."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "azamd.h"\nint main(void) { printf("%zu %zu %zu %d %d", sizeof(az_norm_args), '
+                   'sizeof(az_loss_args), sizeof(az_adam_config), AZ_OPTIM_CHUNK, AZ_OPTIM_PAD); return 0; }\n')
+    subprocess.check_call(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "sizes")])
+    got = [int(v) for v in subprocess.check_output([str(tmp_path / "sizes")]).split()]
+    assert got == [C.sizeof(_lib.NormArgs), C.sizeof(_lib.LossArgs), C.sizeof(_lib.AdamConfig), _lib.OPTIM_CHUNK, _lib.OPTIM_PAD]
+
+
+def test_host_tensors_are_refused():
+    x, v = torch.zeros(2, 4, 3, 3), torch.zeros(4)
+    with pytest.raises(ValueError, match="need a GPU tensor"):
+        ops.norm_act(x, v, v, v, v)
+    with pytest.raises(ValueError, match="need a GPU tensor"):
+        ops.norm_gate_residual(x, x, v, v, v, v, torch.zeros(2, 4), torch.zeros(2), torch.zeros(8, 2), torch.zeros(8))
+    with pytest.raises(ValueError, match="needs GPU tensors"):
+        ops.policy_value_loss(torch.zeros(2, 5), torch.zeros(2, 2), torch.zeros(2, 5), torch.zeros(2, 2))
+    with pytest.raises(ValueError, match="parameters on a GPU"):
+        FusedAdam([torch.zeros(3, requires_grad=True)])
+
+
+@pytest.mark.parametrize("kwargs, match", [({"state_bits": 16}, "state_bits"), ({"betas": (1.0, 0.9)}, "betas"),
+                                           ({"lr": -1.0}, "negative"), ({"eps": -1.0}, "negative"), ({"weight_decay": -1.0}, "negative")])
+def test_optimiser_refuses_hyper_parameters(kwargs, match):
+    with pytest.raises(ValueError, match=match):
+        FusedAdam([torch.zeros(3, requires_grad=True)], **kwargs)
+
+
+def _norm_args(**kw):
+    a = _lib.NormArgs(4, 8, 9, 0, 0, 0, 1, 1e-5, 0.1)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("kw, match", [
+    ({"n": 0}, "out of range"), ({"c": 0}, "out of range"), ({"hw": 0}, "out of range"), ({"n": 1 << 28, "c": 64}, "out of range"),
+    ({"dtype": 3}, "unknown type"), ({"n": 1, "hw": 1}, "two values"), ({"hidden": -1}, "a gate takes"), ({"hidden": 1025}, "a gate takes"),
+    ({"hidden": 2, "c": 1025}, "a gate takes"), ({}, "null argument"),
+])
+def test_c_entries_of_the_norms_check_their_arguments(kw, match):
+    L = _lib.lib()
+    for entry in (L.az_norm_forward, L.az_norm_backward):
+        assert entry(C.byref(_norm_args(**kw)), None) == -1
+        assert match.encode() in L.az_last_error()
+    assert L.az_norm_forward(None, None) == -1 and L.az_norm_sizes(C.byref(_norm_args()), None) == -1
+
+
+def test_c_entries_of_the_norms_check_alignment():
+    L = _lib.lib()
+    full = dict(x=64, weight=64, bias=64, saved=64, workspace=72, out=64)      # addresses are only looked at
+    assert L.az_norm_forward(C.byref(_norm_args(**full)), None) == -1 and b"aligned" in L.az_last_error()
+    full["workspace"] = 64
+    assert L.az_norm_forward(C.byref(_norm_args(training=0, **full)), None) == -1 and b"running" in L.az_last_error()
+
+
+@pytest.mark.parametrize("kw, match", [
+    ({"n": 0}, "rows"), ({"actions": 0}, "actions"), ({"outcomes": 0}, "outcomes"), ({"outcomes": 4097}, "outcomes"),
+    ({"policy": None}, "null input"), ({"stats": 68}, "aligned"), ({"losses": None}, "null output"), ({"dtype": 7}, "unknown type"),
+])
+def test_c_entry_of_the_loss_checks_its_arguments(kw, match):
+    L = _lib.lib()
+    a = _lib.LossArgs(4, 5, 2, 0, 64, 64, 64, 64, None, 64, 64)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    assert L.az_policy_value_loss_forward(C.byref(a), None) == -1
+    assert match.encode() in L.az_last_error()
+    a = _lib.LossArgs(4, 5, 2, 0, 64, 64, 64, 64, None, 64, 64)
+    assert L.az_policy_value_loss_backward(C.byref(a), None) == -1 and b"null gradient" in L.az_last_error()
+
+
+def _adam(**kw):
+    a = _lib.AdamConfig(1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, 0, 32, 0, 1024, 0, 2, 64, 64, None, None, 64, None, None, 64)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("kw, size, offset, slot, match", [
+    ({"state_bits": 16}, 10, 0, 0, "moments in 16 bits"), ({"m": None}, 10, 0, 0, "null state"), ({"state_bits": 8}, 10, 0, 0, "scales"),
+    ({"m": 68}, 10, 0, 0, "aligned"), ({"n_slots": 0}, 10, 0, 0, "step counters"), ({}, 10, 0, 2, "step counter 2 of 2"),
+    ({}, 10, 100, 0, "does not fit"), ({}, 1025, 0, 0, "does not fit"), ({}, 800, 256, 0, "does not fit"), ({}, -1, 0, 0, "does not fit"),
+    ({}, 10, -256, 0, "does not fit"), ({"max_norm": 1.0, "n_partials": 1}, 10, 0, 0, "partial sums"),
+])
+def test_c_entry_of_the_step_checks_its_arguments(kw, size, offset, slot, match):
+    L = _lib.lib()
+    p, s, o, i = (C.c_uint64 * 1)(64), (C.c_int64 * 1)(size), (C.c_int64 * 1)(offset), (C.c_int32 * 1)(slot)
+    assert L.az_adam_step(C.byref(_adam(**kw)), 1, p, p, s, o, i, None) == -1
+    assert match.encode() in L.az_last_error()
+
+
+def test_c_entries_refuse_misaligned_tensors_and_short_partials():
+    L = _lib.lib()
+    good, odd, s, z, i = (C.c_uint64 * 1)(64), (C.c_uint64 * 1)(66), (C.c_int64 * 1)(5000), (C.c_int64 * 1)(0), (C.c_int32 * 1)(0)
+    assert L.az_grad_sumsq(1, good, s, 64, 1, None) == -1 and b"2 partial sums" in L.az_last_error()
+    assert L.az_grad_sumsq(1, odd, s, 64, 2, None) == -1 and b"aligned" in L.az_last_error()
+    cfg = _adam(capacity=8192)
+    assert L.az_adam_step(C.byref(cfg), 1, odd, good, s, z, i, None) == -1 and b"aligned" in L.az_last_error()
+    assert L.az_adam_step(C.byref(cfg), 0, None, None, None, None, None, None) == 0          # nothing to do is fine
+    assert L.az_grad_sumsq(0, None, None, None, 0, None) == 0
+
+
+def test_eight_bit_moments_survive_a_checkpoint():
+    """_encode returns exactly what _decode gave: every code of a block whatever its power of two, and a block whose
+    largest value is small among its codes."""
+    codes = torch.arange(256, dtype=torch.uint8)
+    codes[0x7F] = codes[0xFF] = 0                                    # NaN
+    for exponent in (-108, -20, 0, 40):
+        x = _decode(codes.view(torch.float8_e4m3fn), torch.tensor([2.0 ** exponent]))
+        back = _decode(*_encode(x, False))
+        assert torch.equal(back, x)
+        small = x * (x.abs() <= 3 * 2.0 ** (exponent - 9))
+        assert torch.equal(_decode(*_encode(small, False)), small)
+    root = torch.full((256,), 1e-12)
+    root[0] = 1.0
+    held = _decode(*_encode(root, True))
+    assert held[0] == 1.0 and bool((held[1:] > 0).all())            # a root never becomes zero
+    assert bool((_decode(*_encode(torch.zeros(512), True)) == 0).all())
+
+
+def test_dense_layouts_are_told_apart():
+    t = torch.zeros(4, 6, 3, 3)
+    assert _dense(t) and _dense(t.to(memory_format=torch.channels_last)) and _dense(t.permute(3, 1, 0, 2)) and _dense(t[:, :, :0])
+    assert not _dense(t[:, :3]) and not _dense(t[..., ::2]) and not _dense(torch.zeros(1, 4).expand(3, 4))
+    assert _dense(torch.zeros(())) and _dense(torch.zeros(1)[:, None].expand(1, 1))
