@@ -159,6 +159,27 @@ def check(rc):
         raise AzError(f"libazamd error {rc}: {lib().az_last_error().decode()}")
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The native torch side of the training operators (csrc/torch_ops.cpp), calling the library that lib() loaded."""
+    global _torch_ops
+    if _torch_ops is None:
+        L = lib()
+        try:
+            import torch  # noqa: F401  (the module resolves against torch's libraries)
+            from . import _azops
+        except ImportError as e:
+            raise AzError(f"alphazero_amd/_azops.so does not load ({e}): build it with alphazero_amd/csrc/build.sh "
+                          "(__graft_entry__.build()).  There is no fallback path.") from e
+        names = ("az_last_error", "az_norm_sizes", "az_norm_forward", "az_norm_backward", "az_policy_value_loss_forward",
+                 "az_policy_value_loss_backward", "az_grad_sumsq", "az_adam_step")
+        _azops.bind({n: C.cast(getattr(L, n), C.c_void_p).value for n in names}, AzError)
+        _torch_ops = _azops
+    return _torch_ops
+
+
 def exported_symbols():
     """Every symbol include/azamd.h declares (parsed from the header)."""
     import re

@@ -41,6 +41,14 @@ $HIPCC $COMMON -c train_norm.hip -o $OBJ/train_norm.o & pids+=($!)
 $HIPCC $COMMON -c train_loss.hip -o $OBJ/train_loss.o & pids+=($!)
 $HIPCC $COMMON -ffp-contract=off -c optim.hip -o $OBJ/optim.o & pids+=($!)
 g++ -O2 -fPIC -std=c++17 ${HOSTSAN:+-fsanitize=undefined -fsanitize-undefined-trap-on-error} -c core.cpp -o $OBJ/core.o & pids+=($!)
+# the operators' torch side (autograd nodes, the optimiser's walk over its tensors): host code only, into a module of its own
+if [ "${HOSTSAN:-0}" != "1" ]; then
+  TORCH=$(python3 -c "import os, torch; print(os.path.dirname(torch.__file__))")
+  PYINC=$(python3 -c "import sysconfig; print(sysconfig.get_paths()['include'])")
+  g++ -O2 -fPIC -std=c++17 -shared -fvisibility=hidden -Wall -D__HIP_PLATFORM_AMD__ -DUSE_ROCM -isystem $TORCH/include \
+    -isystem $TORCH/include/torch/csrc/api/include -isystem /opt/rocm/include -isystem $PYINC torch_ops.cpp -o ../_azops.so \
+    -L$TORCH/lib -lc10 -lc10_hip -ltorch_cpu -ltorch -ltorch_python & pids+=($!)
+fi
 for p in "${pids[@]}"; do wait $p; done
 $HIPCC --offload-arch=gfx950 -shared -fPIC -o $OUT $OBJ/*.o
 echo "built $(readlink -f $OUT)"

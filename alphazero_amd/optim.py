@@ -1,15 +1,11 @@
 """Adam and AdamW over all tensors of a model in a few launches (az_grad_sumsq, az_adam_step in include/azamd.h),
 with gradient clipping by the global norm and moments in 32 bits or in 8.  It needs parameters on a GPU; there is
 no CPU fallback."""
-import array
-import ctypes as C
-from operator import is_
-
 import torch
 
 from . import _lib
 
-_PAD, _CHUNK = _lib.OPTIM_PAD, _lib.OPTIM_CHUNK
+_PAD = _lib.OPTIM_PAD
 
 
 def _dense(t):
@@ -95,7 +91,6 @@ class FusedAdam(torch.optim.Optimizer):
             self._offsets.append(total)
             total += -(-p.numel() // _PAD) * _PAD
         self._capacity = total
-        self._partials = sum(-(-p.numel() // _CHUNK) for p in params)
         shape = dict(device=device)
         self._step = torch.zeros(len(params), dtype=torch.float32, **shape)
         if self.state_bits == 32:
@@ -106,14 +101,16 @@ class FusedAdam(torch.optim.Optimizer):
                 self._flat[name] = torch.zeros(total, dtype=torch.uint8, **shape).view(torch.float8_e4m3fn)
                 self._flat[name + "_scale"] = torch.full((total // _PAD,), 2.0 ** -108, **shape)
         self.grad_norm = torch.zeros((), **shape)
-        self._pointers = self._strides = None        # of the parameters, when they were last looked at
-        self._grads = []                             # gradients whose strides were last looked at
         self._groups = []
         at = 0
         for g in self.param_groups:
             k = len(g["params"])
-            self._groups.append(range(at, at + k))
+            self._groups.append((at, at + k))
             at += k
+        m, v = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_rms")
+        self._plan = _lib.torch_ops().AdamPlan(
+            params, self._offsets, total, self.state_bits, self.seed & 0xFFFFFFFF, self._step, self._flat[m], self._flat[v],
+            self._flat.get(m + "_scale"), self._flat.get(v + "_scale"), self.grad_norm)
         self._built = True
         self._attach()
 
@@ -177,35 +174,6 @@ class FusedAdam(torch.optim.Optimizer):
         self._attach()
 
     # ------------------------------------------------------------------ the step
-    def zero_grad(self, set_to_none=True):
-        if set_to_none:
-            self._grads = []                 # do not keep them alive
-        super().zero_grad(set_to_none)
-
-    def _look_at_params(self):
-        for p in self._params:
-            if p.dtype != torch.float32 or p.device != self._device:
-                raise ValueError(f"a parameter became {p.dtype} on {p.device} after FusedAdam was built")
-        strides = [p.stride() for p in self._params]
-        if self._strides is not None and strides != self._strides:
-            raise ValueError("a parameter's strides changed after FusedAdam was built: its moments are in the old order")
-        self._strides = strides
-
-    def _look_at_grads(self, grads):
-        """Gradients in their parameter's memory order (autograd makes them so; anything else is copied)."""
-        out = []
-        for p, g in zip(self._params, grads):
-            if g is not None:
-                if g.is_sparse or g.layout != torch.strided:
-                    raise ValueError("FusedAdam takes dense gradients")
-                if g.dtype != torch.float32 or g.device != self._device or g.shape != p.shape:
-                    raise ValueError(f"the gradient of a parameter of shape {tuple(p.shape)} is {g.dtype} {tuple(g.shape)} on {g.device}")
-                if g.stride() != p.stride() and any(a != b and n > 1 for a, b, n in zip(g.stride(), p.stride(), p.shape)):
-                    g = torch.empty_strided(p.size(), p.stride(), dtype=g.dtype, device=g.device).copy_(g)
-            out.append(g)
-        return out
-
-    @torch.no_grad()
     def step(self, closure=None, max_norm=None):
         """One update.  max_norm (> 0): clip by the global norm first."""
         loss = None
@@ -214,56 +182,6 @@ class FusedAdam(torch.optim.Optimizer):
                 loss = closure()
         if max_norm is not None and not max_norm > 0:
             raise ValueError(f"max_norm must be positive, got {max_norm}")
-        pointers = [p.data_ptr() for p in self._params]
-        if pointers != self._pointers:
-            self._look_at_params()
-            self._pointers = pointers
-        grads = [p.grad for p in self._params]
-        if len(grads) != len(self._grads) or not all(map(is_, grads, self._grads)):
-            seen, grads = grads, self._look_at_grads(grads)
-            self._grads = seen if all(map(is_, seen, grads)) else []
-        with torch.cuda.device(self._device):
-            self._launch(pointers, grads, max_norm)
+        self._plan.step([(*at, g["lr"], *g["betas"], g["eps"], g["weight_decay"], g["decoupled"])
+                         for at, g in zip(self._groups, self.param_groups)], max_norm or 0.0)
         return loss
-
-    def _launch(self, pointers, grads, max_norm):
-        L, params = _lib.lib(), self._params
-        stream = torch.cuda.current_stream(self._device).cuda_stream
-        sizes = [p.numel() for p in params]
-        use = [i for i, g in enumerate(grads) if g is not None and sizes[i]]
-        if not use:
-            return
-        g_ptr = [0 if g is None else g.data_ptr() for g in grads]
-
-        def table(code, values):
-            a = array.array(code, values)
-            return a, a.buffer_info()[0]
-        scratch = torch.empty(4 + 3 * len(params), dtype=torch.float32, device=self._device)
-        partials = None
-        if max_norm is not None:
-            partials = torch.empty(self._partials, dtype=torch.float64, device=self._device)
-            (a, a_at), (b, b_at) = table("Q", [g_ptr[i] for i in use]), table("q", [sizes[i] for i in use])
-            n_partials = sum(-(-sizes[i] // _CHUNK) for i in use)
-            _lib.check(L.az_grad_sumsq(len(use), a_at, b_at, partials.data_ptr(), n_partials, stream))
-        flat = self._flat
-        moments = (flat["exp_avg"], flat["exp_avg_sq"], None, None) if self.state_bits == 32 else (
-            flat["exp_avg"], flat["exp_rms"], flat["exp_avg_scale"], flat["exp_rms_scale"])
-        changed = []
-        for group, members in zip(self.param_groups, self._groups):
-            mine = [i for i in use if i in members]
-            if not mine:
-                continue
-            cfg = _lib.AdamConfig(
-                group["lr"], *group["betas"], group["eps"], group["weight_decay"], max_norm or 0.0, int(group["decoupled"]),
-                self.state_bits, self.seed & 0xFFFFFFFF, self._capacity, 0 if partials is None else n_partials, len(params),
-                *(None if t is None else t.data_ptr() for t in moments), self._step.data_ptr(),
-                None if partials is None else partials.data_ptr(), self.grad_norm.data_ptr() if partials is not None else None,
-                scratch.data_ptr())
-            tables = [table("Q", [pointers[i] for i in mine]), table("Q", [g_ptr[i] for i in mine]), table("q", [sizes[i] for i in mine]),
-                      table("q", [self._offsets[i] for i in mine]), table("i", mine)]
-            _lib.check(L.az_adam_step(C.byref(cfg), len(mine), *(at for _, at in tables), stream))
-            changed += [params[i] for i in mine]
-        if self.state_bits == 32:
-            changed += list(flat.values())
-        # written behind torch's back: whoever watches version counters has to see it
-        torch.autograd.graph.increment_version(changed + [self._step])
