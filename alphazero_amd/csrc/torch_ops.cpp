@@ -51,7 +51,6 @@ void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t
 template <typename T>
 T* ptr(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
 
-std::string shape(const Tensor& t) { return c10::str(t.sizes()); }
 
 int dtype_code(const Tensor& t) {
     switch (t.scalar_type()) {

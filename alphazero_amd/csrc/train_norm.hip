@@ -47,17 +47,20 @@ struct NormParams {
     float *m2, *A, *B;                       // [n][c]; A, B per row if gated, per channel if plain
     // backward workspace
     float *s1, *s2, *de, *dh, *dq, *ca, *cb, *cd;   // [n][c] x 2, [n][2c], [n][hidden], [n][c]; per channel
+    float* partial;                          // [splits][tiles][TILE_OUT]
     float *dweight, *dbias, *dw1, *db1, *dw2, *db2;
 };
 
 __device__ inline float not_below_zero(float v) { return v < 0.f ? 0.f : v; }     // a NaN stays one
 
+__device__ void join_weights(const NormParams& p, int block);
+
 // ---------------------------------------------------------------------------- [n][c][hw]: L lanes to a row
 constexpr int ROWS_AT_ONCE = 4;              // rows per group of lanes: that many loads in flight
 
 template <int L>
-__device__ inline uint32_t row_of(int k) {
-    return (blockIdx.x * ROWS_AT_ONCE + k) * (NORM_THREADS / L) + threadIdx.x / L;
+__device__ inline uint32_t row_of(int k, uint32_t block = blockIdx.x) {
+    return (block * ROWS_AT_ONCE + k) * (NORM_THREADS / L) + threadIdx.x / L;
 }
 
 template <typename T, int L>
@@ -162,12 +165,16 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_sums(const T* __restr
 // grad: the masked one (dresidual) if gated
 template <typename T, int L, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_apply(const T* __restrict__ x, const T* __restrict__ grad,
-                                                                 T* __restrict__ dx, const NormParams p) {
+                                                                 T* __restrict__ dx, const NormParams p, uint32_t joins) {
     constexpr int V = Pack<T>::V;
+    if (GATED && blockIdx.x < joins) {
+        join_weights(p, blockIdx.x);
+        return;
+    }
     const int lane = threadIdx.x % L;
 #pragma unroll
     for (int k = 0; k < ROWS_AT_ONCE; ++k) {
-        const uint32_t row = row_of<L>(k);
+        const uint32_t row = row_of<L>(k, blockIdx.x - joins);
         if (row >= p.rows) continue;
         const size_t at = (size_t)row * p.hw;
         const uint32_t c = row % (uint32_t)p.c;
@@ -331,13 +338,18 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_sums(const T* __rest
 
 template <typename T, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_apply(const T* __restrict__ x, const T* __restrict__ grad,
-                                                                  T* __restrict__ dx, const NormParams p, int wide) {
+                                                                  T* __restrict__ dx, const NormParams p, int wide, uint32_t joins) {
     constexpr int V = Pack<T>::V;
     typedef typename Pack<T>::f32 F;
+    if (GATED && blockIdx.x < joins) {
+        if (blockIdx.y == 0) join_weights(p, blockIdx.x);
+        return;
+    }
+    const uint32_t n = blockIdx.x - joins;
     const Lanes l = lanes_of<T>(p, wide);
     if (!l.on) return;
     F mean, a, b, d;
-    const size_t row = (size_t)blockIdx.x * p.c + l.c;
+    const size_t row = (size_t)n * p.c + l.c;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int c = i < l.left ? l.c + i : 0;
@@ -350,7 +362,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_apply(const T* __res
             a[i] *= p.gate[row + i];
         }
     }
-    const size_t board = (size_t)blockIdx.x * p.hw;
+    const size_t board = (size_t)n * p.hw;
     for (int y = l.ty; y < p.hw; y += l.step) {
         const size_t at = (board + y) * p.c + l.c;
         const F v = load_pack(x + at, l.left);
@@ -366,7 +378,8 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_apply(const T* __res
 }
 
 // ------------------------------------------------------------------- per channel: sums over the boards in 64 bits
-constexpr int CHANNELS = 8, BOARDS = 128;     // a workgroup: 8 neighbouring channels (32 bytes), 128 boards at a time
+constexpr int CHANNELS = 4, BOARDS = 128;     // a workgroup: 4 neighbouring channels, 128 boards at a time
+constexpr int IN_FLIGHT = 8;                  // boards whose loads a thread has under way
 
 template <int K>
 __device__ inline void add_boards(double (&v)[K]) {
@@ -390,11 +403,22 @@ __global__ __launch_bounds__(CHANNELS * BOARDS) void k_channel_stats(const NormP
     double v[3] = {0, 0, 0};          // sum of board means, of their squares, of centred sums
     if (p.training) {
         if (c < p.c)
-            for (int64_t i = b; i < p.n; i += BOARDS) {
-                const double m = p.board_mean[i * p.c + c];
-                v[0] += m;
-                v[1] += m * m;
-                v[2] += p.m2[i * p.c + c];
+            for (int64_t i = b; i < p.n; i += BOARDS * IN_FLIGHT) {
+                float mean[IN_FLIGHT], m2[IN_FLIGHT];
+#pragma unroll
+                for (int u = 0; u < IN_FLIGHT; ++u) {
+                    const int64_t iu = i + u * BOARDS, row = (iu < p.n ? iu : i) * p.c + c;
+                    mean[u] = p.board_mean[row];
+                    m2[u] = p.m2[row];
+                }
+#pragma unroll
+                for (int u = 0; u < IN_FLIGHT; ++u)
+                    if (i + u * BOARDS < p.n) {
+                        const double m = mean[u];
+                        v[0] += m;
+                        v[1] += m * m;
+                        v[2] += m2[u];
+                    }
             }
         add_boards(v);
     }
@@ -428,16 +452,29 @@ __device__ inline void channel_grads(const NormParams& p, int block) {
     double v[2] = {0, 0};
     if (c < p.c) {
         const float mean = p.mean[c];
-        for (int64_t i = b; i < p.n; i += BOARDS) {
-            const int64_t row = i * p.c + c;
-            if (p.hidden) {
-                const float gate = p.gate[row], dq = p.dq[row];
-                v[0] += (double)(gate * p.s1[row] + dq);
-                v[1] += (double)(gate * p.s2[row] + dq * (p.board_mean[row] - mean));
-            } else {
-                v[0] += p.s1[row];
-                v[1] += p.s2[row];
+        for (int64_t i = b; i < p.n; i += BOARDS * IN_FLIGHT) {
+            float s1[IN_FLIGHT], s2[IN_FLIGHT], gate[IN_FLIGHT], dq[IN_FLIGHT], bm[IN_FLIGHT];
+#pragma unroll
+            for (int u = 0; u < IN_FLIGHT; ++u) {
+                const int64_t iu = i + u * BOARDS, row = (iu < p.n ? iu : i) * p.c + c;
+                s1[u] = p.s1[row];
+                s2[u] = p.s2[row];
+                if (p.hidden) {
+                    gate[u] = p.gate[row];
+                    dq[u] = p.dq[row];
+                    bm[u] = p.board_mean[row];
+                }
             }
+#pragma unroll
+            for (int u = 0; u < IN_FLIGHT; ++u)
+                if (i + u * BOARDS < p.n) {
+                    if (p.hidden) {
+                        s1[u] = gate[u] * s1[u] + dq[u];
+                        s2[u] = gate[u] * s2[u] + dq[u] * (bm[u] - mean);
+                    }
+                    v[0] += s1[u];
+                    v[1] += s2[u];
+                }
         }
     }
     add_boards(v);
@@ -558,60 +595,109 @@ __global__ __launch_bounds__(256) void k_gate_backward(const NormParams p) {
     }
 }
 
-// Gradients of the gate's weights: sums over the boards of outer products, as 32 x 32 tiles.  A wavefront takes every
-// 16th board, a lane 4 x 4 of the tile; the 16 partial tiles are added in order.  The bias is one more column, of ones.
-constexpr int TILE = 32, TILE_WAVES = 16;
+// Gradients of the gate's weights: sums over the boards of outer products, as 32 x 32 tiles.  A workgroup takes one tile and
+// one of `splits` ranges of boards, each of its wavefronts every eighth board, a lane 4 x 4 of the tile, four boards' loads
+// in flight.  The bias is the sum of the left factor.  The partial tiles go to the workspace; the last pass's first
+// workgroups add them in order, beside its own work.
+// (One workgroup per tile over all boards, one board in flight, took 62 us at 1024 x 128 and 230 us at 4096 x 256: four times
+// the pass over the activations that follows.)
+constexpr int TILE = 32, TILE_WAVES = CHANNELS * BOARDS / 64, TILE_BOARDS = 4, TILE_OUT = TILE * TILE + TILE;
 
-__device__ inline void weight_tile(const NormParams& p, int tile, float* lds) {
-    const int t2 = (2 * p.c + TILE - 1) / TILE * ((p.hidden + TILE) / TILE);
-    const bool second = tile < t2;                                   // fc2: [2c][hidden + 1], fc1: [hidden][c + 1]
-    const int m = second ? 2 * p.c : p.hidden, k = second ? p.hidden : p.c;
-    if (!second) tile -= t2;
-    const int across = (k + TILE) / TILE, i0 = tile / across * TILE, j0 = tile % across * TILE;
+struct TileShape {
+    int m, k, across, tiles;                                         // [m][k] in `tiles` tiles, `across` to a row
+};
+
+__host__ __device__ inline TileShape tile_shape(int m, int k) {
+    const int across = (k + TILE - 1) / TILE;
+    return {m, k, across, (m + TILE - 1) / TILE * across};
+}
+
+__host__ __device__ inline int weight_tiles(const NormParams& p) { return tile_shape(2 * p.c, p.hidden).tiles + tile_shape(p.hidden, p.c).tiles; }
+
+// Ranges of at least 64 boards (two rounds of a wavefront), and no more than fill the chip a few times.
+__host__ __device__ inline int weight_splits(const NormParams& p) {
+    const int64_t most = (p.n + 63) / 64, enough = 2048 / weight_tiles(p);
+    return (int)(enough < 1 ? 1 : most < enough ? most : enough);
+}
+
+__device__ inline void weight_tile(const NormParams& p, int job) {
+    __shared__ float lds[TILE_WAVES][TILE_OUT];
+    const int tiles = weight_tiles(p), splits = weight_splits(p), split = job / tiles;
+    int tile = job % tiles;
+    const TileShape fc2 = tile_shape(2 * p.c, p.hidden), fc1 = tile_shape(p.hidden, p.c);
+    const bool second = tile < fc2.tiles;
+    const TileShape t = second ? fc2 : fc1;
+    if (!second) tile -= fc2.tiles;
+    const int i0 = tile / t.across * TILE, j0 = tile % t.across * TILE;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = i0 + lane / 8 * 4, lj = j0 + lane % 8 * 4;
-    float acc[4][4] = {};
-    float scale[4], shift[4];
-    if (!second)
+    const float *left = second ? p.de : p.dh, *right = second ? p.h : p.board_mean;
+    f32x4 acc[4], bias, scale, shift;                                // fc1's right factor: q = mean * scale + shift
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {                                // q = mean * scale + shift
-            const int c = lj + j < k ? lj + j : 0;
-            scale[j] = p.weight[c] * p.inv[c];
-            shift[j] = p.bias[c] - scale[j] * p.mean[c];
+    for (int j = 0; j < 4; ++j) {
+        acc[j] = 0.f;
+        bias[j] = 0.f;
+        const int c = lj + j < t.k ? lj + j : 0;
+        scale[j] = second ? 1.f : p.weight[c] * p.inv[c];
+        shift[j] = second ? 0.f : p.bias[c] - scale[j] * p.mean[c];
+    }
+    const int64_t from = p.n * split / splits, to = p.n * (split + 1) / splits;
+    for (int64_t n = from + wave; n < to; n += TILE_WAVES * TILE_BOARDS) {
+        f32x4 a[TILE_BOARDS], b[TILE_BOARDS];
+#pragma unroll
+        for (int u = 0; u < TILE_BOARDS; ++u) {
+            const int64_t nu = n + u * TILE_WAVES;
+            const bool in = nu < to;
+            a[u] = load_pack(left + (in ? nu : n) * t.m + li, in ? t.m - li : 0);
+            b[u] = load_pack(right + (in ? nu : n) * t.k + lj, t.k - lj);
         }
-    for (int64_t n = wave; n < p.n; n += TILE_WAVES) {
-        float a[4], b[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a[i] = li + i < m ? (second ? p.de[n * m + li + i] : p.dh[n * m + li + i]) : 0.f;
-            const bool in = lj + i < k;
-            const float v = in ? (second ? p.h[n * k + lj + i] : p.board_mean[n * k + lj + i]) : 0.f;
-            b[i] = in ? (second ? v : v * scale[i] + shift[i]) : lj + i == k ? 1.f : 0.f;
+        for (int u = 0; u < TILE_BOARDS; ++u) {
+            const f32x4 q = b[u] * scale + shift;
+            bias += a[u];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] += a[u][i] * q;
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] += a[i] * b[j];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) lds[wave * TILE * TILE + (lane / 8 * 4 + i) * TILE + lane % 8 * 4 + j] = acc[i][j];
+    for (int i = 0; i < 4; ++i) *(f32x4*)&lds[wave][(lane / 8 * 4 + i) * TILE + lane % 8 * 4] = acc[i];
+    if (lane % 8 == 0) *(f32x4*)&lds[wave][TILE * TILE + lane / 8 * 4] = bias;
     __syncthreads();
-    const int i = i0 + threadIdx.x / TILE, j = j0 + threadIdx.x % TILE;
+    float* out = p.partial + ((size_t)split * tiles + job % tiles) * TILE_OUT;
+    for (int o = threadIdx.x; o < TILE_OUT; o += TILE_WAVES * 64) {
+        float s = lds[0][o];
+        for (int w = 1; w < TILE_WAVES; ++w) s += lds[w][o];
+        out[o] = s;
+    }
+}
+
+// One output per thread: the partial tiles in order.
+__device__ void join_weights(const NormParams& p, int block) {
+    const int tiles = weight_tiles(p), splits = weight_splits(p);
+    const int o = block * NORM_THREADS + threadIdx.x;
+    if (o >= tiles * TILE_OUT) return;
     float s = 0.f;
-    for (int w = 0; w < TILE_WAVES; ++w) s += lds[w * TILE * TILE + threadIdx.x];
-    if (i < m && j < k) (second ? p.dw2 : p.dw1)[(size_t)i * k + j] = s;
-    if (i < m && j == k) (second ? p.db2 : p.db1)[i] = s;
+    for (int i = 0; i < splits; ++i) s += p.partial[(size_t)i * tiles * TILE_OUT + o];
+    int tile = o / TILE_OUT;
+    const int at = o % TILE_OUT;
+    const TileShape fc2 = tile_shape(2 * p.c, p.hidden), fc1 = tile_shape(p.hidden, p.c);
+    const bool second = tile < fc2.tiles;
+    const TileShape t = second ? fc2 : fc1;
+    if (!second) tile -= fc2.tiles;
+    const int i0 = tile / t.across * TILE, j0 = tile % t.across * TILE;
+    if (at < TILE * TILE) {
+        const int i = i0 + at / TILE, j = j0 + at % TILE;
+        if (i < t.m && j < t.k) (second ? p.dw2 : p.dw1)[(size_t)i * t.k + j] = s;
+    } else {
+        const int i = i0 + at - TILE * TILE;
+        if (i < t.m && j0 == 0) (second ? p.db2 : p.db1)[i] = s;
+    }
 }
 
-__global__ __launch_bounds__(1024) void k_param_grads(const NormParams p, int channel_blocks) {
-    extern __shared__ float lds[];
+static int join_blocks(const NormParams& p) { return p.hidden ? (weight_tiles(p) * TILE_OUT + NORM_THREADS - 1) / NORM_THREADS : 0; }
+
+__global__ __launch_bounds__(CHANNELS * BOARDS) void k_param_grads(const NormParams p, int channel_blocks) {
     if ((int)blockIdx.x < channel_blocks) channel_grads(p, blockIdx.x);
-    else weight_tile(p, (int)blockIdx.x - channel_blocks, lds);
-}
-
-static int weight_tiles(const NormParams& p) {
-    return (2 * p.c + TILE - 1) / TILE * ((p.hidden + TILE) / TILE) + (p.hidden + TILE - 1) / TILE * ((p.c + TILE) / TILE);
+    else weight_tile(p, (int)blockIdx.x - channel_blocks);
 }
 
 // ---------------------------------------------------------------------------------------------- host side
@@ -686,20 +772,21 @@ static int norm_backward(const NormParams& p, bool last, const void* x, const vo
         AZ_HIP(hipGetLastError());
     }
     const int cb = (p.c + CHANNELS - 1) / CHANNELS;
-    hipLaunchKernelGGL(k_param_grads, dim3(cb + (p.hidden ? weight_tiles(p) : 0)), dim3(1024),
-                       p.hidden ? sizeof(float) * TILE_WAVES * TILE * TILE : 0, s, p, cb);
+    hipLaunchKernelGGL(k_param_grads, dim3(cb + (p.hidden ? weight_tiles(p) * weight_splits(p) : 0)), dim3(CHANNELS * BOARDS), 0, s, p, cb);
     AZ_HIP(hipGetLastError());
     const T* mt = p.hidden ? rt : gt;
+    const uint32_t joins = (uint32_t)join_blocks(p);
     if (last) {
-        if (p.hidden) hipLaunchKernelGGL((k_last_grad_apply<T, true>), boards, block, 0, s, xt, mt, dt, p, wide);
-        else hipLaunchKernelGGL((k_last_grad_apply<T, false>), boards, block, 0, s, xt, mt, dt, p, wide);
+        const dim3 grid(boards.x + joins, boards.y);
+        if (p.hidden) hipLaunchKernelGGL((k_last_grad_apply<T, true>), grid, block, 0, s, xt, mt, dt, p, wide, joins);
+        else hipLaunchKernelGGL((k_last_grad_apply<T, false>), grid, block, 0, s, xt, mt, dt, p, wide, joins);
     } else {
         with_lanes(p.nvec, [&](auto L) {
             constexpr int N = decltype(L)::value;
             const uint32_t per = NORM_THREADS / N * ROWS_AT_ONCE;
-            const dim3 grid((p.rows + per - 1) / per);
-            if (p.hidden) hipLaunchKernelGGL((k_row_grad_apply<T, N, true>), grid, block, 0, s, xt, mt, dt, p);
-            else hipLaunchKernelGGL((k_row_grad_apply<T, N, false>), grid, block, 0, s, xt, mt, dt, p);
+            const dim3 grid((p.rows + per - 1) / per + joins);
+            if (p.hidden) hipLaunchKernelGGL((k_row_grad_apply<T, N, true>), grid, block, 0, s, xt, mt, dt, p, joins);
+            else hipLaunchKernelGGL((k_row_grad_apply<T, N, false>), grid, block, 0, s, xt, mt, dt, p, joins);
         });
     }
     AZ_HIP(hipGetLastError());
@@ -773,11 +860,12 @@ static int norm_params(const az_norm_args* a, NormParams* p, int64_t sizes[3]) {
     p->ca = bwd.take<float>(a->c);
     p->cb = bwd.take<float>(a->c);
     p->cd = bwd.take<float>(a->c);
-    p->de = p->dh = p->dq = nullptr;
+    p->de = p->dh = p->dq = p->partial = nullptr;
     if (a->hidden) {
         p->de = bwd.take<float>(2 * rows);
         p->dh = bwd.take<float>(hidden);
         p->dq = bwd.take<float>(rows);
+        p->partial = bwd.take<float>((size_t)weight_tiles(*p) * weight_splits(*p) * TILE_OUT);
     }
     if (sizes) {
         sizes[0] = (int64_t)saved.used;
