@@ -27,13 +27,12 @@ namespace az {
 
 constexpr int NORM_THREADS = 256;
 constexpr int GATE_ROWS = 4;                 // boards per workgroup of the gate kernels
-constexpr int NORM_MAX_GATED = 1024;         // their LDS: GATE_ROWS * (2 c + hidden) floats
+constexpr int NORM_MAX_GATED = 1024;         // their LDS: 16 (3 c + hidden) bytes forward, 16 (2 c + hidden + 1024) backward: 64 KB
 
 struct NormParams {
     int64_t n;
     int c, hw, hidden, nvec;                 // nvec: 16-byte pieces of a row (hw values, or c with channels last)
     int training;
-    uint32_t rows;                           // n * c
     double eps, momentum;
     const float *weight, *bias;
     float *running_mean, *running_var;
@@ -41,12 +40,16 @@ struct NormParams {
     const float *w1, *b1, *w2, *b2;
     // saved
     float *mean, *inv;                       // [c]
-    float *board_mean, *gate, *h;            // [n][c], [n][c], [n][hidden] (board_mean: workspace if plain)
+    float *board_mean, *gate, *h;            // gated: [n][c], [n][c], [n][hidden]
     uint8_t* mask;                           // a byte per 16 bytes of x: out > 0
+    // partial sums over chunks of boards, [chunks][c]: means and centred sums forward, dy's sums backward
+    float *part_a, *part_b;
+    int64_t chunks;
+    int chunk_boards, abreast;
     // forward workspace
-    float *m2, *A, *B;                       // [n][c]; A, B per row if gated, per channel if plain
+    float *A, *B;                            // per row if gated, per channel if plain
     // backward workspace
-    float *s1, *s2, *de, *dh, *dq, *ca, *cb, *cd;   // [n][c] x 2, [n][2c], [n][hidden], [n][c]; per channel
+    float *s1, *s2, *de, *dh, *dq, *ca, *cb, *cd;   // gated: [n][c] x 2, [n][2c], [n][hidden], [n][c]; per channel
     float* partial;                          // [splits][tiles][TILE_OUT]
     float *dweight, *dbias, *dw1, *db1, *dw2, *db2;
 };
@@ -55,26 +58,67 @@ __device__ inline float not_below_zero(float v) { return v < 0.f ? 0.f : v; }   
 
 __device__ void join_weights(const NormParams& p, int block);
 
-// ---------------------------------------------------------------------------- [n][c][hw]: L lanes to a row
-constexpr int ROWS_AT_ONCE = 4;              // rows per group of lanes: that many loads in flight
-
-template <int L>
-__device__ inline uint32_t row_of(int k, uint32_t block = blockIdx.x) {
-    return (block * ROWS_AT_ONCE + k) * (NORM_THREADS / L) + threadIdx.x / L;
+// The boards whose sums chunk i holds: p.chunk_boards of them, p.abreast apart, fewer at the end.
+__device__ inline int64_t boards_in_chunk(const NormParams& p, int64_t i) {
+    const int64_t first = i / p.abreast * p.chunk_boards * p.abreast + i % p.abreast;
+    const int64_t k = first < p.n ? (p.n - 1 - first) / p.abreast + 1 : 0;
+    return k < p.chunk_boards ? k : p.chunk_boards;
 }
 
-template <typename T, int L>
-__global__ __launch_bounds__(NORM_THREADS) void k_row_stats(const T* __restrict__ x, const NormParams p) {
+// ---------------------------------------------------------------------------- [n][c][hw]: L lanes to a row
+// A group of L lanes takes one channel and BOARDS_AT_ONCE boards: that many loads in flight, the channel's numbers loaded
+// once, and the boards' sums joined in registers before they leave (a chunk).  The groups of a workgroup lie along the
+// channels, so what it loads at once is one stretch of memory; where there are fewer channels than groups, `abreast`
+// boards lie side by side.
+constexpr int BOARDS_AT_ONCE = 4;
+
+struct RowGrid {
+    uint32_t wide, abreast, across;          // channels and boards side by side in a workgroup; workgroups to a board
+    uint32_t blocks;
+};
+
+template <int L>
+static RowGrid row_grid(const NormParams& p) {
+    const uint32_t groups = NORM_THREADS / L, c = (uint32_t)p.c;
+    RowGrid g;
+    g.wide = c < groups ? c : groups;
+    g.abreast = groups / g.wide;
+    g.across = (c + groups - 1) / groups;
+    g.blocks = (uint32_t)((p.n + BOARDS_AT_ONCE * g.abreast - 1) / (BOARDS_AT_ONCE * g.abreast)) * g.across;
+    return g;
+}
+
+struct RowPlace {
+    uint32_t c, chunk, lane;
+    int64_t first;                           // first board; the others follow `abreast` apart
+    bool on;
+};
+
+template <int L>
+__device__ inline RowPlace row_place(const NormParams& p, const RowGrid& g, uint32_t block) {
+    const uint32_t group = threadIdx.x / L, nb = block / g.across, beside = g.abreast == 1 ? 0 : group / g.wide;
+    RowPlace r;
+    r.lane = threadIdx.x % L;
+    r.c = block % g.across * (NORM_THREADS / L) + group - beside * g.wide;
+    r.chunk = nb * g.abreast + beside;
+    r.first = (int64_t)nb * BOARDS_AT_ONCE * g.abreast + beside;
+    r.on = r.c < (uint32_t)p.c && beside < g.abreast;        // (a chunk may be empty: its sums are zero)
+    return r;
+}
+
+template <typename T, int L, bool GATED>
+__global__ __launch_bounds__(NORM_THREADS) void k_row_stats(const T* __restrict__ x, const NormParams p, const RowGrid grid) {
     constexpr int V = Pack<T>::V;
-    const int lane = threadIdx.x % L;
-    float first[ROWS_AT_ONCE], s[ROWS_AT_ONCE], ss[ROWS_AT_ONCE];
+    const RowPlace r = row_place<L>(p, grid, blockIdx.x);
+    float first[BOARDS_AT_ONCE], s[BOARDS_AT_ONCE], ss[BOARDS_AT_ONCE];
 #pragma unroll
-    for (int k = 0; k < ROWS_AT_ONCE; ++k) {
-        const uint32_t row = row_of<L>(k);
-        const T* xr = x + (size_t)(row < p.rows ? row : 0) * p.hw;
+    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+        const int64_t n = r.first + k * grid.abreast;
+        first[k] = s[k] = ss[k] = 0.f;
+        if (!r.on || n >= p.n) continue;
+        const T* xr = x + (size_t)(n * p.c + r.c) * p.hw;
         first[k] = (float)xr[0];
-        s[k] = ss[k] = 0.f;
-        for (int j = lane; j < p.nvec; j += L) {
+        for (int j = r.lane; j < p.nvec; j += L) {
             const int left = p.hw - j * V;
             const auto v = load_pack(xr + j * V, left);
 #pragma unroll
@@ -85,30 +129,39 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_stats(const T* __restrict_
             }
         }
     }
+    const float hw = (float)p.hw;
+    float mean = 0.f, m2 = 0.f, boards = 0.f;
 #pragma unroll
-    for (int k = 0; k < ROWS_AT_ONCE; ++k) {
-        const uint32_t row = row_of<L>(k);
+    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+        const int64_t n = r.first + k * grid.abreast;
         const float a = lane_sum<L>(s[k]), b = lane_sum<L>(ss[k]);
-        if (lane == 0 && row < p.rows) {
-            p.board_mean[row] = first[k] + a / (float)p.hw;
-            p.m2[row] = not_below_zero(b - a * a / (float)p.hw);
-        }
+        if (!r.on || n >= p.n) continue;
+        const float board = first[k] + a / hw;
+        if (GATED && r.lane == 0) p.board_mean[n * p.c + r.c] = board;
+        boards += 1.f;                       // join this board's mean and centred sum to the chunk's
+        const float d = board - mean;
+        mean += d / boards;
+        m2 += not_below_zero(b - a * a / hw) + hw * d * (board - mean);
+    }
+    if (r.on && r.lane == 0) {
+        p.part_a[(size_t)r.chunk * p.c + r.c] = mean;
+        p.part_b[(size_t)r.chunk * p.c + r.c] = m2;
     }
 }
 
 template <typename T, int L, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_row_apply(const T* __restrict__ x, const T* __restrict__ residual,
-                                                            T* __restrict__ out, const NormParams p) {
+                                                            T* __restrict__ out, const NormParams p, const RowGrid grid) {
     constexpr int V = Pack<T>::V;
-    const int lane = threadIdx.x % L;
+    const RowPlace r = row_place<L>(p, grid, blockIdx.x);
+    if (!r.on) return;
 #pragma unroll
-    for (int k = 0; k < ROWS_AT_ONCE; ++k) {
-        const uint32_t row = row_of<L>(k);
-        if (row >= p.rows) continue;
+    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+        const int64_t n = r.first + k * grid.abreast, row = n * p.c + r.c;
+        if (n >= p.n) return;
         const size_t at = (size_t)row * p.hw;
-        const uint32_t q = GATED ? row : row % (uint32_t)p.c;
-        const float A = p.A[q], B = p.B[q];
-        for (int j = lane; j < p.nvec; j += L) {
+        const float A = p.A[GATED ? row : r.c], B = p.B[GATED ? row : r.c];
+        for (int j = r.lane; j < p.nvec; j += L) {
             const int left = p.hw - j * V;
             auto v = load_pack(x + at + j * V, left) * A + B;
             if (GATED) v += load_pack(residual + at + j * V, left);
@@ -119,25 +172,25 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_apply(const T* __restrict_
                 v[i] = not_below_zero(v[i]);
             }
             store_pack(out + at + j * V, v, left);
-            if (p.mask) p.mask[(size_t)row * p.nvec + j] = (uint8_t)bits;
+            p.mask[(size_t)row * p.nvec + j] = (uint8_t)bits;
         }
     }
 }
 
 template <typename T, int L, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_sums(const T* __restrict__ x, const T* __restrict__ grad,
-                                                                T* __restrict__ dresidual, const NormParams p) {
+                                                                T* __restrict__ dresidual, const NormParams p, const RowGrid grid) {
     constexpr int V = Pack<T>::V;
-    const int lane = threadIdx.x % L;
-    float s1[ROWS_AT_ONCE], s2[ROWS_AT_ONCE];
+    const RowPlace r = row_place<L>(p, grid, blockIdx.x);
+    const float mean = r.on ? p.mean[r.c] : 0.f;
+    float s1[BOARDS_AT_ONCE], s2[BOARDS_AT_ONCE];
 #pragma unroll
-    for (int k = 0; k < ROWS_AT_ONCE; ++k) {
-        const uint32_t row = row_of<L>(k);
+    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+        const int64_t n = r.first + k * grid.abreast, row = n * p.c + r.c;
         s1[k] = s2[k] = 0.f;
-        if (row >= p.rows) continue;
+        if (!r.on || n >= p.n) continue;
         const size_t at = (size_t)row * p.hw;
-        const float mean = p.mean[row % (uint32_t)p.c];
-        for (int j = lane; j < p.nvec; j += L) {
+        for (int j = r.lane; j < p.nvec; j += L) {
             const int left = p.hw - j * V;
             const auto v = load_pack(x + at + j * V, left);
             auto g = load_pack(grad + at + j * V, left);
@@ -151,13 +204,27 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_sums(const T* __restr
             if (GATED) store_pack(dresidual + at + j * V, g, left);
         }
     }
+    float a = 0.f, b = 0.f;
 #pragma unroll
-    for (int k = 0; k < ROWS_AT_ONCE; ++k) {
-        const uint32_t row = row_of<L>(k);
-        const float a = lane_sum<L>(s1[k]), b = lane_sum<L>(s2[k]);
-        if (lane == 0 && row < p.rows) {
-            p.s1[row] = a;
-            p.s2[row] = b;
+    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+        const int64_t n = r.first + k * grid.abreast;
+        if (GATED) {                         // the gate's gradient needs every board's
+            const float sa = lane_sum<L>(s1[k]), sb = lane_sum<L>(s2[k]);
+            if (r.on && n < p.n && r.lane == 0) {
+                p.s1[n * p.c + r.c] = sa;
+                p.s2[n * p.c + r.c] = sb;
+            }
+        } else {
+            a += s1[k];
+            b += s2[k];
+        }
+    }
+    if (!GATED) {
+        a = lane_sum<L>(a);
+        b = lane_sum<L>(b);
+        if (r.on && r.lane == 0) {
+            p.part_a[(size_t)r.chunk * p.c + r.c] = a;
+            p.part_b[(size_t)r.chunk * p.c + r.c] = b;
         }
     }
 }
@@ -165,26 +232,22 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_sums(const T* __restr
 // grad: the masked one (dresidual) if gated
 template <typename T, int L, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_apply(const T* __restrict__ x, const T* __restrict__ grad,
-                                                                 T* __restrict__ dx, const NormParams p, uint32_t joins) {
+                                                                 T* __restrict__ dx, const NormParams p, const RowGrid grid, uint32_t joins) {
     constexpr int V = Pack<T>::V;
     if (GATED && blockIdx.x < joins) {
         join_weights(p, blockIdx.x);
         return;
     }
-    const int lane = threadIdx.x % L;
+    const RowPlace r = row_place<L>(p, grid, blockIdx.x - joins);
+    if (!r.on) return;
+    const float mean = p.mean[r.c], b = p.cb[r.c], ca = p.ca[r.c], cd = p.cd[r.c], per_place = ca / (float)p.hw;
 #pragma unroll
-    for (int k = 0; k < ROWS_AT_ONCE; ++k) {
-        const uint32_t row = row_of<L>(k, blockIdx.x - joins);
-        if (row >= p.rows) continue;
+    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+        const int64_t n = r.first + k * grid.abreast, row = n * p.c + r.c;
+        if (n >= p.n) return;
         const size_t at = (size_t)row * p.hw;
-        const uint32_t c = row % (uint32_t)p.c;
-        const float mean = p.mean[c], b = p.cb[c];
-        float a = p.ca[c], d = p.cd[c];
-        if (GATED) {
-            d += a * p.dq[row] / (float)p.hw;
-            a *= p.gate[row];
-        }
-        for (int j = lane; j < p.nvec; j += L) {
+        const float a = GATED ? ca * p.gate[row] : ca, d = GATED ? cd + per_place * p.dq[row] : cd;
+        for (int j = r.lane; j < p.nvec; j += L) {
             const int left = p.hw - j * V;
             const auto v = load_pack(x + at + j * V, left);
             auto g = load_pack(grad + at + j * V, left);
@@ -200,7 +263,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_apply(const T* __rest
 }
 
 // ---------------------------------------------- [n][hw][c]: a workgroup to a board and a range of channels
-// Thread (ty, tx): 16 bytes of channels, every ty-th place of the board; the ty are added through LDS.
+// Thread (ty, tx): 16 bytes of channels, every ty-th place of the board; the ty are added through LDS.  A chunk is a board.
 struct Lanes {
     int tx, ty, step;          // step: places taken at once
     int j;                     // which 16 bytes of the channels
@@ -221,8 +284,23 @@ __device__ inline Lanes lanes_of(const NormParams& p, int wide) {
     return l;
 }
 
-template <int V, typename F>
-__device__ inline void add_places(F a, F b, const Lanes& l, int wide, float* out_a, float* out_b, int n_out) {
+// Numbers of the thread's channels, 16 bytes at a time.
+template <typename F>
+__device__ inline F load_channels(const float* p, int left) {
+    constexpr int V = sizeof(F) / 4;
+    F r;
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+        const f32x4 v = load_pack(p + i, left - i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[i + k] = v[k];
+    }
+    return r;
+}
+
+// Sums over the places; out(c, a, b) for each of the workgroup's channels.
+template <int V, typename F, typename Out>
+__device__ inline void add_places(F a, F b, const Lanes& l, const NormParams& p, int wide, Out&& out) {
     __shared__ float red[2][NORM_THREADS * V];
     if (l.ty < l.step) {
 #pragma unroll
@@ -232,47 +310,42 @@ __device__ inline void add_places(F a, F b, const Lanes& l, int wide, float* out
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < wide * V; i += NORM_THREADS) {
+    const int c0 = blockIdx.y * wide * V;
+    for (int i = threadIdx.x; i < wide * V && c0 + i < p.c; i += NORM_THREADS) {
         float s = 0.f, ss = 0.f;
         for (int y = 0; y < l.step; ++y) {
             s += red[0][y * wide * V + i];
             ss += red[1][y * wide * V + i];
         }
-        if (i < n_out) {
-            out_a[i] = s;
-            out_b[i] = ss;
-        }
+        out(c0 + i, s, ss);
     }
 }
 
-template <typename T>
+template <typename T, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_last_stats(const T* __restrict__ x, const NormParams p, int wide) {
     constexpr int V = Pack<T>::V;
     typedef typename Pack<T>::f32 F;
     const Lanes l = lanes_of<T>(p, wide);
     const T* xb = x + (size_t)blockIdx.x * p.hw * p.c;
-    F s, ss, first;
+    F s, ss;
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] = ss[i] = 0.f;
     if (l.on) {
-        first = load_pack(xb + l.c, l.left);
+        const F first = load_pack(xb + l.c, l.left);
+#pragma unroll 4
         for (int y = l.ty; y < p.hw; y += l.step) {
             const F d = load_pack(xb + (size_t)y * p.c + l.c, l.left) - first;
             s += d;
             ss += d * d;
         }
     }
-    const int c0 = blockIdx.y * wide * V;
-    float* mean = p.board_mean + (size_t)blockIdx.x * p.c + c0;
-    float* m2 = p.m2 + (size_t)blockIdx.x * p.c + c0;
-    const int n_out = p.c - c0;
-    add_places<V>(s, ss, l, wide, mean, m2, n_out);
-    // the same threads that wrote the sums turn them into the mean and the centred sum
-    for (int i = threadIdx.x; i < wide * V && i < n_out; i += NORM_THREADS) {
-        const float a = mean[i], b = m2[i];
-        mean[i] = (float)xb[c0 + i] + a / (float)p.hw;
-        m2[i] = not_below_zero(b - a * a / (float)p.hw);
-    }
+    add_places<V>(s, ss, l, p, wide, [&](int c, float a, float b) {
+        const float mean = (float)xb[c] + a / (float)p.hw;
+        const size_t row = (size_t)blockIdx.x * p.c + c;
+        if (GATED) p.board_mean[row] = mean;
+        p.part_a[row] = mean;
+        p.part_b[row] = not_below_zero(b - a * a / (float)p.hw);
+    });
 }
 
 template <typename T, bool GATED>
@@ -282,14 +355,10 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_apply(const T* __restrict
     typedef typename Pack<T>::f32 F;
     const Lanes l = lanes_of<T>(p, wide);
     if (!l.on) return;
-    F A, B;
     const size_t q = (GATED ? (size_t)blockIdx.x * p.c : 0) + l.c;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        A[i] = i < l.left ? p.A[q + i] : 0.f;
-        B[i] = i < l.left ? p.B[q + i] : 0.f;
-    }
+    const F A = load_channels<F>(p.A + q, l.left), B = load_channels<F>(p.B + q, l.left);
     const size_t board = (size_t)blockIdx.x * p.hw;
+#pragma unroll 4
     for (int y = l.ty; y < p.hw; y += l.step) {
         const size_t at = (board + y) * p.c + l.c;
         F v = load_pack(x + at, l.left) * A + B;
@@ -301,7 +370,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_apply(const T* __restrict
             v[i] = not_below_zero(v[i]);
         }
         store_pack(out + at, v, l.left);
-        if (p.mask) p.mask[(board + y) * p.nvec + l.j] = (uint8_t)bits;
+        p.mask[(board + y) * p.nvec + l.j] = (uint8_t)bits;
     }
 }
 
@@ -311,14 +380,13 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_sums(const T* __rest
     constexpr int V = Pack<T>::V;
     typedef typename Pack<T>::f32 F;
     const Lanes l = lanes_of<T>(p, wide);
-    F s1, s2, mean;
+    F s1, s2;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        s1[i] = s2[i] = 0.f;
-        mean[i] = l.on && i < l.left ? p.mean[l.c + i] : 0.f;
-    }
+    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
     const size_t board = (size_t)blockIdx.x * p.hw;
-    if (l.on)
+    if (l.on) {
+        const F mean = load_channels<F>(p.mean + l.c, l.left);
+#pragma unroll 4
         for (int y = l.ty; y < p.hw; y += l.step) {
             const size_t at = (board + y) * p.c + l.c;
             const F v = load_pack(x + at, l.left);
@@ -332,8 +400,12 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_sums(const T* __rest
             }
             if (GATED) store_pack(dresidual + at, g, l.left);
         }
-    const int c0 = blockIdx.y * wide * V;
-    add_places<V>(s1, s2, l, wide, p.s1 + (size_t)blockIdx.x * p.c + c0, p.s2 + (size_t)blockIdx.x * p.c + c0, p.c - c0);
+    }
+    float *a = GATED ? p.s1 : p.part_a, *b = GATED ? p.s2 : p.part_b;
+    add_places<V>(s1, s2, l, p, wide, [&](int c, float u, float v) {
+        a[(size_t)blockIdx.x * p.c + c] = u;
+        b[(size_t)blockIdx.x * p.c + c] = v;
+    });
 }
 
 template <typename T, bool GATED>
@@ -348,21 +420,15 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_apply(const T* __res
     const uint32_t n = blockIdx.x - joins;
     const Lanes l = lanes_of<T>(p, wide);
     if (!l.on) return;
-    F mean, a, b, d;
     const size_t row = (size_t)n * p.c + l.c;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int c = i < l.left ? l.c + i : 0;
-        mean[i] = p.mean[c];
-        a[i] = p.ca[c];
-        b[i] = p.cb[c];
-        d[i] = p.cd[c];
-        if (GATED && i < l.left) {
-            d[i] += a[i] * p.dq[row + i] / (float)p.hw;
-            a[i] *= p.gate[row + i];
-        }
+    const F mean = load_channels<F>(p.mean + l.c, l.left), b = load_channels<F>(p.cb + l.c, l.left);
+    F a = load_channels<F>(p.ca + l.c, l.left), d = load_channels<F>(p.cd + l.c, l.left);
+    if (GATED) {
+        d += a * load_channels<F>(p.dq + row, l.left) / (float)p.hw;
+        a *= load_channels<F>(p.gate + row, l.left);
     }
     const size_t board = (size_t)n * p.hw;
+#pragma unroll 4
     for (int y = l.ty; y < p.hw; y += l.step) {
         const size_t at = (board + y) * p.c + l.c;
         const F v = load_pack(x + at, l.left);
@@ -377,70 +443,85 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_apply(const T* __res
     }
 }
 
-// ------------------------------------------------------------------- per channel: sums over the boards in 64 bits
-constexpr int CHANNELS = 4, BOARDS = 128;     // a workgroup: 4 neighbouring channels, 128 boards at a time
-constexpr int IN_FLIGHT = 8;                  // boards whose loads a thread has under way
+// ------------------------------------------------------------ per channel: sums over chunks of boards in 64 bits
+constexpr int CHANNELS = 8, LINES = 64;       // a workgroup: 8 neighbouring channels, 64 chunks at a time
+constexpr int IN_FLIGHT = 4;                  // chunks whose loads a thread has under way
 
+// Sums of v over the threads of a channel; thread 0 to CHANNELS - 1 get theirs.
 template <int K>
-__device__ inline void add_boards(double (&v)[K]) {
-    __shared__ double red[BOARDS][CHANNELS][K];
-    const int ch = threadIdx.x % CHANNELS, b = threadIdx.x / CHANNELS;
+__device__ inline void add_lines(double (&v)[K]) {
+    __shared__ double red[CHANNELS * LINES / 64][CHANNELS][K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) red[b][ch][k] = v[k];
-    for (int half = BOARDS / 2; half; half >>= 1) {
-        __syncthreads();
-        if (b < half)
+    for (int k = 0; k < K; ++k)
+        for (int off = CHANNELS; off < 64; off <<= 1) v[k] += __shfl_xor(v[k], off);
+    const int lane = threadIdx.x & 63;
+    if (lane < CHANNELS)
 #pragma unroll
-            for (int k = 0; k < K; ++k) red[b][ch][k] += red[b + half][ch][k];
-    }
-    if (b == 0)
+        for (int k = 0; k < K; ++k) red[threadIdx.x >> 6][lane][k] = v[k];
+    __syncthreads();
+    if (threadIdx.x < CHANNELS)
 #pragma unroll
-        for (int k = 0; k < K; ++k) v[k] = red[0][ch][k];
+        for (int k = 0; k < K; ++k)
+            for (int w = 1; w < CHANNELS * LINES / 64; ++w) v[k] += red[w][threadIdx.x][k];
 }
 
-__global__ __launch_bounds__(CHANNELS * BOARDS) void k_channel_stats(const NormParams p) {
-    const int c = blockIdx.x * CHANNELS + threadIdx.x % CHANNELS, b = threadIdx.x / CHANNELS;
-    double v[3] = {0, 0, 0};          // sum of board means, of their squares, of centred sums
-    if (p.training) {
-        if (c < p.c)
-            for (int64_t i = b; i < p.n; i += BOARDS * IN_FLIGHT) {
-                float mean[IN_FLIGHT], m2[IN_FLIGHT];
+// term(i, a, b) for every chunk i of the thread's channel c.
+template <typename F>
+__device__ inline void over_chunks(const NormParams& p, int c, F&& term) {
+    if (c >= p.c) return;
+    for (int64_t i = threadIdx.x / CHANNELS; i < p.chunks; i += LINES * IN_FLIGHT) {
+        float a[IN_FLIGHT], b[IN_FLIGHT];
 #pragma unroll
-                for (int u = 0; u < IN_FLIGHT; ++u) {
-                    const int64_t iu = i + u * BOARDS, row = (iu < p.n ? iu : i) * p.c + c;
-                    mean[u] = p.board_mean[row];
-                    m2[u] = p.m2[row];
-                }
+        for (int u = 0; u < IN_FLIGHT; ++u) {
+            const int64_t iu = i + u * LINES, at = (iu < p.chunks ? iu : i) * p.c + c;
+            a[u] = p.part_a[at];
+            b[u] = p.part_b[at];
+        }
 #pragma unroll
-                for (int u = 0; u < IN_FLIGHT; ++u)
-                    if (i + u * BOARDS < p.n) {
-                        const double m = mean[u];
-                        v[0] += m;
-                        v[1] += m * m;
-                        v[2] += m2[u];
-                    }
-            }
-        add_boards(v);
+        for (int u = 0; u < IN_FLIGHT; ++u)
+            if (i + u * LINES < p.chunks) term(i + u * LINES, a[u], b[u]);
     }
-    if (b == 0 && c < p.c) {
+}
+
+__global__ __launch_bounds__(CHANNELS * LINES) void k_channel_stats(const NormParams p) {
+    const int c = blockIdx.x * CHANNELS + threadIdx.x % CHANNELS;
+    const bool mine = threadIdx.x < CHANNELS && c < p.c;
+    float old_mean = 0.f, old_var = 0.f, weight = 0.f, bias = 0.f;
+    if (mine) {                       // under way during the sums
+        if (p.running_mean) old_mean = p.running_mean[c];
+        if (p.running_var) old_var = p.running_var[c];
+        weight = p.weight[c];
+        bias = p.bias[c];
+    }
+    double v[3] = {0, 0, 0};          // sums over the boards: of their means, of the means' squares, of the centred sums
+    if (p.training) {
+        over_chunks(p, c, [&](int64_t i, float mean, float m2) {
+            const double k = (double)boards_in_chunk(p, i), m = mean;
+            v[0] += k * m;
+            v[1] += k * (m * m);
+            v[2] += m2;
+        });
+        add_lines(v);
+    }
+    if (mine) {
         double mean, var;
         if (p.training) {
             const double count = (double)p.n * p.hw;
             mean = v[0] / p.n;
             var = (v[2] + p.hw * (v[1] - p.n * mean * mean)) / count;
             if (var < 0.0) var = 0.0;          // a NaN stays one
-            if (p.running_mean) p.running_mean[c] = (float)((1.0 - p.momentum) * p.running_mean[c] + p.momentum * mean);
-            if (p.running_var) p.running_var[c] = (float)((1.0 - p.momentum) * p.running_var[c] + p.momentum * var * count / (count - 1.0));
+            if (p.running_mean) p.running_mean[c] = (float)((1.0 - p.momentum) * old_mean + p.momentum * mean);
+            if (p.running_var) p.running_var[c] = (float)((1.0 - p.momentum) * old_var + p.momentum * var * count / (count - 1.0));
         } else {
-            mean = p.running_mean[c];
-            var = p.running_var[c];
+            mean = old_mean;
+            var = old_var;
         }
         const float inv = (float)(1.0 / sqrt(var + p.eps)), m = (float)mean;
         p.mean[c] = m;
         p.inv[c] = inv;
         if (!p.hidden) {
-            p.A[c] = p.weight[c] * inv;
-            p.B[c] = p.bias[c] - p.weight[c] * inv * m;
+            p.A[c] = weight * inv;
+            p.B[c] = bias - weight * inv * m;
         }
     }
     if (p.num_batches && p.training && blockIdx.x == 0 && threadIdx.x == 0) *p.num_batches += 1;
@@ -448,38 +529,16 @@ __global__ __launch_bounds__(CHANNELS * BOARDS) void k_channel_stats(const NormP
 
 // dy's channel sums, and with them what the last pass needs: dx = ca gm (gate) + (x - mean) cb + cd (+ ca dq / hw)
 __device__ inline void channel_grads(const NormParams& p, int block) {
-    const int c = block * CHANNELS + threadIdx.x % CHANNELS, b = threadIdx.x / CHANNELS;
+    const int c = block * CHANNELS + threadIdx.x % CHANNELS;
+    const bool mine = threadIdx.x < CHANNELS && c < p.c;
+    const float inv = mine ? p.inv[c] : 0.f, a = mine ? p.weight[c] * inv : 0.f;
     double v[2] = {0, 0};
-    if (c < p.c) {
-        const float mean = p.mean[c];
-        for (int64_t i = b; i < p.n; i += BOARDS * IN_FLIGHT) {
-            float s1[IN_FLIGHT], s2[IN_FLIGHT], gate[IN_FLIGHT], dq[IN_FLIGHT], bm[IN_FLIGHT];
-#pragma unroll
-            for (int u = 0; u < IN_FLIGHT; ++u) {
-                const int64_t iu = i + u * BOARDS, row = (iu < p.n ? iu : i) * p.c + c;
-                s1[u] = p.s1[row];
-                s2[u] = p.s2[row];
-                if (p.hidden) {
-                    gate[u] = p.gate[row];
-                    dq[u] = p.dq[row];
-                    bm[u] = p.board_mean[row];
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < IN_FLIGHT; ++u)
-                if (i + u * BOARDS < p.n) {
-                    if (p.hidden) {
-                        s1[u] = gate[u] * s1[u] + dq[u];
-                        s2[u] = gate[u] * s2[u] + dq[u] * (bm[u] - mean);
-                    }
-                    v[0] += s1[u];
-                    v[1] += s2[u];
-                }
-        }
-    }
-    add_boards(v);
-    if (b == 0 && c < p.c) {
-        const float inv = p.inv[c], a = p.weight[c] * inv;
+    over_chunks(p, c, [&](int64_t, float s1, float s2) {
+        v[0] += s1;
+        v[1] += s2;
+    });
+    add_lines(v);
+    if (mine) {
         const double count = (double)p.n * p.hw;
         p.dbias[c] = (float)v[0];
         p.dweight[c] = (float)(v[1] * inv);
@@ -490,46 +549,96 @@ __device__ inline void channel_grads(const NormParams& p, int block) {
 }
 
 // --------------------------------------------------------------------------------------------- the gate
-__global__ __launch_bounds__(256) void k_gate_forward(const NormParams p) {
-    extern __shared__ float lds[];
-    float* q = lds;                                  // [GATE_ROWS][c]
-    float* h = lds + GATE_ROWS * p.c;                // [GATE_ROWS][hidden]
-    const int64_t n0 = (int64_t)blockIdx.x * GATE_ROWS;
-    const int rows = (int)(p.n - n0 < GATE_ROWS ? p.n - n0 : GATE_ROWS);
-    for (int i = threadIdx.x; i < GATE_ROWS * p.c; i += 256) {
-        const int c = i % p.c;
-        q[i] = i / p.c < rows ? (p.board_mean[n0 * p.c + i] - p.mean[c]) * (p.weight[c] * p.inv[c]) + p.bias[c] : 0.f;
-    }
-    __syncthreads();
-    // four lanes to a hidden unit of a board
-    for (int o = threadIdx.x / 4; o < GATE_ROWS * p.hidden; o += 64) {
-        const int r = o / p.hidden, k = o % p.hidden;
-        float s = 0.f;
-        for (int c = threadIdx.x % 4; c < p.c; c += 4) s += p.w1[(size_t)k * p.c + c] * q[r * p.c + c];
-        s = lane_sum<4>(s);
-        if (threadIdx.x % 4 == 0) {
-            const float on = not_below_zero(s + p.b1[k]);
-            h[o] = on;
-            if (r < rows) p.h[(n0 + r) * p.hidden + k] = on;
-        }
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < p.c; c += 256) {
-        float w[GATE_ROWS], b[GATE_ROWS];
+// A workgroup takes four boards: their vectors lie in the LDS as [element][board], so one 16-byte read serves four boards
+// and a weight is loaded once for all of them.  Weights are read along their rows, 16 bytes a lane.
+constexpr int GATE_THREADS = 256;
+
+// out(j, sums) for every row j of w [rows][cols]: the row against the four boards' vectors v.  L lanes to a row; every lane
+// of them gets the sums.
+template <int L, typename F>
+__device__ inline void rows_times(const float* w, int rows, int cols, const f32x4* v, F&& out) {
+    const int lane = threadIdx.x % L;
+    for (int j = threadIdx.x / L; j < rows; j += GATE_THREADS / L) {
+        f32x4 s = 0.f;
+        for (int c = lane * 4; c < cols; c += L * 4) {
+            const f32x4 q = load_pack(w + (size_t)j * cols + c, cols - c);
 #pragma unroll
-        for (int r = 0; r < GATE_ROWS; ++r) {
-            w[r] = p.b2[c];
-            b[r] = p.b2[p.c + c];
+            for (int i = 0; i < 4; ++i) s += q[i] * v[c + i < cols ? c + i : 0];
         }
-        for (int k = 0; k < p.hidden; ++k) {
-            const float ww = p.w2[(size_t)c * p.hidden + k], wb = p.w2[(size_t)(p.c + c) * p.hidden + k];
 #pragma unroll
-            for (int r = 0; r < GATE_ROWS; ++r) {
-                w[r] += ww * h[r * p.hidden + k];
-                b[r] += wb * h[r * p.hidden + k];
+        for (int r = 0; r < 4; ++r) s[r] = lane_sum<L>(s[r]);
+        out(j, s);
+    }
+}
+
+template <typename F>
+__device__ inline void rows_times(const float* w, int rows, int cols, const f32x4* v, F&& out) {
+    if (cols <= 16) rows_times<4>(w, rows, cols, v, out);
+    else if (cols <= 32) rows_times<8>(w, rows, cols, v, out);
+    else rows_times<16>(w, rows, cols, v, out);
+}
+
+// out(k, sums) for every column k: the columns of w against v.  A thread takes four columns and every parts-th row; the parts
+// are added through the LDS in `part` (GATE_THREADS * 4 vectors).
+template <typename F>
+__device__ inline void columns_times(const float* w, int rows, int cols, const f32x4* v, f32x4* part, F&& out) {
+    const int fours = (cols + 3) / 4;
+    int wide = 1;
+    while (wide < fours && wide < GATE_THREADS) wide *= 2;
+    const int parts = GATE_THREADS / wide, x = threadIdx.x % wide, y = threadIdx.x / wide;
+    for (int at = 0; at < fours; at += wide) {
+        const int k = (at + x) * 4;
+        f32x4 s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (k < cols) {
+#pragma unroll 4
+            for (int j = y; j < rows; j += parts) {
+                const f32x4 q = load_pack(w + (size_t)j * cols + k, cols - k), vj = v[j];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] += q[i] * vj;
             }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[(y * wide + x) * 4 + i] = s[i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < wide * 4 && at * 4 + i < cols; i += GATE_THREADS) {
+            f32x4 t = part[i];
+            for (int q = 1; q < parts; ++q) t += part[q * wide * 4 + i];
+            out(at * 4 + i, t);
+        }
+        __syncthreads();
+    }
+}
+
+__global__ __launch_bounds__(GATE_THREADS) void k_gate_forward(const NormParams p) {
+    extern __shared__ f32x4 lds4[];
+    f32x4 *q = lds4, *h = q + p.c, *e = h + p.hidden;        // [c], [hidden], [2c]
+    const int64_t n0 = (int64_t)blockIdx.x * GATE_ROWS;
+    const int rows = (int)(p.n - n0 < GATE_ROWS ? p.n - n0 : GATE_ROWS);
+    for (int c = threadIdx.x; c < p.c; c += GATE_THREADS) {
+        const float scale = p.weight[c] * p.inv[c], mean = p.mean[c], bias = p.bias[c];
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < GATE_ROWS; ++r) v[r] = (p.board_mean[(n0 + (r < rows ? r : 0)) * p.c + c] - mean) * scale + bias;
+        q[c] = v;
+    }
+    __syncthreads();
+    rows_times(p.w1, p.hidden, p.c, q, [&](int k, const f32x4 s) {
+        const float b = p.b1[k];
+        f32x4 on;
+#pragma unroll
+        for (int r = 0; r < GATE_ROWS; ++r) on[r] = not_below_zero(s[r] + b);
+        h[k] = on;                                           // every lane of the row writes the same
+    });
+    __syncthreads();
+    for (int i = threadIdx.x; i < GATE_ROWS * p.hidden; i += GATE_THREADS) {
+        const int r = i / p.hidden, k = i % p.hidden;
+        if (r < rows) p.h[(n0 + r) * p.hidden + k] = h[k][r];
+    }
+    rows_times(p.w2, 2 * p.c, p.hidden, h, [&](int j, const f32x4 s) { e[j] = s + p.b2[j]; });
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.c; c += GATE_THREADS) {
         const float scale = p.weight[c] * p.inv[c], shift = p.bias[c] - scale * p.mean[c];
+        const f32x4 w = e[c], b = e[p.c + c];
 #pragma unroll
         for (int r = 0; r < GATE_ROWS; ++r)
             if (r < rows) {
@@ -542,57 +651,54 @@ __global__ __launch_bounds__(256) void k_gate_forward(const NormParams p) {
     }
 }
 
-__global__ __launch_bounds__(256) void k_gate_backward(const NormParams p) {
-    extern __shared__ float lds[];
-    float* de = lds;                                 // [GATE_ROWS][2c]
-    float* dh = lds + GATE_ROWS * 2 * p.c;           // [GATE_ROWS][hidden]
+__global__ __launch_bounds__(GATE_THREADS) void k_gate_backward(const NormParams p) {
+    extern __shared__ f32x4 lds4[];
+    f32x4 *de = lds4, *dh = de + 2 * p.c, *part = dh + p.hidden;     // [2c], [hidden], [GATE_THREADS * 4]
     const int64_t n0 = (int64_t)blockIdx.x * GATE_ROWS;
     const int rows = (int)(p.n - n0 < GATE_ROWS ? p.n - n0 : GATE_ROWS);
-    for (int i = threadIdx.x; i < GATE_ROWS * p.c; i += 256) {
-        const int r = i / p.c, c = i % p.c;
-        float w = 0.f, b = 0.f;
-        if (r < rows) {
-            const int64_t row = (n0 + r) * p.c + c;
-            const float gate = p.gate[row];
-            b = p.s1[row];
-            w = gate * (1.f - gate) * (p.weight[c] * p.inv[c] * p.s2[row] + p.bias[c] * b);
-            p.de[(n0 + r) * 2 * p.c + c] = w;
-            p.de[(n0 + r) * 2 * p.c + p.c + c] = b;
-        }
-        de[r * 2 * p.c + c] = w;
-        de[r * 2 * p.c + p.c + c] = b;
-    }
-    __syncthreads();
-    // a wavefront to a hidden unit: its column of fc2 against the four boards
-    for (int k = threadIdx.x / 64; k < p.hidden; k += 4) {
-        float s[GATE_ROWS] = {};
-        for (int j = threadIdx.x % 64; j < 2 * p.c; j += 64) {
-            const float w = p.w2[(size_t)j * p.hidden + k];
-#pragma unroll
-            for (int r = 0; r < GATE_ROWS; ++r) s[r] += w * de[r * 2 * p.c + j];
-        }
-#pragma unroll
-        for (int r = 0; r < GATE_ROWS; ++r) {
-            s[r] = lane_sum<64>(s[r]);
-            if (r >= rows || !(p.h[(n0 + (r < rows ? r : 0)) * p.hidden + k] > 0.f)) s[r] = 0.f;
-            if (threadIdx.x % 64 == 0) {
-                dh[r * p.hidden + k] = s[r];
-                if (r < rows) p.dh[(n0 + r) * p.hidden + k] = s[r];
-            }
-        }
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < p.c; c += 256) {
-        float s[GATE_ROWS] = {};
-        for (int k = 0; k < p.hidden; ++k) {
-            const float w = p.w1[(size_t)k * p.c + c];
-#pragma unroll
-            for (int r = 0; r < GATE_ROWS; ++r) s[r] += w * dh[r * p.hidden + k];
-        }
+    for (int c = threadIdx.x; c < p.c; c += GATE_THREADS) {
+        const float scale = p.weight[c] * p.inv[c], bias = p.bias[c];
+        f32x4 w = 0.f, b = 0.f;
 #pragma unroll
         for (int r = 0; r < GATE_ROWS; ++r)
-            if (r < rows) p.dq[(n0 + r) * p.c + c] = s[r];
+            if (r < rows) {
+                const int64_t row = (n0 + r) * p.c + c;
+                const float gate = p.gate[row];
+                b[r] = p.s1[row];
+                w[r] = gate * (1.f - gate) * (scale * p.s2[row] + bias * b[r]);
+                p.de[(n0 + r) * 2 * p.c + c] = w[r];
+                p.de[(n0 + r) * 2 * p.c + p.c + c] = b[r];
+            }
+        de[c] = w;
+        de[p.c + c] = b;
     }
+    __syncthreads();
+    columns_times(p.w2, 2 * p.c, p.hidden, de, part, [&](int k, f32x4 s) {
+#pragma unroll
+        for (int r = 0; r < GATE_ROWS; ++r)
+            if (r < rows) {
+                const int64_t at = (n0 + r) * p.hidden + k;
+                if (!(p.h[at] > 0.f)) s[r] = 0.f;
+                p.dh[at] = s[r];
+            }
+        dh[k] = s;
+    });
+    columns_times(p.w1, p.hidden, p.c, dh, part, [&](int c, const f32x4 s) {
+        // this workgroup's share of dy's channel sums
+        const float mean = p.mean[c];
+        float a = 0.f, b = 0.f;
+#pragma unroll
+        for (int r = 0; r < GATE_ROWS; ++r)
+            if (r < rows) {
+                const int64_t row = (n0 + r) * p.c + c;
+                const float gate = p.gate[row];
+                p.dq[row] = s[r];
+                a += gate * p.s1[row] + s[r];
+                b += gate * p.s2[row] + s[r] * (p.board_mean[row] - mean);
+            }
+        p.part_a[(size_t)blockIdx.x * p.c + c] = a;
+        p.part_b[(size_t)blockIdx.x * p.c + c] = b;
+    });
 }
 
 // Gradients of the gate's weights: sums over the boards of outer products, as 32 x 32 tiles.  A workgroup takes one tile and
@@ -601,7 +707,7 @@ __global__ __launch_bounds__(256) void k_gate_backward(const NormParams p) {
 // workgroups add them in order, beside its own work.
 // (One workgroup per tile over all boards, one board in flight, took 62 us at 1024 x 128 and 230 us at 4096 x 256: four times
 // the pass over the activations that follows.)
-constexpr int TILE = 32, TILE_WAVES = CHANNELS * BOARDS / 64, TILE_BOARDS = 4, TILE_OUT = TILE * TILE + TILE;
+constexpr int TILE = 32, TILE_WAVES = CHANNELS * LINES / 64, TILE_BOARDS = 4, TILE_OUT = TILE * TILE + TILE;
 
 struct TileShape {
     int m, k, across, tiles;                                         // [m][k] in `tiles` tiles, `across` to a row
@@ -695,7 +801,7 @@ __device__ void join_weights(const NormParams& p, int block) {
 
 static int join_blocks(const NormParams& p) { return p.hidden ? (weight_tiles(p) * TILE_OUT + NORM_THREADS - 1) / NORM_THREADS : 0; }
 
-__global__ __launch_bounds__(CHANNELS * BOARDS) void k_param_grads(const NormParams p, int channel_blocks) {
+__global__ __launch_bounds__(CHANNELS * LINES) void k_param_grads(const NormParams p, int channel_blocks) {
     if ((int)blockIdx.x < channel_blocks) channel_grads(p, blockIdx.x);
     else weight_tile(p, (int)blockIdx.x - channel_blocks);
 }
@@ -709,86 +815,75 @@ static void with_lanes(int nvec, F&& f) {
     else f(std::integral_constant<int, 16>());
 }
 
-template <typename T>
-static int norm_forward(const NormParams& p, bool last, const void* x, const void* residual, void* out, hipStream_t s) {
-    const T *xt = (const T*)x, *rt = (const T*)residual;
-    T* ot = (T*)out;
-    const bool need_rows = p.training || p.hidden;
+// Which boards a chunk of the pass over the activations holds.
+static void set_chunks(NormParams& p, bool last) {
+    p.chunk_boards = p.abreast = 1;
+    p.chunks = p.n;
+    if (last) return;
+    with_lanes(p.nvec, [&](auto L) {
+        const RowGrid g = row_grid<decltype(L)::value>(p);
+        p.chunk_boards = BOARDS_AT_ONCE;
+        p.abreast = (int)g.abreast;
+        p.chunks = (int64_t)(g.blocks / g.across) * g.abreast;
+    });
+}
+
+template <typename T, bool GATED>
+static int norm_forward(NormParams p, bool last, const T* x, const T* residual, T* out, hipStream_t s) {
     const int wide = p.nvec < 64 ? p.nvec : 64;
     const dim3 boards((uint32_t)p.n, (p.nvec + wide - 1) / wide), block(NORM_THREADS);
-    if (need_rows) {
-        if (last) hipLaunchKernelGGL((k_last_stats<T>), boards, block, 0, s, xt, p, wide);
+    set_chunks(p, last);
+    if (p.training || GATED) {
+        if (last) hipLaunchKernelGGL((k_last_stats<T, GATED>), boards, block, 0, s, x, p, wide);
         else with_lanes(p.nvec, [&](auto L) {
-            const uint32_t per = NORM_THREADS / L * ROWS_AT_ONCE;
-            hipLaunchKernelGGL((k_row_stats<T, decltype(L)::value>), dim3((p.rows + per - 1) / per), block, 0, s, xt, p);
+            const RowGrid g = row_grid<decltype(L)::value>(p);
+            hipLaunchKernelGGL((k_row_stats<T, decltype(L)::value, GATED>), dim3(g.blocks), block, 0, s, x, p, g);
         });
         AZ_HIP(hipGetLastError());
     }
-    hipLaunchKernelGGL(k_channel_stats, dim3((p.c + CHANNELS - 1) / CHANNELS), dim3(CHANNELS * BOARDS), 0, s, p);
+    hipLaunchKernelGGL(k_channel_stats, dim3((p.c + CHANNELS - 1) / CHANNELS), dim3(CHANNELS * LINES), 0, s, p);
     AZ_HIP(hipGetLastError());
-    if (p.hidden) {
-        hipLaunchKernelGGL(k_gate_forward, dim3((uint32_t)((p.n + GATE_ROWS - 1) / GATE_ROWS)), dim3(256),
-                           sizeof(float) * GATE_ROWS * (p.c + p.hidden), s, p);
+    if (GATED) {
+        hipLaunchKernelGGL(k_gate_forward, dim3((uint32_t)((p.n + GATE_ROWS - 1) / GATE_ROWS)), dim3(GATE_THREADS),
+                           sizeof(f32x4) * (3 * p.c + p.hidden), s, p);
         AZ_HIP(hipGetLastError());
     }
-    if (last) {
-        if (p.hidden) hipLaunchKernelGGL((k_last_apply<T, true>), boards, block, 0, s, xt, rt, ot, p, wide);
-        else hipLaunchKernelGGL((k_last_apply<T, false>), boards, block, 0, s, xt, rt, ot, p, wide);
-    } else {
-        with_lanes(p.nvec, [&](auto L) {
-            constexpr int N = decltype(L)::value;
-            const uint32_t per = NORM_THREADS / N * ROWS_AT_ONCE;
-            const dim3 grid((p.rows + per - 1) / per);
-            if (p.hidden) hipLaunchKernelGGL((k_row_apply<T, N, true>), grid, block, 0, s, xt, rt, ot, p);
-            else hipLaunchKernelGGL((k_row_apply<T, N, false>), grid, block, 0, s, xt, rt, ot, p);
-        });
-    }
+    if (last) hipLaunchKernelGGL((k_last_apply<T, GATED>), boards, block, 0, s, x, residual, out, p, wide);
+    else with_lanes(p.nvec, [&](auto L) {
+        const RowGrid g = row_grid<decltype(L)::value>(p);
+        hipLaunchKernelGGL((k_row_apply<T, decltype(L)::value, GATED>), dim3(g.blocks), block, 0, s, x, residual, out, p, g);
+    });
     AZ_HIP(hipGetLastError());
     return AZ_OK;
 }
 
-template <typename T>
-static int norm_backward(const NormParams& p, bool last, const void* x, const void* grad, void* dx, void* dresidual, hipStream_t s) {
-    const T *xt = (const T*)x, *gt = (const T*)grad;
-    T *dt = (T*)dx, *rt = (T*)dresidual;
+template <typename T, bool GATED>
+static int norm_backward(NormParams p, bool last, const T* x, const T* grad, T* dx, T* dresidual, hipStream_t s) {
     const int wide = p.nvec < 64 ? p.nvec : 64;
     const dim3 boards((uint32_t)p.n, (p.nvec + wide - 1) / wide), block(NORM_THREADS);
-    if (last) {
-        if (p.hidden) hipLaunchKernelGGL((k_last_grad_sums<T, true>), boards, block, 0, s, xt, gt, rt, p, wide);
-        else hipLaunchKernelGGL((k_last_grad_sums<T, false>), boards, block, 0, s, xt, gt, rt, p, wide);
-    } else {
-        with_lanes(p.nvec, [&](auto L) {
-            constexpr int N = decltype(L)::value;
-            const uint32_t per = NORM_THREADS / N * ROWS_AT_ONCE;
-            const dim3 grid((p.rows + per - 1) / per);
-            if (p.hidden) hipLaunchKernelGGL((k_row_grad_sums<T, N, true>), grid, block, 0, s, xt, gt, rt, p);
-            else hipLaunchKernelGGL((k_row_grad_sums<T, N, false>), grid, block, 0, s, xt, gt, rt, p);
-        });
-    }
+    set_chunks(p, last);
+    if (last) hipLaunchKernelGGL((k_last_grad_sums<T, GATED>), boards, block, 0, s, x, grad, dresidual, p, wide);
+    else with_lanes(p.nvec, [&](auto L) {
+        const RowGrid g = row_grid<decltype(L)::value>(p);
+        hipLaunchKernelGGL((k_row_grad_sums<T, decltype(L)::value, GATED>), dim3(g.blocks), block, 0, s, x, grad, dresidual, p, g);
+    });
     AZ_HIP(hipGetLastError());
-    if (p.hidden) {
-        hipLaunchKernelGGL(k_gate_backward, dim3((uint32_t)((p.n + GATE_ROWS - 1) / GATE_ROWS)), dim3(256),
-                           sizeof(float) * GATE_ROWS * (2 * p.c + p.hidden), s, p);
+    if (GATED) {
+        p.chunks = (p.n + GATE_ROWS - 1) / GATE_ROWS;
+        hipLaunchKernelGGL(k_gate_backward, dim3((uint32_t)p.chunks), dim3(GATE_THREADS),
+                           sizeof(f32x4) * (2 * p.c + p.hidden + GATE_THREADS * 4), s, p);
         AZ_HIP(hipGetLastError());
     }
     const int cb = (p.c + CHANNELS - 1) / CHANNELS;
-    hipLaunchKernelGGL(k_param_grads, dim3(cb + (p.hidden ? weight_tiles(p) * weight_splits(p) : 0)), dim3(CHANNELS * BOARDS), 0, s, p, cb);
+    hipLaunchKernelGGL(k_param_grads, dim3(cb + (GATED ? weight_tiles(p) * weight_splits(p) : 0)), dim3(CHANNELS * LINES), 0, s, p, cb);
     AZ_HIP(hipGetLastError());
-    const T* mt = p.hidden ? rt : gt;
+    const T* masked = GATED ? dresidual : grad;
     const uint32_t joins = (uint32_t)join_blocks(p);
-    if (last) {
-        const dim3 grid(boards.x + joins, boards.y);
-        if (p.hidden) hipLaunchKernelGGL((k_last_grad_apply<T, true>), grid, block, 0, s, xt, mt, dt, p, wide, joins);
-        else hipLaunchKernelGGL((k_last_grad_apply<T, false>), grid, block, 0, s, xt, mt, dt, p, wide, joins);
-    } else {
-        with_lanes(p.nvec, [&](auto L) {
-            constexpr int N = decltype(L)::value;
-            const uint32_t per = NORM_THREADS / N * ROWS_AT_ONCE;
-            const dim3 grid((p.rows + per - 1) / per + joins);
-            if (p.hidden) hipLaunchKernelGGL((k_row_grad_apply<T, N, true>), grid, block, 0, s, xt, mt, dt, p, joins);
-            else hipLaunchKernelGGL((k_row_grad_apply<T, N, false>), grid, block, 0, s, xt, mt, dt, p, joins);
-        });
-    }
+    if (last) hipLaunchKernelGGL((k_last_grad_apply<T, GATED>), dim3(boards.x + joins, boards.y), block, 0, s, x, masked, dx, p, wide, joins);
+    else with_lanes(p.nvec, [&](auto L) {
+        const RowGrid g = row_grid<decltype(L)::value>(p);
+        hipLaunchKernelGGL((k_row_grad_apply<T, decltype(L)::value, GATED>), dim3(g.blocks + joins), block, 0, s, x, masked, dx, p, g, joins);
+    });
     AZ_HIP(hipGetLastError());
     return AZ_OK;
 }
@@ -822,7 +917,6 @@ static int norm_params(const az_norm_args* a, NormParams* p, int64_t sizes[3]) {
     p->hidden = a->hidden;
     p->nvec = ((a->channels_last ? a->c : a->hw) + V - 1) / V;
     p->training = a->training != 0;
-    p->rows = (uint32_t)rows;
     p->eps = a->eps;
     p->momentum = a->momentum;
     p->weight = a->weight_dev;
@@ -841,27 +935,27 @@ static int norm_params(const az_norm_args* a, NormParams* p, int64_t sizes[3]) {
     p->dw2 = a->dfc2_weight_dev;
     p->db2 = a->dfc2_bias_dev;
     Carver saved = {(char*)a->saved_dev, 0}, fwd = {(char*)a->workspace_dev, 0}, bwd = {(char*)a->workspace_dev, 0};
+    p->board_mean = p->gate = p->h = p->s1 = p->s2 = p->de = p->dh = p->dq = p->partial = nullptr;
     p->mean = saved.take<float>(a->c);
     p->inv = saved.take<float>(a->c);
     if (a->hidden) {
         p->board_mean = saved.take<float>(rows);
         p->gate = saved.take<float>(rows);
         p->h = saved.take<float>(hidden);
-    } else {
-        p->board_mean = fwd.take<float>(rows);
-        p->gate = p->h = nullptr;
     }
     p->mask = saved.take<uint8_t>((size_t)p->nvec * (a->channels_last ? (size_t)a->n * a->hw : rows));
-    p->m2 = fwd.take<float>(rows);
+    // both passes begin with the partial sums: at most one chunk per board, and a row more per board that lies abreast
+    p->part_a = fwd.take<float>(rows + (size_t)NORM_THREADS * a->c);
+    p->part_b = fwd.take<float>(rows + (size_t)NORM_THREADS * a->c);
+    bwd.used = fwd.used;
     p->A = fwd.take<float>(a->hidden ? rows : a->c);
     p->B = fwd.take<float>(a->hidden ? rows : a->c);
-    p->s1 = bwd.take<float>(rows);
-    p->s2 = bwd.take<float>(rows);
     p->ca = bwd.take<float>(a->c);
     p->cb = bwd.take<float>(a->c);
     p->cd = bwd.take<float>(a->c);
-    p->de = p->dh = p->dq = p->partial = nullptr;
     if (a->hidden) {
+        p->s1 = bwd.take<float>(rows);
+        p->s2 = bwd.take<float>(rows);
         p->de = bwd.take<float>(2 * rows);
         p->dh = bwd.take<float>(hidden);
         p->dq = bwd.take<float>(rows);
@@ -882,6 +976,13 @@ static int norm_check(const az_norm_args* a) {
     return AZ_OK;
 }
 
+// f(a value of the activations' type, whether there is a gate)
+template <typename F>
+static int with_type(const az_norm_args* a, F&& f) {
+    const auto gated = [&](auto t) { return a->hidden ? f(t, std::true_type()) : f(t, std::false_type()); };
+    return a->dtype == AZ_F32 ? gated(0.f) : a->dtype == AZ_BF16 ? gated((__bf16)0.f) : gated((_Float16)0.f);
+}
+
 }  // namespace az
 
 using namespace az;
@@ -899,12 +1000,11 @@ extern "C" int az_norm_forward(const az_norm_args* a, void* stream) {
     if (rc != AZ_OK) return rc;
     AZ_CHECK_ARG(a->out_dev && (!a->hidden || a->residual_dev), "az_norm_forward: null argument");
     AZ_CHECK_ARG(a->training || (a->running_mean_dev && a->running_var_dev), "az_norm_forward: evaluation without running statistics");
-    const bool last = a->channels_last != 0;
-    switch (a->dtype) {
-        case AZ_F32: return norm_forward<float>(p, last, a->x_dev, a->residual_dev, a->out_dev, (hipStream_t)stream);
-        case AZ_BF16: return norm_forward<__bf16>(p, last, a->x_dev, a->residual_dev, a->out_dev, (hipStream_t)stream);
-        default: return norm_forward<_Float16>(p, last, a->x_dev, a->residual_dev, a->out_dev, (hipStream_t)stream);
-    }
+    return with_type(a, [&](auto t, auto gated) {
+        typedef decltype(t) T;
+        return norm_forward<T, decltype(gated)::value>(p, a->channels_last != 0, (const T*)a->x_dev, (const T*)a->residual_dev, (T*)a->out_dev,
+                                                       (hipStream_t)stream);
+    });
 }
 
 extern "C" int az_norm_backward(const az_norm_args* a, void* stream) {
@@ -915,10 +1015,9 @@ extern "C" int az_norm_backward(const az_norm_args* a, void* stream) {
     AZ_CHECK_ARG(a->grad_dev && a->dx_dev && a->dweight_dev && a->dbias_dev, "az_norm_backward: null argument");
     AZ_CHECK_ARG(!a->hidden || (a->dresidual_dev && a->dfc1_weight_dev && a->dfc1_bias_dev && a->dfc2_weight_dev && a->dfc2_bias_dev),
                  "az_norm_backward: null gate gradient");
-    const bool last = a->channels_last != 0;
-    switch (a->dtype) {
-        case AZ_F32: return norm_backward<float>(p, last, a->x_dev, a->grad_dev, a->dx_dev, a->dresidual_dev, (hipStream_t)stream);
-        case AZ_BF16: return norm_backward<__bf16>(p, last, a->x_dev, a->grad_dev, a->dx_dev, a->dresidual_dev, (hipStream_t)stream);
-        default: return norm_backward<_Float16>(p, last, a->x_dev, a->grad_dev, a->dx_dev, a->dresidual_dev, (hipStream_t)stream);
-    }
+    return with_type(a, [&](auto t, auto gated) {
+        typedef decltype(t) T;
+        return norm_backward<T, decltype(gated)::value>(p, a->channels_last != 0, (const T*)a->x_dev, (const T*)a->grad_dev, (T*)a->dx_dev,
+                                                        (T*)a->dresidual_dev, (hipStream_t)stream);
+    });
 }
