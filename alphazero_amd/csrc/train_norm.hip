@@ -70,16 +70,23 @@ __device__ inline int64_t boards_in_chunk(const NormParams& p, int64_t i) {
 // once, and the boards' sums joined in registers before they leave (a chunk).  The groups of a workgroup lie along the
 // channels, so what it loads at once is one stretch of memory; where there are fewer channels than groups, `abreast`
 // boards lie side by side.
+//
+// How a row fits its lanes (a row of up to 64 pieces of 16 bytes takes one piece a lane, all boards' loads issued before
+// the first is used):
+//   EXACT  hw is L pieces.
+//   ONE    up to L pieces, the last one moved back to end with the row: no partial loads or stores.  The values that it
+//          shares with its neighbour are left out of the sums and stored twice, the same.
+//   LOOP   longer rows, and rows shorter than a piece: round after round, the last piece value by value.
 constexpr int BOARDS_AT_ONCE = 4;
+enum Fit { EXACT, ONE, LOOP };
 
 struct RowGrid {
     uint32_t wide, abreast, across;          // channels and boards side by side in a workgroup; workgroups to a board
     uint32_t blocks;
 };
 
-template <int L>
-static RowGrid row_grid(const NormParams& p) {
-    const uint32_t groups = NORM_THREADS / L, c = (uint32_t)p.c;
+static RowGrid row_grid(const NormParams& p, int lanes) {
+    const uint32_t groups = NORM_THREADS / lanes, c = (uint32_t)p.c;
     RowGrid g;
     g.wide = c < groups ? c : groups;
     g.abreast = groups / g.wide;
@@ -88,141 +95,234 @@ static RowGrid row_grid(const NormParams& p) {
     return g;
 }
 
+template <typename T, int L, Fit FIT>
 struct RowPlace {
-    uint32_t c, chunk, lane;
-    int64_t first;                           // first board; the others follow `abreast` apart
+    static constexpr int V = Pack<T>::V;
+    uint32_t c, chunk, lane, abreast;
+    int64_t n_first;                         // first board; the others follow `abreast` apart
     bool on;
+    int off, own;                            // EXACT, ONE: where the lane's piece begins, and its first value that is its own
+
+    __device__ RowPlace(const NormParams& p, const RowGrid& g, uint32_t block) {
+        const uint32_t group = threadIdx.x / L, nb = block / g.across, beside = g.abreast == 1 ? 0 : group / g.wide;
+        lane = threadIdx.x % L;
+        c = block % g.across * (NORM_THREADS / L) + group - beside * g.wide;
+        chunk = nb * g.abreast + beside;
+        abreast = g.abreast;
+        n_first = (int64_t)nb * BOARDS_AT_ONCE * g.abreast + beside;
+        on = c < (uint32_t)p.c && beside < g.abreast;
+        const int at = lane * V;
+        off = FIT == EXACT || at < p.hw - V ? at : p.hw - V;
+        own = FIT == EXACT ? 0 : at - off < V ? at - off : V;
+    }
+    __device__ int64_t board(int k) const { return n_first + k * abreast; }
+    __device__ size_t row(const NormParams& p, int k) const { return (size_t)(board(k) < p.n ? board(k) : n_first) * p.c + c; }
+    __device__ bool has_piece(const NormParams& p) const { return FIT == EXACT || (int)lane < p.nvec; }
 };
 
-template <int L>
-__device__ inline RowPlace row_place(const NormParams& p, const RowGrid& g, uint32_t block) {
-    const uint32_t group = threadIdx.x / L, nb = block / g.across, beside = g.abreast == 1 ? 0 : group / g.wide;
-    RowPlace r;
-    r.lane = threadIdx.x % L;
-    r.c = block % g.across * (NORM_THREADS / L) + group - beside * g.wide;
-    r.chunk = nb * g.abreast + beside;
-    r.first = (int64_t)nb * BOARDS_AT_ONCE * g.abreast + beside;
-    r.on = r.c < (uint32_t)p.c && beside < g.abreast;        // (a chunk may be empty: its sums are zero)
-    return r;
+template <typename T> __device__ inline typename Pack<T>::raw load_raw(const T* p) { return *(const typename Pack<T>::loose*)p; }
+template <typename T> __device__ inline typename Pack<T>::f32 widen(typename Pack<T>::raw v) { return __builtin_convertvector(v, typename Pack<T>::f32); }
+template <typename T> __device__ inline void store_raw(T* p, typename Pack<T>::f32 v) {
+    *(typename Pack<T>::loose*)p = __builtin_convertvector(v, typename Pack<T>::raw);
 }
 
-template <typename T, int L, bool GATED>
+// Mean and centred sum of a board's values, joined to a chunk's.
+struct ChunkStats {
+    float mean = 0.f, m2 = 0.f, boards = 0.f;
+    __device__ void join(float board, float board_m2, float hw) {
+        boards += 1.f;
+        const float d = board - mean;
+        mean += d / boards;
+        m2 += board_m2 + hw * d * (board - mean);
+    }
+};
+
+template <typename T, int L, Fit FIT, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_row_stats(const T* __restrict__ x, const NormParams p, const RowGrid grid) {
     constexpr int V = Pack<T>::V;
-    const RowPlace r = row_place<L>(p, grid, blockIdx.x);
-    float first[BOARDS_AT_ONCE], s[BOARDS_AT_ONCE], ss[BOARDS_AT_ONCE];
+    const RowPlace<T, L, FIT> r(p, grid, blockIdx.x);
+    if (!r.on) return;                       // whole groups: the sums below stay within one
+    const float hw = (float)p.hw;
+    ChunkStats chunk;
+    if (r.n_first < p.n) {
+        if constexpr (FIT != LOOP) {
+            typename Pack<T>::raw raw[BOARDS_AT_ONCE];
 #pragma unroll
-    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
-        const int64_t n = r.first + k * grid.abreast;
-        first[k] = s[k] = ss[k] = 0.f;
-        if (!r.on || n >= p.n) continue;
-        const T* xr = x + (size_t)(n * p.c + r.c) * p.hw;
-        first[k] = (float)xr[0];
-        for (int j = r.lane; j < p.nvec; j += L) {
-            const int left = p.hw - j * V;
-            const auto v = load_pack(xr + j * V, left);
+            for (int k = 0; k < BOARDS_AT_ONCE; ++k) raw[k] = load_raw(x + r.row(p, k) * p.hw + r.off);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float d = i < left ? v[i] - first[k] : 0.f;
-                s[k] += d;
-                ss[k] += d * d;
+            for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+                const auto v = widen<T>(raw[k]);
+                float s = 0.f, ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) s += FIT == EXACT || i >= r.own ? v[i] : 0.f;
+                const float mean = lane_sum<L>(s) / hw;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float d = FIT == EXACT || i >= r.own ? v[i] - mean : 0.f;
+                    ss += d * d;
+                }
+                ss = lane_sum<L>(ss);
+                if (r.board(k) >= p.n) continue;
+                if (GATED && r.lane == 0) p.board_mean[r.row(p, k)] = mean;
+                chunk.join(mean, ss, hw);
+            }
+        } else {
+            for (int k = 0; k < BOARDS_AT_ONCE && r.board(k) < p.n; ++k) {
+                const T* xr = x + r.row(p, k) * p.hw;
+                const float first = (float)xr[0];
+                float s = 0.f, ss = 0.f;
+                for (int j = r.lane; j < p.nvec; j += L) {
+                    const int left = p.hw - j * V;
+                    const auto v = load_pack(xr + j * V, left);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float d = i < left ? v[i] - first : 0.f;
+                        s += d;
+                        ss += d * d;
+                    }
+                }
+                s = lane_sum<L>(s);
+                ss = lane_sum<L>(ss);
+                const float mean = first + s / hw;
+                if (GATED && r.lane == 0) p.board_mean[r.row(p, k)] = mean;
+                chunk.join(mean, not_below_zero(ss - s * s / hw), hw);
             }
         }
     }
-    const float hw = (float)p.hw;
-    float mean = 0.f, m2 = 0.f, boards = 0.f;
-#pragma unroll
-    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
-        const int64_t n = r.first + k * grid.abreast;
-        const float a = lane_sum<L>(s[k]), b = lane_sum<L>(ss[k]);
-        if (!r.on || n >= p.n) continue;
-        const float board = first[k] + a / hw;
-        if (GATED && r.lane == 0) p.board_mean[n * p.c + r.c] = board;
-        boards += 1.f;                       // join this board's mean and centred sum to the chunk's
-        const float d = board - mean;
-        mean += d / boards;
-        m2 += not_below_zero(b - a * a / hw) + hw * d * (board - mean);
-    }
-    if (r.on && r.lane == 0) {
-        p.part_a[(size_t)r.chunk * p.c + r.c] = mean;
-        p.part_b[(size_t)r.chunk * p.c + r.c] = m2;
+    if (r.lane == 0) {
+        p.part_a[(size_t)r.chunk * p.c + r.c] = chunk.mean;
+        p.part_b[(size_t)r.chunk * p.c + r.c] = chunk.m2;
     }
 }
 
-template <typename T, int L, bool GATED>
+// relu of v, and which of its values are positive
+template <typename F>
+__device__ inline uint32_t relu_bits(F& v) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(F) / 4); ++i) {
+        bits |= (v[i] > 0.f ? 1u : 0u) << i;
+        v[i] = not_below_zero(v[i]);
+    }
+    return bits;
+}
+
+template <typename T, int L, Fit FIT, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_row_apply(const T* __restrict__ x, const T* __restrict__ residual,
                                                             T* __restrict__ out, const NormParams p, const RowGrid grid) {
     constexpr int V = Pack<T>::V;
-    const RowPlace r = row_place<L>(p, grid, blockIdx.x);
-    if (!r.on) return;
+    const RowPlace<T, L, FIT> r(p, grid, blockIdx.x);
+    if (!r.on || r.n_first >= p.n) return;
+    if constexpr (FIT != LOOP) {
+        typename Pack<T>::raw raw[BOARDS_AT_ONCE], res[BOARDS_AT_ONCE];
+        float A[BOARDS_AT_ONCE], B[BOARDS_AT_ONCE];
 #pragma unroll
-    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
-        const int64_t n = r.first + k * grid.abreast, row = n * p.c + r.c;
-        if (n >= p.n) return;
-        const size_t at = (size_t)row * p.hw;
-        const float A = p.A[GATED ? row : r.c], B = p.B[GATED ? row : r.c];
-        for (int j = r.lane; j < p.nvec; j += L) {
-            const int left = p.hw - j * V;
-            auto v = load_pack(x + at + j * V, left) * A + B;
-            if (GATED) v += load_pack(residual + at + j * V, left);
-            uint32_t bits = 0;
+        for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+            const size_t row = r.row(p, k);
+            A[k] = p.A[GATED ? row : r.c];
+            B[k] = p.B[GATED ? row : r.c];
+            raw[k] = load_raw(x + row * p.hw + r.off);
+            if (GATED) res[k] = load_raw(residual + row * p.hw + r.off);
+        }
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                bits |= (v[i] > 0.f ? 1u : 0u) << i;
-                v[i] = not_below_zero(v[i]);
+        for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+            if (r.board(k) >= p.n) return;
+            const size_t row = r.row(p, k);
+            auto v = widen<T>(raw[k]) * A[k] + B[k];
+            if (GATED) v += widen<T>(res[k]);
+            const uint32_t bits = relu_bits(v);
+            store_raw(out + row * p.hw + r.off, v);
+            if (r.has_piece(p)) p.mask[row * p.nvec + r.lane] = (uint8_t)bits;
+        }
+    } else {
+        for (int k = 0; k < BOARDS_AT_ONCE && r.board(k) < p.n; ++k) {
+            const size_t row = r.row(p, k), at = row * p.hw;
+            const float A = p.A[GATED ? row : r.c], B = p.B[GATED ? row : r.c];
+            for (int j = r.lane; j < p.nvec; j += L) {
+                const int left = p.hw - j * V;
+                auto v = load_pack(x + at + j * V, left) * A + B;
+                if (GATED) v += load_pack(residual + at + j * V, left);
+                const uint32_t bits = relu_bits(v);
+                store_pack(out + at + j * V, v, left);
+                p.mask[row * p.nvec + j] = (uint8_t)bits;
             }
-            store_pack(out + at + j * V, v, left);
-            p.mask[(size_t)row * p.nvec + j] = (uint8_t)bits;
         }
     }
 }
 
-template <typename T, int L, bool GATED>
+template <typename T, int L, Fit FIT, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_sums(const T* __restrict__ x, const T* __restrict__ grad,
                                                                 T* __restrict__ dresidual, const NormParams p, const RowGrid grid) {
     constexpr int V = Pack<T>::V;
-    const RowPlace r = row_place<L>(p, grid, blockIdx.x);
-    const float mean = r.on ? p.mean[r.c] : 0.f;
-    float s1[BOARDS_AT_ONCE], s2[BOARDS_AT_ONCE];
-#pragma unroll
-    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
-        const int64_t n = r.first + k * grid.abreast, row = n * p.c + r.c;
-        s1[k] = s2[k] = 0.f;
-        if (!r.on || n >= p.n) continue;
-        const size_t at = (size_t)row * p.hw;
-        for (int j = r.lane; j < p.nvec; j += L) {
-            const int left = p.hw - j * V;
-            const auto v = load_pack(x + at + j * V, left);
-            auto g = load_pack(grad + at + j * V, left);
-            const uint32_t bits = p.mask[(size_t)row * p.nvec + j];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                g[i] = bits >> i & 1 ? g[i] : 0.f;
-                s1[k] += g[i];
-                s2[k] += g[i] * (v[i] - mean);
-            }
-            if (GATED) store_pack(dresidual + at + j * V, g, left);
-        }
-    }
+    const RowPlace<T, L, FIT> r(p, grid, blockIdx.x);
+    if (!r.on) return;
+    const float mean = p.mean[r.c];
     float a = 0.f, b = 0.f;
-#pragma unroll
-    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
-        const int64_t n = r.first + k * grid.abreast;
+    const auto board_sums = [&](int k, float s1, float s2) {
         if (GATED) {                         // the gate's gradient needs every board's
-            const float sa = lane_sum<L>(s1[k]), sb = lane_sum<L>(s2[k]);
-            if (r.on && n < p.n && r.lane == 0) {
-                p.s1[n * p.c + r.c] = sa;
-                p.s2[n * p.c + r.c] = sb;
+            s1 = lane_sum<L>(s1);
+            s2 = lane_sum<L>(s2);
+            if (r.board(k) < p.n && r.lane == 0) {
+                p.s1[r.row(p, k)] = s1;
+                p.s2[r.row(p, k)] = s2;
+            }
+        } else if (r.board(k) < p.n) {
+            a += s1;
+            b += s2;
+        }
+    };
+    if (r.n_first < p.n) {
+        if constexpr (FIT != LOOP) {
+            typename Pack<T>::raw raw[BOARDS_AT_ONCE], gr[BOARDS_AT_ONCE];
+            uint32_t bits[BOARDS_AT_ONCE];
+            const uint32_t piece = r.has_piece(p) ? r.lane : 0;
+#pragma unroll
+            for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+                const size_t row = r.row(p, k);
+                raw[k] = load_raw(x + row * p.hw + r.off);
+                gr[k] = load_raw(grad + row * p.hw + r.off);
+                bits[k] = p.mask[row * p.nvec + piece];
+            }
+#pragma unroll
+            for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+                const auto v = widen<T>(raw[k]);
+                auto g = widen<T>(gr[k]);
+                float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    g[i] = bits[k] >> i & 1 ? g[i] : 0.f;
+                    const float gi = FIT == EXACT || i >= r.own ? g[i] : 0.f;
+                    s1 += gi;
+                    s2 += gi * (v[i] - mean);
+                }
+                if (GATED && r.board(k) < p.n && r.has_piece(p)) store_raw(dresidual + r.row(p, k) * p.hw + r.off, g);
+                board_sums(k, s1, s2);
             }
         } else {
-            a += s1[k];
-            b += s2[k];
+            for (int k = 0; k < BOARDS_AT_ONCE && r.board(k) < p.n; ++k) {
+                const size_t row = r.row(p, k), at = row * p.hw;
+                float s1 = 0.f, s2 = 0.f;
+                for (int j = r.lane; j < p.nvec; j += L) {
+                    const int left = p.hw - j * V;
+                    const auto v = load_pack(x + at + j * V, left);
+                    auto g = load_pack(grad + at + j * V, left);
+                    const uint32_t bits = p.mask[row * p.nvec + j];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        g[i] = bits >> i & 1 ? g[i] : 0.f;
+                        s1 += g[i];
+                        s2 += g[i] * (v[i] - mean);
+                    }
+                    if (GATED) store_pack(dresidual + at + j * V, g, left);
+                }
+                board_sums(k, s1, s2);
+            }
         }
     }
     if (!GATED) {
         a = lane_sum<L>(a);
         b = lane_sum<L>(b);
-        if (r.on && r.lane == 0) {
+        if (r.lane == 0) {
             p.part_a[(size_t)r.chunk * p.c + r.c] = a;
             p.part_b[(size_t)r.chunk * p.c + r.c] = b;
         }
@@ -230,7 +330,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_sums(const T* __restr
 }
 
 // grad: the masked one (dresidual) if gated
-template <typename T, int L, bool GATED>
+template <typename T, int L, Fit FIT, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_apply(const T* __restrict__ x, const T* __restrict__ grad,
                                                                  T* __restrict__ dx, const NormParams p, const RowGrid grid, uint32_t joins) {
     constexpr int V = Pack<T>::V;
@@ -238,32 +338,63 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_apply(const T* __rest
         join_weights(p, blockIdx.x);
         return;
     }
-    const RowPlace r = row_place<L>(p, grid, blockIdx.x - joins);
-    if (!r.on) return;
+    const RowPlace<T, L, FIT> r(p, grid, blockIdx.x - joins);
+    if (!r.on || r.n_first >= p.n) return;
     const float mean = p.mean[r.c], b = p.cb[r.c], ca = p.ca[r.c], cd = p.cd[r.c], per_place = ca / (float)p.hw;
+    if constexpr (FIT != LOOP) {
+        typename Pack<T>::raw raw[BOARDS_AT_ONCE], gr[BOARDS_AT_ONCE];
+        float gate[BOARDS_AT_ONCE], dq[BOARDS_AT_ONCE];
+        uint32_t bits[BOARDS_AT_ONCE];
+        const uint32_t piece = r.has_piece(p) ? r.lane : 0;
 #pragma unroll
-    for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
-        const int64_t n = r.first + k * grid.abreast, row = n * p.c + r.c;
-        if (n >= p.n) return;
-        const size_t at = (size_t)row * p.hw;
-        const float a = GATED ? ca * p.gate[row] : ca, d = GATED ? cd + per_place * p.dq[row] : cd;
-        for (int j = r.lane; j < p.nvec; j += L) {
-            const int left = p.hw - j * V;
-            const auto v = load_pack(x + at + j * V, left);
-            auto g = load_pack(grad + at + j * V, left);
-            const uint32_t bits = GATED ? 0 : p.mask[(size_t)row * p.nvec + j];
+        for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+            const size_t row = r.row(p, k);
+            if (GATED) {
+                gate[k] = p.gate[row];
+                dq[k] = p.dq[row];
+            } else {
+                bits[k] = p.mask[row * p.nvec + piece];
+            }
+            raw[k] = load_raw(x + row * p.hw + r.off);
+            gr[k] = load_raw(grad + row * p.hw + r.off);
+        }
+#pragma unroll
+        for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
+            if (r.board(k) >= p.n) return;
+            const float a = GATED ? ca * gate[k] : ca, d = GATED ? cd + per_place * dq[k] : cd;
+            const auto v = widen<T>(raw[k]);
+            auto g = widen<T>(gr[k]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                if (!GATED) g[i] = bits >> i & 1 ? g[i] : 0.f;
+                if (!GATED) g[i] = bits[k] >> i & 1 ? g[i] : 0.f;
                 g[i] = g[i] * a + ((v[i] - mean) * b + d);
             }
-            store_pack(dx + at + j * V, g, left);
+            if (r.has_piece(p)) store_raw(dx + r.row(p, k) * p.hw + r.off, g);
+        }
+    } else {
+        for (int k = 0; k < BOARDS_AT_ONCE && r.board(k) < p.n; ++k) {
+            const size_t row = r.row(p, k), at = row * p.hw;
+            const float a = GATED ? ca * p.gate[row] : ca, d = GATED ? cd + per_place * p.dq[row] : cd;
+            for (int j = r.lane; j < p.nvec; j += L) {
+                const int left = p.hw - j * V;
+                const auto v = load_pack(x + at + j * V, left);
+                auto g = load_pack(grad + at + j * V, left);
+                const uint32_t bits = GATED ? 0 : p.mask[row * p.nvec + j];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    if (!GATED) g[i] = bits >> i & 1 ? g[i] : 0.f;
+                    g[i] = g[i] * a + ((v[i] - mean) * b + d);
+                }
+                store_pack(dx + at + j * V, g, left);
+            }
         }
     }
 }
 
 // ---------------------------------------------- [n][hw][c]: a workgroup to a board and a range of channels
 // Thread (ty, tx): 16 bytes of channels, every ty-th place of the board; the ty are added through LDS.  A chunk is a board.
+// The last 16 bytes are moved back to end with the channels (what they share with their neighbours is computed twice, the
+// same); fewer channels than 16 bytes go value by value.
 struct Lanes {
     int tx, ty, step;          // step: places taken at once
     int j;                     // which 16 bytes of the channels
@@ -273,16 +404,23 @@ struct Lanes {
 
 template <typename T>
 __device__ inline Lanes lanes_of(const NormParams& p, int wide) {
+    constexpr int V = Pack<T>::V;
     Lanes l;
     l.tx = threadIdx.x % wide;
     l.ty = threadIdx.x / wide;
     l.step = NORM_THREADS / wide;
     l.j = blockIdx.y * wide + l.tx;
     l.on = l.ty < l.step && l.j < p.nvec;
-    l.c = l.j * Pack<T>::V;
+    l.c = p.c >= V && l.j * V > p.c - V ? p.c - V : l.j * V;
     l.left = p.c - l.c;
     return l;
 }
+
+// FULL: every piece is whole.
+template <bool FULL, typename T>
+__device__ inline typename Pack<T>::f32 load_piece(const T* p, int left) { return load_pack(p, FULL ? Pack<T>::V : left); }
+template <bool FULL, typename T>
+__device__ inline void store_piece(T* p, typename Pack<T>::f32 v, int left) { store_pack(p, v, FULL ? Pack<T>::V : left); }
 
 // Numbers of the thread's channels, 16 bytes at a time.
 template <typename F>
@@ -311,17 +449,20 @@ __device__ inline void add_places(F a, F b, const Lanes& l, const NormParams& p,
     }
     __syncthreads();
     const int c0 = blockIdx.y * wide * V;
-    for (int i = threadIdx.x; i < wide * V && c0 + i < p.c; i += NORM_THREADS) {
+    for (int i = threadIdx.x; i < wide * V; i += NORM_THREADS) {
+        // channel of the i-th value: the last piece is moved back
+        const int piece = c0 + i / V * V, c = (p.c >= V && piece > p.c - V && piece < p.c ? p.c - V : piece) + i % V;
+        if (c >= p.c) continue;
         float s = 0.f, ss = 0.f;
         for (int y = 0; y < l.step; ++y) {
             s += red[0][y * wide * V + i];
             ss += red[1][y * wide * V + i];
         }
-        out(c0 + i, s, ss);
+        out(c, s, ss);
     }
 }
 
-template <typename T, bool GATED>
+template <typename T, bool FULL, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_last_stats(const T* __restrict__ x, const NormParams p, int wide) {
     constexpr int V = Pack<T>::V;
     typedef typename Pack<T>::f32 F;
@@ -331,10 +472,10 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_stats(const T* __restrict
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] = ss[i] = 0.f;
     if (l.on) {
-        const F first = load_pack(xb + l.c, l.left);
+        const F first = load_piece<FULL>(xb + l.c, l.left);
 #pragma unroll 4
         for (int y = l.ty; y < p.hw; y += l.step) {
-            const F d = load_pack(xb + (size_t)y * p.c + l.c, l.left) - first;
+            const F d = load_piece<FULL>(xb + (size_t)y * p.c + l.c, l.left) - first;
             s += d;
             ss += d * d;
         }
@@ -348,7 +489,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_stats(const T* __restrict
     });
 }
 
-template <typename T, bool GATED>
+template <typename T, bool FULL, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_last_apply(const T* __restrict__ x, const T* __restrict__ residual,
                                                              T* __restrict__ out, const NormParams p, int wide) {
     constexpr int V = Pack<T>::V;
@@ -361,20 +502,20 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_apply(const T* __restrict
 #pragma unroll 4
     for (int y = l.ty; y < p.hw; y += l.step) {
         const size_t at = (board + y) * p.c + l.c;
-        F v = load_pack(x + at, l.left) * A + B;
-        if (GATED) v += load_pack(residual + at, l.left);
+        F v = load_piece<FULL>(x + at, l.left) * A + B;
+        if (GATED) v += load_piece<FULL>(residual + at, l.left);
         uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             bits |= (v[i] > 0.f ? 1u : 0u) << i;
             v[i] = not_below_zero(v[i]);
         }
-        store_pack(out + at, v, l.left);
+        store_piece<FULL>(out + at, v, l.left);
         p.mask[(board + y) * p.nvec + l.j] = (uint8_t)bits;
     }
 }
 
-template <typename T, bool GATED>
+template <typename T, bool FULL, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_sums(const T* __restrict__ x, const T* __restrict__ grad,
                                                                  T* __restrict__ dresidual, const NormParams p, int wide) {
     constexpr int V = Pack<T>::V;
@@ -389,8 +530,8 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_sums(const T* __rest
 #pragma unroll 4
         for (int y = l.ty; y < p.hw; y += l.step) {
             const size_t at = (board + y) * p.c + l.c;
-            const F v = load_pack(x + at, l.left);
-            F g = load_pack(grad + at, l.left);
+            const F v = load_piece<FULL>(x + at, l.left);
+            F g = load_piece<FULL>(grad + at, l.left);
             const uint32_t bits = p.mask[(board + y) * p.nvec + l.j];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -398,7 +539,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_sums(const T* __rest
                 s1[i] += g[i];
                 s2[i] += g[i] * (v[i] - mean[i]);
             }
-            if (GATED) store_pack(dresidual + at, g, l.left);
+            if (GATED) store_piece<FULL>(dresidual + at, g, l.left);
         }
     }
     float *a = GATED ? p.s1 : p.part_a, *b = GATED ? p.s2 : p.part_b;
@@ -408,7 +549,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_sums(const T* __rest
     });
 }
 
-template <typename T, bool GATED>
+template <typename T, bool FULL, bool GATED>
 __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_apply(const T* __restrict__ x, const T* __restrict__ grad,
                                                                   T* __restrict__ dx, const NormParams p, int wide, uint32_t joins) {
     constexpr int V = Pack<T>::V;
@@ -431,15 +572,15 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_apply(const T* __res
 #pragma unroll 4
     for (int y = l.ty; y < p.hw; y += l.step) {
         const size_t at = (board + y) * p.c + l.c;
-        const F v = load_pack(x + at, l.left);
-        F g = load_pack(grad + at, l.left);
+        const F v = load_piece<FULL>(x + at, l.left);
+        F g = load_piece<FULL>(grad + at, l.left);
         const uint32_t bits = GATED ? 0 : p.mask[(board + y) * p.nvec + l.j];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             if (!GATED) g[i] = bits >> i & 1 ? g[i] : 0.f;
             g[i] = g[i] * a[i] + ((v[i] - mean[i]) * b[i] + d[i]);
         }
-        store_pack(dx + at, g, l.left);
+        store_piece<FULL>(dx + at, g, l.left);
     }
 }
 
@@ -600,10 +741,14 @@ __device__ inline void columns_times(const float* w, int rows, int cols, const f
 #pragma unroll
         for (int i = 0; i < 4; ++i) part[(y * wide + x) * 4 + i] = s[i];
         __syncthreads();
-        for (int i = threadIdx.x; i < wide * 4 && at * 4 + i < cols; i += GATE_THREADS) {
-            f32x4 t = part[i];
-            for (int q = 1; q < parts; ++q) t += part[q * wide * 4 + i];
-            out(at * 4 + i, t);
+        const int share = GATE_THREADS / (wide * 4) > 64 ? 64 : wide * 4 < GATE_THREADS ? GATE_THREADS / (wide * 4) : 1;   // lanes to a sum
+        for (int i = threadIdx.x / share; i < wide * 4; i += GATE_THREADS / share) {
+            f32x4 t = 0.f;
+            for (int q = threadIdx.x % share; q < parts; q += share) t += part[q * wide * 4 + i];
+            for (int off = 1; off < share; off <<= 1)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) t[r] += __shfl_xor(t[r], off);
+            if (threadIdx.x % share == 0 && at * 4 + i < cols) out(at * 4 + i, t);
         }
         __syncthreads();
     }
@@ -807,21 +952,36 @@ __global__ __launch_bounds__(CHANNELS * LINES) void k_param_grads(const NormPara
 }
 
 // ---------------------------------------------------------------------------------------------- host side
-// Lanes to a row: a piece of 16 bytes each, as many as the row has, up to 16 (a longer row takes several rounds).
-template <typename F>
-static void with_lanes(int nvec, F&& f) {
-    if (nvec <= 4) f(std::integral_constant<int, 4>());
-    else if (nvec <= 8) f(std::integral_constant<int, 8>());
-    else f(std::integral_constant<int, 16>());
+// f(lanes to a row, how the row fits them)
+template <typename T, typename F>
+static void with_lanes(const NormParams& p, F&& f) {
+    constexpr int V = Pack<T>::V;
+    typedef std::integral_constant<Fit, EXACT> Exact;
+    typedef std::integral_constant<Fit, ONE> One;
+    if (p.hw == 8 * V) f(std::integral_constant<int, 8>(), Exact());
+    else if (p.hw == 16 * V) f(std::integral_constant<int, 16>(), Exact());
+    else if (p.hw < V || p.nvec > 64) f(std::integral_constant<int, 16>(), std::integral_constant<Fit, LOOP>());
+    else if (p.nvec <= 8) f(std::integral_constant<int, 8>(), One());
+    else if (p.nvec <= 16) f(std::integral_constant<int, 16>(), One());
+    else if (p.nvec <= 32) f(std::integral_constant<int, 32>(), One());
+    else f(std::integral_constant<int, 64>(), One());
+}
+
+// f(whether the channels are at least one piece of 16 bytes)
+template <typename T, typename F>
+static void with_pieces(const NormParams& p, F&& f) {
+    if (p.c >= Pack<T>::V) f(std::true_type());
+    else f(std::false_type());
 }
 
 // Which boards a chunk of the pass over the activations holds.
+template <typename T>
 static void set_chunks(NormParams& p, bool last) {
     p.chunk_boards = p.abreast = 1;
     p.chunks = p.n;
     if (last) return;
-    with_lanes(p.nvec, [&](auto L) {
-        const RowGrid g = row_grid<decltype(L)::value>(p);
+    with_lanes<T>(p, [&](auto L, auto) {
+        const RowGrid g = row_grid(p, L);
         p.chunk_boards = BOARDS_AT_ONCE;
         p.abreast = (int)g.abreast;
         p.chunks = (int64_t)(g.blocks / g.across) * g.abreast;
@@ -832,12 +992,12 @@ template <typename T, bool GATED>
 static int norm_forward(NormParams p, bool last, const T* x, const T* residual, T* out, hipStream_t s) {
     const int wide = p.nvec < 64 ? p.nvec : 64;
     const dim3 boards((uint32_t)p.n, (p.nvec + wide - 1) / wide), block(NORM_THREADS);
-    set_chunks(p, last);
+    set_chunks<T>(p, last);
     if (p.training || GATED) {
-        if (last) hipLaunchKernelGGL((k_last_stats<T, GATED>), boards, block, 0, s, x, p, wide);
-        else with_lanes(p.nvec, [&](auto L) {
-            const RowGrid g = row_grid<decltype(L)::value>(p);
-            hipLaunchKernelGGL((k_row_stats<T, decltype(L)::value, GATED>), dim3(g.blocks), block, 0, s, x, p, g);
+        if (last) with_pieces<T>(p, [&](auto full) { hipLaunchKernelGGL((k_last_stats<T, decltype(full)::value, GATED>), boards, block, 0, s, x, p, wide); });
+        else with_lanes<T>(p, [&](auto L, auto fit) {
+            const RowGrid g = row_grid(p, L);
+            hipLaunchKernelGGL((k_row_stats<T, decltype(L)::value, decltype(fit)::value, GATED>), dim3(g.blocks), block, 0, s, x, p, g);
         });
         AZ_HIP(hipGetLastError());
     }
@@ -848,10 +1008,10 @@ static int norm_forward(NormParams p, bool last, const T* x, const T* residual, 
                            sizeof(f32x4) * (3 * p.c + p.hidden), s, p);
         AZ_HIP(hipGetLastError());
     }
-    if (last) hipLaunchKernelGGL((k_last_apply<T, GATED>), boards, block, 0, s, x, residual, out, p, wide);
-    else with_lanes(p.nvec, [&](auto L) {
-        const RowGrid g = row_grid<decltype(L)::value>(p);
-        hipLaunchKernelGGL((k_row_apply<T, decltype(L)::value, GATED>), dim3(g.blocks), block, 0, s, x, residual, out, p, g);
+    if (last) with_pieces<T>(p, [&](auto full) { hipLaunchKernelGGL((k_last_apply<T, decltype(full)::value, GATED>), boards, block, 0, s, x, residual, out, p, wide); });
+    else with_lanes<T>(p, [&](auto L, auto fit) {
+        const RowGrid g = row_grid(p, L);
+        hipLaunchKernelGGL((k_row_apply<T, decltype(L)::value, decltype(fit)::value, GATED>), dim3(g.blocks), block, 0, s, x, residual, out, p, g);
     });
     AZ_HIP(hipGetLastError());
     return AZ_OK;
@@ -861,11 +1021,11 @@ template <typename T, bool GATED>
 static int norm_backward(NormParams p, bool last, const T* x, const T* grad, T* dx, T* dresidual, hipStream_t s) {
     const int wide = p.nvec < 64 ? p.nvec : 64;
     const dim3 boards((uint32_t)p.n, (p.nvec + wide - 1) / wide), block(NORM_THREADS);
-    set_chunks(p, last);
-    if (last) hipLaunchKernelGGL((k_last_grad_sums<T, GATED>), boards, block, 0, s, x, grad, dresidual, p, wide);
-    else with_lanes(p.nvec, [&](auto L) {
-        const RowGrid g = row_grid<decltype(L)::value>(p);
-        hipLaunchKernelGGL((k_row_grad_sums<T, decltype(L)::value, GATED>), dim3(g.blocks), block, 0, s, x, grad, dresidual, p, g);
+    set_chunks<T>(p, last);
+    if (last) with_pieces<T>(p, [&](auto full) { hipLaunchKernelGGL((k_last_grad_sums<T, decltype(full)::value, GATED>), boards, block, 0, s, x, grad, dresidual, p, wide); });
+    else with_lanes<T>(p, [&](auto L, auto fit) {
+        const RowGrid g = row_grid(p, L);
+        hipLaunchKernelGGL((k_row_grad_sums<T, decltype(L)::value, decltype(fit)::value, GATED>), dim3(g.blocks), block, 0, s, x, grad, dresidual, p, g);
     });
     AZ_HIP(hipGetLastError());
     if (GATED) {
@@ -879,10 +1039,10 @@ static int norm_backward(NormParams p, bool last, const T* x, const T* grad, T* 
     AZ_HIP(hipGetLastError());
     const T* masked = GATED ? dresidual : grad;
     const uint32_t joins = (uint32_t)join_blocks(p);
-    if (last) hipLaunchKernelGGL((k_last_grad_apply<T, GATED>), dim3(boards.x + joins, boards.y), block, 0, s, x, masked, dx, p, wide, joins);
-    else with_lanes(p.nvec, [&](auto L) {
-        const RowGrid g = row_grid<decltype(L)::value>(p);
-        hipLaunchKernelGGL((k_row_grad_apply<T, decltype(L)::value, GATED>), dim3(g.blocks + joins), block, 0, s, x, masked, dx, p, g, joins);
+    if (last) with_pieces<T>(p, [&](auto full) { hipLaunchKernelGGL((k_last_grad_apply<T, decltype(full)::value, GATED>), dim3(boards.x + joins, boards.y), block, 0, s, x, masked, dx, p, wide, joins); });
+    else with_lanes<T>(p, [&](auto L, auto fit) {
+        const RowGrid g = row_grid(p, L);
+        hipLaunchKernelGGL((k_row_grad_apply<T, decltype(L)::value, decltype(fit)::value, GATED>), dim3(g.blocks + joins), block, 0, s, x, masked, dx, p, g, joins);
     });
     AZ_HIP(hipGetLastError());
     return AZ_OK;

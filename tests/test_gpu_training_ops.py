@@ -186,25 +186,31 @@ def test_norms_at_the_default_batch_equal_the_torch_modules(hidden):
 
 
 def test_norm_gradient_against_differences():
-    """Directional derivatives of <out, grad> along random directions of x, residual and every parameter.  With a step of
-    2^-7 the second-order error of the central difference is step^2 times the third derivative (order one here): 1e-4;
-    float32 noise is 1e-7 / step; crossings of the ReLU's border move the difference by their share of the values,
-    step times the density: 1e-2 of the derivative's scale, the norm of gradient times direction."""
-    from alphazero_amd import ops
+    """The kernels' gradients along random directions of x, residual and every parameter against central differences of the
+    float64 forward pass.  Across a ReLU's border a difference is no derivative: the step is halved until neither a hidden
+    unit nor an output that receives gradient changes sides.  Allowed: the chain's half-steps on every gradient's
+    magnitude, as above, and step^2 (2^-36) times a third derivative of the derivative's own size for the difference."""
     t = norm_inputs(6, 16, 8, 8, 4, torch.float32, seed=9)
     names = ["x", "residual", "weight", "bias", "fc1_weight", "fc1_bias", "fc2_weight", "fc2_bias"]
-    got = run_norm(t)
+    got, (ref, _, _) = run_norm(t), norm_reference(t, True)
+    k = 64 + 64 + 16 + 6 + 4
+    gen = torch.Generator("cuda").manual_seed(21)
 
-    def value(u):
-        out = ops.norm_gate_residual(u["x"], u["residual"], u["weight"], u["bias"], None, None, u["fc1_weight"], u["fc1_bias"], u["fc2_weight"], u["fc2_bias"])
-        return float((out.double() * t["grad"].double()).sum())
+    def at(name, value):
+        r, pre, hid = norm_reference({**t, name: value}, True)
+        return float((r["out"][0] * t["grad"].double()).sum()), (pre > 0) | (t["grad"] == 0), hid > 0
     for name in names:
-        d = torch.randn_like(t[name])
-        step = 2.0 ** -7
-        diff = (value({**t, name: t[name] + step * d}) - value({**t, name: t[name] - step * d})) / (2 * step)
-        slope = float((got[name].double() * d.double()).sum())
-        scale = float((got[name].double() * d.double()).norm()) + 1e-3
-        assert abs(diff - slope) <= 0.1 * scale, (name, diff, slope, scale)
+        d = torch.randn(t[name].shape, device="cuda", generator=gen, dtype=torch.float64)
+        for step in (2.0 ** -j for j in range(18, 26)):
+            up, down = at(name, t[name].double() + step * d), at(name, t[name].double() - step * d)
+            if torch.equal(up[1], down[1]) and torch.equal(up[2], down[2]):
+                break
+        else:
+            raise AssertionError("a border too near")
+        diff = (up[0] - down[0]) / (2 * step)
+        along = got[name].double() * d
+        allowed = k * 2.0 ** -24 * float((ref[name][1] * d.abs()).sum()) + 1e-6 * float(along.norm())
+        assert abs(diff - float(along.sum())) <= allowed, (name, step, diff, float(along.sum()), allowed)
 
 
 @pytest.mark.parametrize("layout", [torch.contiguous_format, torch.channels_last], ids=["nchw", "nhwc"])
