@@ -60,7 +60,8 @@ class NormArgs(C.Structure):
 class LossArgs(C.Structure):
     _fields_ = ([("n", C.c_int64)] + [(k, C.c_int32) for k in ("actions", "outcomes", "dtype")]
                 + [(k, C.c_void_p) for k in ("policy", "wl", "target_pi", "target_wl", "mask", "losses", "stats", "up_loss",
-                                             "up_pi", "up_wl", "dpolicy", "dwl")])
+                                             "up_pi", "up_wl", "dpolicy", "dwl")]
+                + [("grads_ready", C.c_int32)])
 
 
 class AdamConfig(C.Structure):
@@ -119,6 +120,7 @@ _SIGNATURES = {
     "az_norm_sizes": [C.POINTER(NormArgs), C.POINTER(C.c_int64)],
     "az_norm_forward": [C.POINTER(NormArgs), _VP],
     "az_norm_backward": [C.POINTER(NormArgs), _VP],
+    "az_policy_value_loss_ready": [C.POINTER(LossArgs)],
     "az_policy_value_loss_forward": [C.POINTER(LossArgs), _VP],
     "az_policy_value_loss_backward": [C.POINTER(LossArgs), _VP],
     "az_grad_sumsq": [C.c_int32, _VP, _VP, _VP, C.c_int64, _VP],
@@ -173,7 +175,7 @@ def torch_ops():
         except ImportError as e:
             raise AzError(f"alphazero_amd/_azops.so does not load ({e}): build it with alphazero_amd/csrc/build.sh "
                           "(__graft_entry__.build()).  There is no fallback path.") from e
-        names = ("az_last_error", "az_norm_sizes", "az_norm_forward", "az_norm_backward", "az_policy_value_loss_forward",
+        names = ("az_last_error", "az_norm_sizes", "az_norm_forward", "az_norm_backward", "az_policy_value_loss_ready", "az_policy_value_loss_forward",
                  "az_policy_value_loss_backward", "az_grad_sumsq", "az_adam_step")
         _azops.bind({n: C.cast(getattr(L, n), C.c_void_p).value for n in names}, AzError)
         _torch_ops = _azops

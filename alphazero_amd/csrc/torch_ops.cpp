@@ -4,6 +4,8 @@
 // Why this is native: a Python autograd node costs 30 us in the backward pass and 25 us of argument handling per call,
 // and a step over 216 parameters 100 us of list building, where the kernels themselves take 40 to 100 us (measured on the
 // box's host: norm_gate_residual forward + backward 152 us in Python; FusedAdam.step 150 us).
+#include <mutex>
+
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
@@ -30,6 +32,7 @@ struct Entries {
     decltype(&az_norm_sizes) norm_sizes;
     decltype(&az_norm_forward) norm_forward;
     decltype(&az_norm_backward) norm_backward;
+    decltype(&az_policy_value_loss_ready) loss_ready;
     decltype(&az_policy_value_loss_forward) loss_forward;
     decltype(&az_policy_value_loss_backward) loss_backward;
     decltype(&az_grad_sumsq) grad_sumsq;
@@ -245,12 +248,18 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
     }
 
     static variable_list forward(AutogradContext* ctx, const Tensor& policy, const Tensor& wl, const Tensor& target_pi,
-                                 const Tensor& target_wl, const MaybeTensor& mask_) {
+                                 const Tensor& target_wl, const MaybeTensor& mask_, bool differentiated) {
         const Tensor mask = held(mask_);
         const c10::DeviceGuard guard(policy.device());
         const Tensor losses = floats(3, policy), stats = floats(8 * policy.size(0), policy);
         az_loss_args a = arguments(policy, wl, target_pi, target_wl, mask, stats);
         a.losses_dev = ptr<float>(losses);
+        if (differentiated && lib.loss_ready(&a)) {
+            const Tensor dpolicy = at::empty_like(policy), dwl = at::empty_like(wl);
+            a.dpolicy_dev = dpolicy.data_ptr();
+            a.dwl_dev = dwl.data_ptr();
+            ctx->saved_data["grads"] = std::vector<Tensor>{dpolicy, dwl};
+        }
         check(lib.loss_forward(&a, stream_of(policy)));
         ctx->save_for_backward({policy, wl, target_pi, target_wl, mask, stats});
         ctx->set_materialize_grads(false);
@@ -260,12 +269,27 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto s = ctx->get_saved_variables();
         const c10::DeviceGuard guard(s[0].device());
-        variable_list out(5);
+        variable_list out(6);
         {
             const at::NoGradGuard no_grad;
-            out[0] = at::empty_like(s[0]);
-            out[1] = at::empty_like(s[1]);
             az_loss_args a = arguments(s[0], s[1], s[2], s[3], s[4], s[5]);
+            // the forward pass's gradients serve one backward pass (they are scaled in place and belong to whoever gets them)
+            static std::mutex taking;
+            {
+                const std::lock_guard<std::mutex> lock(taking);
+                const auto ready = ctx->saved_data.find("grads");
+                if (ready != ctx->saved_data.end()) {
+                    const auto held = ready->second.toTensorVector();
+                    out[0] = held[0];
+                    out[1] = held[1];
+                    a.grads_ready = 1;
+                    ctx->saved_data.erase(ready);
+                }
+            }
+            if (!a.grads_ready) {
+                out[0] = at::empty_like(s[0]);
+                out[1] = at::empty_like(s[1]);
+            }
             for (int i = 0; i < 3; ++i) a.upstream_dev[i] = ptr<float>(grads[i]);
             a.dpolicy_dev = out[0].data_ptr();
             a.dwl_dev = out[1].data_ptr();
@@ -297,7 +321,8 @@ py::tuple policy_value_loss(const Tensor& policy, const Tensor& wl, const Tensor
                           (!mask || mask->device() == policy.device()),
                       "all tensors must be on ", policy.device());
     const auto r = LossFunction::apply(policy.contiguous(), wl.contiguous(), target_pi.contiguous(), target_wl.contiguous(),
-                                       mask ? MaybeTensor(mask->contiguous()) : mask);
+                                       mask ? MaybeTensor(mask->contiguous()) : mask,
+                                       at::GradMode::is_enabled() && (policy.requires_grad() || wl.requires_grad()));
     return py::make_tuple(r[0], r[1], r[2]);
 }
 
@@ -430,6 +455,7 @@ PYBIND11_MODULE(_azops, m) {
         set(lib.norm_sizes, a, "az_norm_sizes");
         set(lib.norm_forward, a, "az_norm_forward");
         set(lib.norm_backward, a, "az_norm_backward");
+        set(lib.loss_ready, a, "az_policy_value_loss_ready");
         set(lib.loss_forward, a, "az_policy_value_loss_forward");
         set(lib.loss_backward, a, "az_policy_value_loss_backward");
         set(lib.grad_sumsq, a, "az_grad_sumsq");

@@ -6,6 +6,12 @@
 // One pass keeps (m, S, T, U) in registers: when the maximum grows by d, S shrinks by exp(-d) and U grows by d T.  A place
 // whose target is zero adds nothing whatever its logit; a row that keeps nothing has loss 0 and gradient 0.
 //
+// Where the row fits a workgroup's registers (8192 actions) it is read once: first the maximum, then the sums, then the
+// gradient for an upstream of 1, written by the same kernel.  The backward pass then only looks at the upstream and, if
+// it is 1 (as it is when the loss itself is what backward() starts from), leaves what is there.  In float16 a gradient
+// divided by the rows and not yet multiplied with the program's loss scale would underflow: there, for longer rows and for
+// a second backward pass the gradient is computed from the logits again.
+//
 // What bounds it: memory at large action spaces, launches at small ones.  All sums in 32 bits; rows are added in 64 bits
 // in a fixed order.
 #include <math.h>
@@ -20,7 +26,7 @@ struct LossParams {
     const void *policy, *wl;
     const float *target_pi, *target_wl;
     const uint8_t* mask;
-    float* stats;              // [2n][4]: m, 1 / S, T, loss: the policy's rows, then the outcome's
+    float *loss, *top, *inv, *total;   // [2n]: loss, m, 1 / S, T: the policy's rows, then the outcome's
     const float* upstream[3];  // gradients of (loss, policy loss, outcome loss), each may be null
     void *dpolicy, *dwl;
     int n, actions, outcomes;
@@ -60,17 +66,18 @@ __device__ inline RowSum join_lanes(RowSum r) {
     return r;
 }
 
-__device__ inline f32x4 row_stats(const RowSum& r) {
-    f32x4 s;
-    s[0] = r.m;
-    s[1] = r.T == 0.f && r.S == 0.f ? 0.f : 1.f / r.S;
-    s[2] = r.T;
-    s[3] = r.T == 0.f && r.U == 0.f && !(r.S != r.S) ? 0.f : r.T * logf(r.S) + r.U;
-    return s;
+__device__ inline void put_row(const LossParams& p, size_t at, const RowSum& r) {
+    p.top[at] = r.m;
+    p.inv[at] = r.T == 0.f && r.S == 0.f ? 0.f : 1.f / r.S;
+    p.total[at] = r.T;
+    p.loss[at] = r.T == 0.f && r.U == 0.f && !(r.S != r.S) ? 0.f : r.T * logf(r.S) + r.U;
 }
 
+// weight: T / S; up: upstream / rows
+__device__ inline float gradient(float z, float t, float m, float weight, float up) { return (__expf(z - m) * weight - t) * up; }
+
 // One outcome row by one thread: two or three classes.
-template <typename T>
+template <typename T, bool GRAD>
 __device__ void outcome_forward(const LossParams& p, int row) {
     const T* z = (const T*)p.wl + (size_t)row * p.outcomes;
     const float* t = p.target_wl + (size_t)row * p.outcomes;
@@ -80,16 +87,117 @@ __device__ void outcome_forward(const LossParams& p, int row) {
         raise(r, zi);
         absorb(r, zi, t[i]);
     }
-    *(f32x4*)(p.stats + 4 * ((size_t)p.n + row)) = row_stats(r);
+    put_row(p, (size_t)p.n + row, r);
+    if (GRAD) {
+        const float weight = 1.f / r.S * r.T, up = 1.f / (float)p.n;
+        for (int i = 0; i < p.outcomes; ++i) ((T*)p.dwl)[(size_t)row * p.outcomes + i] = (T)gradient((float)z[i], t[i], r.m, weight, up);
+    }
 }
 
-// GROUP threads to a policy row: a wavefront up to 1024 actions, a workgroup above.
+// Sums over a group's threads, in all of them.
+template <int GROUP>
+__device__ inline float group_max(float v, float* red) {
+    v = lane_max<64>(v);
+    if (GROUP == 64) return v;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+    for (int w = 1; w < GROUP / 64; ++w) v = fmaxf(v, red[w]);
+    return v;
+}
+
+// A row in the registers of GROUP threads, PIECES pieces of 16 bytes each (actions: at least one piece, at most
+// GROUP * PIECES).  The last piece is moved back to end with the row: what it shares with its neighbour is left out of
+// the sums and written twice, the same.
+template <typename T, int GROUP, int PIECES, bool GRAD>
+__global__ __launch_bounds__(LOSS_THREADS) void k_loss_row(const LossParams p, int policy_blocks) {
+    constexpr int V = Pack<T>::V, ROWS = LOSS_THREADS / GROUP, WAVES = LOSS_THREADS / 64;
+    __shared__ float red[4][WAVES];
+    if ((int)blockIdx.x >= policy_blocks) {
+        const int row = ((int)blockIdx.x - policy_blocks) * LOSS_THREADS + threadIdx.x;
+        if (row < p.n) outcome_forward<T, GRAD>(p, row);
+        return;
+    }
+    const int row = blockIdx.x * ROWS + threadIdx.x / GROUP, lane = threadIdx.x % GROUP;
+    const size_t base = (size_t)(row < p.n ? row : 0) * p.actions;
+    typedef uint8_t bytes_t __attribute__((ext_vector_type(V)));
+    typedef bytes_t loose_bytes __attribute__((aligned(1)));
+    typename Pack<T>::raw raw[PIECES];
+    f32x4 t[PIECES][V / 4];
+    bytes_t legal[PIECES];
+    int off[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int at = (i * GROUP + lane) * V;
+        off[i] = at < p.actions - V ? at : p.actions - V;
+        raw[i] = *(const typename Pack<T>::loose*)((const T*)p.policy + base + off[i]);
+#pragma unroll
+        for (int k = 0; k < V / 4; ++k) t[i][k] = *(const f32x4_loose*)(p.target_pi + base + off[i] + 4 * k);
+        if (p.mask) legal[i] = *(const loose_bytes*)(p.mask + base + off[i]);
+    }
+    float z[PIECES][V], top = -INFINITY;
+    uint32_t keep[PIECES];                       // legal places of the piece
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        keep[i] = 0;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            z[i][k] = (float)raw[i][k];
+            const bool on = !p.mask || legal[i][k];
+            keep[i] |= (on ? 1u : 0u) << k;
+            if (on) top = fmaxf(top, z[i][k]);
+        }
+    }
+    top = group_max<GROUP>(top, red[3]);
+    RowSum r = {top, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int own = (i * GROUP + lane) * V - off[i];            // the first place that is not the neighbour's
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if ((keep[i] >> k & 1) && k >= own) absorb(r, z[i][k], t[i][k / 4][k % 4]);
+    }
+    r.S = lane_sum<64>(r.S);
+    r.T = lane_sum<64>(r.T);
+    r.U = lane_sum<64>(r.U);
+    if (GROUP > 64) {
+        if ((threadIdx.x & 63) == 0) {
+            red[0][threadIdx.x >> 6] = r.S;
+            red[1][threadIdx.x >> 6] = r.T;
+            red[2][threadIdx.x >> 6] = r.U;
+        }
+        __syncthreads();
+        r.S = red[0][0];
+        r.T = red[1][0];
+        r.U = red[2][0];
+        for (int w = 1; w < WAVES; ++w) {
+            r.S += red[0][w];
+            r.T += red[1][w];
+            r.U += red[2][w];
+        }
+    }
+    if (row >= p.n) return;
+    if (lane == 0) put_row(p, row, r);
+    if (GRAD) {
+        const float weight = (r.T == 0.f && r.S == 0.f ? 0.f : 1.f / r.S) * r.T, up = 1.f / (float)p.n;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            if ((i * GROUP + lane) * V >= p.actions) break;
+            typename Pack<T>::f32 g;
+#pragma unroll
+            for (int k = 0; k < V; ++k) g[k] = keep[i] >> k & 1 ? gradient(z[i][k], t[i][k / 4][k % 4], r.m, weight, up) : 0.f;
+            *(typename Pack<T>::loose*)((T*)p.dpolicy + base + off[i]) = __builtin_convertvector(g, typename Pack<T>::raw);
+        }
+    }
+}
+
+// Any row: a wavefront up to 1024 actions, a workgroup above; (m, S, T, U) on the way.
 template <typename T, int GROUP>
 __global__ __launch_bounds__(LOSS_THREADS) void k_loss_forward(const LossParams p, int policy_blocks) {
     constexpr int V = Pack<T>::V, ROWS = LOSS_THREADS / GROUP;
     if ((int)blockIdx.x >= policy_blocks) {
         const int row = ((int)blockIdx.x - policy_blocks) * LOSS_THREADS + threadIdx.x;
-        if (row < p.n) outcome_forward<T>(p, row);
+        if (row < p.n) outcome_forward<T, false>(p, row);
         return;
     }
     const int row = blockIdx.x * ROWS + threadIdx.x / GROUP, lane = threadIdx.x % GROUP;
@@ -121,24 +229,25 @@ __global__ __launch_bounds__(LOSS_THREADS) void k_loss_forward(const LossParams 
     }
     r = join_lanes(r);
     if (GROUP == 64) {
-        if (lane == 0 && row < p.n) *(f32x4*)(p.stats + 4 * (size_t)row) = row_stats(r);
+        if (lane == 0 && row < p.n) put_row(p, row, r);
     } else {
         __shared__ RowSum part[LOSS_THREADS / 64];
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = r;
         __syncthreads();
         if (threadIdx.x == 0) {
             for (int w = 1; w < LOSS_THREADS / 64; ++w) r = join(r, part[w]);
-            *(f32x4*)(p.stats + 4 * (size_t)row) = row_stats(r);
+            put_row(p, row, r);
         }
     }
 }
 
 // Means over the rows: losses = (sum, policy, outcome).
-__global__ __launch_bounds__(1024) void k_loss_sum(const float* stats, int n, float* losses) {
+__global__ __launch_bounds__(1024) void k_loss_sum(const float* loss, int n, float* losses) {
     double a = 0.0, b = 0.0;
+#pragma unroll 4
     for (int i = threadIdx.x; i < n; i += 1024) {
-        a += stats[4 * (size_t)i + 3];
-        b += stats[4 * ((size_t)n + i) + 3];
+        a += loss[i];
+        b += loss[(size_t)n + i];
     }
     for (int off = 32; off; off >>= 1) {
         a += __shfl_xor(a, off);
@@ -162,7 +271,26 @@ __global__ __launch_bounds__(1024) void k_loss_sum(const float* stats, int n, fl
 }
 
 __device__ inline float upstream_of(const LossParams& p, int which) {
-    return ((p.upstream[0] ? *p.upstream[0] : 0.f) + (p.upstream[which] ? *p.upstream[which] : 0.f)) / (float)p.n;
+    return (p.upstream[0] ? *p.upstream[0] : 0.f) + (p.upstream[which] ? *p.upstream[which] : 0.f);
+}
+
+// Gradients for an upstream of 1 are there: multiply them with what it is, in place.
+template <typename T>
+__global__ __launch_bounds__(LOSS_THREADS) void k_loss_scale(const LossParams p) {
+    constexpr int V = Pack<T>::V;
+    const float up = upstream_of(p, 1), up_wl = upstream_of(p, 2);
+    const int64_t stride = (int64_t)gridDim.x * LOSS_THREADS, first = (int64_t)blockIdx.x * LOSS_THREADS + threadIdx.x;
+    if (up != 1.f) {
+        const int64_t n = (int64_t)p.n * p.actions;
+        for (int64_t i = first * V; i < n; i += stride * V) {
+            const int left = n - i < V ? (int)(n - i) : V;
+            store_pack((T*)p.dpolicy + i, load_pack((const T*)p.dpolicy + i, left) * up, left);
+        }
+    }
+    if (up_wl != 1.f) {
+        const int64_t n = (int64_t)p.n * p.outcomes;
+        for (int64_t i = first; i < n; i += stride) ((T*)p.dwl)[i] = (T)((float)((T*)p.dwl)[i] * up_wl);
+    }
 }
 
 template <typename T, int GROUP>
@@ -171,19 +299,17 @@ __global__ __launch_bounds__(LOSS_THREADS) void k_loss_backward(const LossParams
     if ((int)blockIdx.x >= policy_blocks) {
         const int row = ((int)blockIdx.x - policy_blocks) * LOSS_THREADS + threadIdx.x;
         if (row >= p.n) return;
-        const float up = upstream_of(p, 2);
-        const f32x4 s = *(const f32x4*)(p.stats + 4 * ((size_t)p.n + row));
+        const float up = upstream_of(p, 2) / (float)p.n, m = p.top[(size_t)p.n + row];
+        const float weight = p.inv[(size_t)p.n + row] * p.total[(size_t)p.n + row];
         for (int i = 0; i < p.outcomes; ++i) {
             const size_t k = (size_t)row * p.outcomes + i;
-            ((T*)p.dwl)[k] = (T)((__expf((float)((const T*)p.wl)[k] - s[0]) * s[1] * s[2] - p.target_wl[k]) * up);
+            ((T*)p.dwl)[k] = (T)gradient((float)((const T*)p.wl)[k], p.target_wl[k], m, weight, up);
         }
         return;
     }
     const int row = blockIdx.x * ROWS + threadIdx.x / GROUP, lane = threadIdx.x % GROUP;
     if (row >= p.n) return;
-    const float up = upstream_of(p, 1);
-    const f32x4 s = *(const f32x4*)(p.stats + 4 * (size_t)row);
-    const float weight = s[1] * s[2];
+    const float up = upstream_of(p, 1) / (float)p.n, m = p.top[row], weight = p.inv[row] * p.total[row];
     const size_t at = (size_t)row * p.actions;
     for (int i = lane * V; i < p.actions; i += GROUP * V) {
         const int left = p.actions - i;
@@ -194,29 +320,54 @@ __global__ __launch_bounds__(LOSS_THREADS) void k_loss_backward(const LossParams
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const bool keep = k + j < left && (!p.mask || p.mask[at + i + k + j]);
-                z[k + j] = keep ? (__expf(z[k + j] - s[0]) * weight - q[j]) * up : 0.f;
+                z[k + j] = keep ? gradient(z[k + j], q[j], m, weight, up) : 0.f;
             }
         }
         store_pack((T*)p.dpolicy + at + i, z, left);
     }
 }
 
+// How many threads a row of so many actions gets, and how it is read: in registers, or (longer than 8192 actions, or
+// shorter than a piece) in rounds.
+template <typename T, bool GRAD>
+static bool launch_row(const LossParams& p, hipStream_t s) {
+    constexpr int V = Pack<T>::V;
+    const dim3 block(LOSS_THREADS);
+    const int outcome_blocks = (p.n + LOSS_THREADS - 1) / LOSS_THREADS, waves = (p.n + 3) / 4;
+    if (p.actions < V || p.actions > 8192) return false;
+    if (p.actions <= 512) hipLaunchKernelGGL((k_loss_row<T, 64, 512 / 64 / V, GRAD>), dim3(waves + outcome_blocks), block, 0, s, p, waves);
+    else if (p.actions <= 2048) hipLaunchKernelGGL((k_loss_row<T, 256, 2048 / 256 / V, GRAD>), dim3(p.n + outcome_blocks), block, 0, s, p, p.n);
+    else if (p.actions <= 4096) hipLaunchKernelGGL((k_loss_row<T, 256, 4096 / 256 / V, GRAD>), dim3(p.n + outcome_blocks), block, 0, s, p, p.n);
+    else hipLaunchKernelGGL((k_loss_row<T, 256, 8192 / 256 / V, GRAD>), dim3(p.n + outcome_blocks), block, 0, s, p, p.n);
+    return true;
+}
+
 template <typename T>
-static int launch_loss(const LossParams& p, float* losses, bool backward, hipStream_t s) {
+static int launch_loss(const LossParams& p, float* losses, bool backward, bool ready, hipStream_t s) {
     const int group = p.actions <= 1024 ? 64 : LOSS_THREADS;
     const int pb = (p.n + LOSS_THREADS / group - 1) / (LOSS_THREADS / group), ob = (p.n + LOSS_THREADS - 1) / LOSS_THREADS;
     const dim3 grid(pb + ob), block(LOSS_THREADS);
-    if (backward) {
+    if (backward && ready) {
+        const int64_t blocks = ((int64_t)p.n * p.actions + LOSS_THREADS * Pack<T>::V - 1) / (LOSS_THREADS * Pack<T>::V) + ob;
+        hipLaunchKernelGGL((k_loss_scale<T>), dim3((uint32_t)(blocks < 1024 ? blocks : 1024)), block, 0, s, p);
+    } else if (backward) {
         if (group == 64) hipLaunchKernelGGL((k_loss_backward<T, 64>), grid, block, 0, s, p, pb);
         else hipLaunchKernelGGL((k_loss_backward<T, LOSS_THREADS>), grid, block, 0, s, p, pb);
     } else {
-        if (group == 64) hipLaunchKernelGGL((k_loss_forward<T, 64>), grid, block, 0, s, p, pb);
-        else hipLaunchKernelGGL((k_loss_forward<T, LOSS_THREADS>), grid, block, 0, s, p, pb);
+        if (!(p.dpolicy ? launch_row<T, true>(p, s) : launch_row<T, false>(p, s))) {
+            if (group == 64) hipLaunchKernelGGL((k_loss_forward<T, 64>), grid, block, 0, s, p, pb);
+            else hipLaunchKernelGGL((k_loss_forward<T, LOSS_THREADS>), grid, block, 0, s, p, pb);
+        }
         AZ_HIP(hipGetLastError());
-        hipLaunchKernelGGL(k_loss_sum, dim3(1), dim3(1024), 0, s, p.stats, p.n, losses);
+        hipLaunchKernelGGL(k_loss_sum, dim3(1), dim3(1024), 0, s, p.loss, p.n, losses);
     }
     AZ_HIP(hipGetLastError());
     return AZ_OK;
+}
+
+// Whether the forward call can write the gradients.
+static bool loss_ready(const az_loss_args* a) {
+    return a->dtype != AZ_F16 && a->actions >= (a->dtype == AZ_F32 ? 4 : 8) && a->actions <= 8192;
 }
 
 static int loss_entry(const az_loss_args* a, bool backward, void* stream) {
@@ -232,7 +383,10 @@ static int loss_entry(const az_loss_args* a, bool backward, void* stream) {
     p.target_pi = a->target_pi_dev;
     p.target_wl = a->target_wl_dev;
     p.mask = a->mask_dev;
-    p.stats = a->stats_dev;
+    p.loss = a->stats_dev;
+    p.top = p.loss + 2 * a->n;
+    p.inv = p.top + 2 * a->n;
+    p.total = p.inv + 2 * a->n;
     for (int i = 0; i < 3; ++i) p.upstream[i] = a->upstream_dev[i];
     p.dpolicy = a->dpolicy_dev;
     p.dwl = a->dwl_dev;
@@ -241,10 +395,13 @@ static int loss_entry(const az_loss_args* a, bool backward, void* stream) {
     p.outcomes = a->outcomes;
     if (backward) AZ_CHECK_ARG(p.dpolicy && p.dwl, "policy/value loss: null gradient");
     else AZ_CHECK_ARG(a->losses_dev, "policy/value loss: null output");
+    AZ_CHECK_ARG(!p.dpolicy == !p.dwl, "policy/value loss: one gradient without the other");
+    AZ_CHECK_ARG(backward ? !a->grads_ready || loss_ready(a) : !p.dpolicy || loss_ready(a),
+                 "policy/value loss: the forward call writes no gradients of type %d with %d actions", a->dtype, a->actions);
     switch (a->dtype) {
-        case AZ_F32: return launch_loss<float>(p, a->losses_dev, backward, (hipStream_t)stream);
-        case AZ_BF16: return launch_loss<__bf16>(p, a->losses_dev, backward, (hipStream_t)stream);
-        case AZ_F16: return launch_loss<_Float16>(p, a->losses_dev, backward, (hipStream_t)stream);
+        case AZ_F32: return launch_loss<float>(p, a->losses_dev, backward, a->grads_ready != 0, (hipStream_t)stream);
+        case AZ_BF16: return launch_loss<__bf16>(p, a->losses_dev, backward, a->grads_ready != 0, (hipStream_t)stream);
+        case AZ_F16: return launch_loss<_Float16>(p, a->losses_dev, backward, a->grads_ready != 0, (hipStream_t)stream);
     }
     AZ_FAIL(AZ_ERR_ARG, "policy/value loss: unknown type %d", a->dtype);
 }
@@ -253,3 +410,4 @@ static int loss_entry(const az_loss_args* a, bool backward, void* stream) {
 
 extern "C" int az_policy_value_loss_forward(const az_loss_args* args, void* stream) { return az::loss_entry(args, false, stream); }
 extern "C" int az_policy_value_loss_backward(const az_loss_args* args, void* stream) { return az::loss_entry(args, true, stream); }
+extern "C" int az_policy_value_loss_ready(const az_loss_args* args) { return args && az::loss_ready(args) ? 1 : 0; }

@@ -372,7 +372,11 @@ int az_norm_backward(const az_norm_args* args, void* stream);
  * policy [n][actions] and wl [n][outcomes] (src/parallel_trainer.py:251-260).  mask_dev
  * ([n][actions] bytes, may be null): places with 0 take no part, whatever they hold; a row
  * without any has loss 0.  stats_dev: 8 n floats, 16-byte aligned, filled by the forward call and
- * read by the backward call.  upstream_dev: gradients of the three losses, null = 0. */
+ * read by the backward call.  upstream_dev: gradients of the three losses, null = 0.
+ * Where az_policy_value_loss_ready answers 1 (float32 and bfloat16, one piece of 16 bytes to 8192
+ * actions), the forward call also writes the gradients for an upstream of 1 if dpolicy_dev and dwl_dev
+ * are given; a backward call with grads_ready != 0 then only multiplies them, in place, with an
+ * upstream that is not 1. */
 typedef struct {
     int64_t n;
     int32_t actions, outcomes, dtype;
@@ -382,7 +386,9 @@ typedef struct {
     float *losses_dev, *stats_dev;
     const float* upstream_dev[3];
     void *dpolicy_dev, *dwl_dev;
+    int32_t grads_ready;
 } az_loss_args;
+int az_policy_value_loss_ready(const az_loss_args* args);
 int az_policy_value_loss_forward(const az_loss_args* args, void* stream);
 int az_policy_value_loss_backward(const az_loss_args* args, void* stream);
 
