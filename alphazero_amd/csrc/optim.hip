@@ -4,13 +4,18 @@
 //   c = min(1, max_norm / (|g| + 1e-6))                  |g| over all gradients, summed in 64 bits
 //   g = c g (+ wd p: weight decay in the gradient)        m = b1 m + (1 - b1) g        v = b2 v + (1 - b2) g^2
 //   p = p (- lr wd p: decoupled decay) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
-// Every operation is rounded on its own to 32 bits (this file is built without contraction), so a step is the same
-// numbers as the same operations in elementary tensor code.
+// Every operation on the moments is rounded on its own to 32 bits (this file is built without contraction, the root is
+// correctly rounded), so they are the same numbers as the same operations in elementary tensor code, and so are the codes
+// that they become in 8 bits.  The quotient is a product with the hardware's reciprocal: one last place of the update.
 //
 // What bounds it: memory.  A 32-bit step reads 16 and writes 12 bytes per weight, an 8-bit one 10 and 6; clipping reads
-// the gradients once more.  The pointers travel in the kernel arguments (at most AZ_OPTIM_TABLE tensors a launch):
-// nothing is uploaded, so the step can be captured, and tensors may move between steps.
+// the gradients once more.
+// Layout: a workgroup takes a piece of OPT_CHUNK elements of one tensor.  Which one is in a table that is made once, in
+// device memory; the tensors' addresses travel in the kernel arguments (OPT_TABLE tensors a launch, so that the default
+// network's 214 are one), nothing is uploaded per step: it can be captured, and tensors may move between steps.
 #include <math.h>
+
+#include <type_traits>
 
 #include "train_common.h"
 
@@ -19,21 +24,21 @@ namespace az {
 constexpr int OPT_THREADS = 256;
 constexpr int OPT_CHUNK = AZ_OPTIM_CHUNK;          // elements of one tensor that one workgroup takes
 constexpr int OPT_BLOCK = AZ_OPTIM_PAD;            // elements that share a scale: one wavefront x 4
-constexpr int OPT_TABLE = 136;                     // 28 bytes each: 3.8 KB of the 4 KB of kernel arguments
-constexpr int OPT_SLOTS = 960;
+constexpr int OPT_ROUNDS = OPT_CHUNK / (OPT_THREADS * 4);
+constexpr int OPT_TABLE = 240;                     // 16 bytes each: 3.75 of the 4 KB of kernel arguments
+constexpr int OPT_MASK = 896;                      // words: 28,672 tensors a launch of k_adam_begin
 static_assert(OPT_CHUNK % (OPT_THREADS * 4) == 0 && OPT_BLOCK == 256, "a wavefront covers one block of a moment");
 
-struct OptTable {
-    uint64_t grad[OPT_TABLE];
-    uint64_t param[OPT_TABLE];
-    uint32_t first[OPT_TABLE];      // first workgroup of the tensor in this launch
-    uint32_t offset[OPT_TABLE];     // its place in the moments, in units of OPT_BLOCK
-    uint32_t slot_tail[OPT_TABLE];  // step counter (20 bits) | elements of the last chunk - 1 (12 bits)
-    uint32_t count, chunks;
+struct GradTable {
+    uint64_t grad[OPT_TABLE];       // 0: none, the tensor is left alone
 };
 
-struct SlotList {
-    uint32_t slot[OPT_SLOTS];
+struct TensorTable {
+    uint64_t grad[OPT_TABLE], param[OPT_TABLE];
+};
+
+struct TensorMask {
+    uint32_t has_grad[OPT_MASK];
 };
 
 struct StepFactors {                // per tensor, from its step counter
@@ -55,51 +60,43 @@ struct OptHyper {
 struct AdamParams {
     float beta1, one_beta1, beta2, one_beta2, eps, decay;   // decay: wd, or 1 - lr wd
     int decoupled;
+    const az_adam_piece* pieces;
+    uint32_t first_tensor;
     const float* coef;
     const StepFactors* factors;
     void *m, *v;
     float *m_scale, *v_scale;
 };
 
-// The tensor that workgroup b works on.  Every lane compares its part of `first`: one round trip instead of the
-// eight of a search by halves.
-__device__ inline uint32_t find_tensor(const OptTable& t, uint32_t b) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t n = 0;
-#pragma unroll
-    for (uint32_t k = 0; k < OPT_TABLE; k += 64) {
-        const uint32_t i = k + lane;
-        const bool at_or_before = i < t.count && t.first[i < OPT_TABLE ? i : 0] <= b;
-        n += __popcll(__ballot(at_or_before));
-    }
-    return __builtin_amdgcn_readfirstlane(n - 1);
+// f(whether the piece is whole): a whole piece's loads are issued together, the last one of a tensor goes round by round.
+template <typename F>
+__device__ inline void with_whole(const az_adam_piece& c, F&& f) {
+    if (c.n == OPT_CHUNK) f(std::true_type());
+    else f(std::false_type());
 }
 
-struct Chunk {
-    uint32_t tensor, index, n;     // which tensor, which chunk of it, its elements
-};
-
-__device__ inline Chunk find_chunk(const OptTable& t, uint32_t b) {
-    Chunk c;
-    c.tensor = find_tensor(t, b);
-    c.index = b - t.first[c.tensor];
-    const uint32_t end = c.tensor + 1 < t.count ? t.first[c.tensor + 1] : t.chunks;
-    c.n = b + 1 == end ? (t.slot_tail[c.tensor] >> 20) + 1 : OPT_CHUNK;
-    return c;
+template <bool WHOLE>
+__device__ inline f32x4 load_four(const float* p, int i, const az_adam_piece& c) {
+    return WHOLE ? *(const f32x4_loose*)(p + i) : load_pack(p + i, (int)c.n - i);
 }
 
-// Sum of squares of a chunk in 64 bits (the products are exact there): the norm of 8 M gradients whose sizes lie decades
+// Sum of squares of a piece in 64 bits (the products are exact there): the norm of 8 M gradients whose sizes lie decades
 // apart, and a clipping factor that does not depend on the order of the sum.
-__global__ __launch_bounds__(OPT_THREADS) void k_grad_sumsq(const OptTable t, double* partials) {
-    const Chunk c = find_chunk(t, blockIdx.x);
-    const float* g = (const float*)t.grad[c.tensor] + (size_t)c.index * OPT_CHUNK;
+__global__ __launch_bounds__(OPT_THREADS) void k_grad_sumsq(const GradTable t, const az_adam_piece* pieces, uint32_t first_tensor, double* partials) {
+    const az_adam_piece c = pieces[blockIdx.x];
+    const float* g = (const float*)t.grad[c.tensor - first_tensor];
     double s = 0.0;
+    if (g) {
+        g += (size_t)c.chunk * OPT_CHUNK;
+        with_whole(c, [&](auto whole) {
+            f32x4 v[OPT_ROUNDS];
 #pragma unroll
-    for (int it = 0; it < OPT_CHUNK / (OPT_THREADS * 4); ++it) {
-        const int i = it * OPT_THREADS * 4 + threadIdx.x * 4;
-        const f32x4 v = load_pack(g + i, (int)c.n - i);
+            for (int it = 0; it < OPT_ROUNDS; ++it) v[it] = load_four<decltype(whole)::value>(g, (it * OPT_THREADS + threadIdx.x) * 4, c);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s += (double)v[k] * (double)v[k];
+            for (int it = 0; it < OPT_ROUNDS; ++it)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s += (double)v[it][k] * (double)v[it][k];
+        });
     }
     for (int off = 32; off; off >>= 1) s += __shfl_xor(s, off);
     __shared__ double part[OPT_THREADS / 64];
@@ -113,9 +110,10 @@ __global__ __launch_bounds__(OPT_THREADS) void k_grad_sumsq(const OptTable t, do
 
 // One workgroup: the norm and the clipping factor from the partial sums (in a fixed order), and the tensors' step
 // counters with what follows from them.
-__global__ __launch_bounds__(1024) void k_adam_begin(const SlotList l, uint32_t count, OptHyper h) {
+__global__ __launch_bounds__(1024) void k_adam_begin(const TensorMask mask, uint32_t first, uint32_t count, OptHyper h) {
     if (h.coef) {
         double s = 0.0;
+#pragma unroll 4
         for (uint32_t i = threadIdx.x; i < h.n_partials; i += 1024) s += h.partials[i];
         for (int off = 32; off; off >>= 1) s += __shfl_xor(s, off);
         __shared__ double part[16];
@@ -129,15 +127,25 @@ __global__ __launch_bounds__(1024) void k_adam_begin(const SlotList l, uint32_t 
         }
     }
     for (uint32_t i = threadIdx.x; i < count; i += 1024) {
-        const uint32_t slot = l.slot[i];
-        const float t = h.steps[slot] + 1.f;
-        h.steps[slot] = t;
+        if (!(mask.has_grad[i / 32] >> (i % 32) & 1)) continue;
+        const float t = h.steps[first + i] + 1.f;
+        h.steps[first + i] = t;
         StepFactors f;
         f.step_size = (float)(h.lr / (1.0 - pow(h.beta1, (double)t)));
         f.inv_root_bias2 = 1.f / (float)sqrt(1.0 - pow(h.beta2, (double)t));
         f.key = h.seed_key + (uint32_t)t * 0x85EBCA6Bu;
-        h.factors[slot] = f;
+        h.factors[first + i] = f;
     }
+}
+
+// Correctly rounded root of a value that is not denormal: the hardware's, off by at most a last place, and the signs of what
+// is left of v beside its two neighbours.
+__device__ inline float exact_root(float v) {
+    const float r = __builtin_amdgcn_sqrtf(v), below = __uint_as_float(__float_as_uint(r) - 1), above = __uint_as_float(__float_as_uint(r) + 1);
+    float best = r;
+    if (__builtin_fmaf(-below, r, v) <= 0.f) best = below;
+    if (__builtin_fmaf(-above, r, v) > 0.f) best = above;
+    return best;                       // (0 and infinity: the neighbours' remainders are NaN or zero)
 }
 
 // ---- moments in 8 bits -------------------------------------------------------------------------------------------
@@ -147,32 +155,46 @@ __global__ __launch_bounds__(1024) void k_adam_begin(const SlotList l, uint32_t 
 // a code's step (6 %) per step, so rounding to nearest would freeze it: values are rounded at random, up with the
 // probability of the way they have gone, which keeps the averages right.  A root that is not zero never becomes zero
 // (the update would divide by eps alone).  What is not finite becomes the code of NaN.
-__device__ inline float block_top(const f32x4 x) {
-    float top = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float a = fabsf(x[k]);
-        top = fmaxf(top, a <= 3.402823466e38f ? a : 0.f);
-    }
-    return lane_max<64>(top);
+
+// The largest finite magnitude of the wavefront's 256 values, as the bits of a float (those order like integers).
+__device__ inline uint32_t wave_max(uint32_t v) {
+#define AZ_MAX_DPP(CTRL) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true))
+    AZ_MAX_DPP(0xB1);
+    AZ_MAX_DPP(0x4E);
+    AZ_MAX_DPP(0x141);
+    AZ_MAX_DPP(0x140);
+#undef AZ_MAX_DPP
+    v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+    return max(v, (uint32_t)__shfl_xor((int)v, 32));
 }
 
-__device__ inline int scale_exponent(float top) {
-    const uint32_t b = __float_as_uint(top);
-    const int k = (int)(b >> 23) - 127 - 8 + ((b & 0x7FFFFFu) > 0x600000u);
+__device__ inline uint32_t block_top(const f32x4 x) {
+    constexpr uint32_t INF = 0x7F800000u;
+    uint32_t b[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) b[k] = __float_as_uint(x[k]) & 0x7FFFFFFFu;
+    const uint32_t top = wave_max(max(max(b[0], b[1]), max(b[2], b[3])));
+    if (top < INF) return top;               // the same in every lane
+#pragma unroll
+    for (int k = 0; k < 4; ++k) b[k] = b[k] < INF ? b[k] : 0;
+    return wave_max(max(max(b[0], b[1]), max(b[2], b[3])));
+}
+
+__device__ inline int scale_exponent(uint32_t top) {
+    const int k = (int)(top >> 23) - 127 - 8 + ((top & 0x7FFFFFu) > 0x600000u);
     return k < -108 ? -108 : k;
 }
 
 __device__ inline float pow2(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
 
-__device__ inline uint32_t encode(float x, float inv_scale, uint32_t r16, bool keep) {
+// The magnitude of x in units of the scale as a code, rounded by 16 random bits.  From 2^-6 on a code is the float's exponent
+// and its first three mantissa bits: the random bits go on top of what is cut off, as an integer.  Below, codes are
+// multiples of 2^-9.  What is not finite ends above the largest code.
+__device__ inline uint32_t encode(float x, float inv_scale, uint32_t r16) {
     const float y = fabsf(x) * inv_scale;
-    const int e = (int)(__float_as_uint(y) >> 23) - 127, place = (e < -6 ? -6 : e) - 3;
-    const float q = floorf(y * pow2(-place) + (float)r16 * (1.f / 65536.f));
-    uint32_t code = ((uint32_t)(place + 9) << 3) + (uint32_t)q;
-    if (keep && code == 0 && y > 0.f) code = 1;
-    if (!(y <= 448.f)) code = 0x7F;
-    return code | (__float_as_uint(x) >> 31 << 7);
+    const uint32_t code = ((__float_as_uint(y) + (r16 << 4)) >> 20) - (120u << 3);
+    const uint32_t small = (uint32_t)__builtin_fmaf((float)r16, 1.f / 65536.f, y * 512.f);     // both products exact
+    return y < 0.015625f ? small : min(code, 0x7Fu);
 }
 
 __device__ inline f32x4 decode(uint32_t codes, float scale) {
@@ -191,128 +213,174 @@ __device__ inline uint32_t mix32(uint32_t z) {
 }
 
 template <int BITS>
-__global__ __launch_bounds__(OPT_THREADS) void k_adam(const OptTable t, const AdamParams a) {
-    const Chunk c = find_chunk(t, blockIdx.x);
-    const float* gp = (const float*)t.grad[c.tensor] + (size_t)c.index * OPT_CHUNK;
-    float* pp = (float*)t.param[c.tensor] + (size_t)c.index * OPT_CHUNK;
-    const size_t at = (size_t)t.offset[c.tensor] * OPT_BLOCK + (size_t)c.index * OPT_CHUNK;   // place in the moments
-    const StepFactors f = a.factors[t.slot_tail[c.tensor] & 0xFFFFFu];
+__global__ __launch_bounds__(OPT_THREADS) void k_adam(const TensorTable t, const AdamParams a) {
+    const az_adam_piece c = a.pieces[blockIdx.x];
+    const float* gp = (const float*)t.grad[c.tensor - a.first_tensor];
+    if (!gp) return;
+    gp += (size_t)c.chunk * OPT_CHUNK;
+    float* pp = (float*)t.param[c.tensor - a.first_tensor] + (size_t)c.chunk * OPT_CHUNK;
+    const size_t at = (size_t)c.offset * OPT_BLOCK;                 // the piece's place in the moments
+    const StepFactors f = a.factors[c.tensor];
     const float coef = a.coef ? *a.coef : 1.f;
+    with_whole(c, [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        constexpr int AHEAD = WHOLE ? OPT_ROUNDS : 1;          // rounds whose loads are under way together
 #pragma unroll
-    for (int it = 0; it < OPT_CHUNK / (OPT_THREADS * 4); ++it) {
-        const int i = it * OPT_THREADS * 4 + threadIdx.x * 4, left = (int)c.n - i;
-        if (left + (int)(threadIdx.x & 63) * 4 <= 0) break;             // the wavefront's whole block is past the end
-        f32x4 p = load_pack((const float*)pp + i, left), g = load_pack(gp + i, left), m, v;
-        // the moments' own places run on to a multiple of OPT_BLOCK: no tail there
-        if (BITS == 32) {
-            m = *(const f32x4*)((const float*)a.m + at + i);
-            v = *(const f32x4*)((const float*)a.v + at + i);
-        } else {
-            m = decode(*(const uint32_t*)((const uint8_t*)a.m + at + i), a.m_scale[(at + i) / OPT_BLOCK]);
-            v = decode(*(const uint32_t*)((const uint8_t*)a.v + at + i), a.v_scale[(at + i) / OPT_BLOCK]);
-        }
-        f32x4 root;
+        for (int it0 = 0; it0 < OPT_ROUNDS; it0 += AHEAD) {
+            f32x4 p[AHEAD], g[AHEAD], m[AHEAD], v[AHEAD];
+            uint32_t cm[AHEAD], cv[AHEAD];
+            float sm[AHEAD], sv[AHEAD];
+            // a wavefront whose block is past the end of the tensor is done (the moments run on to a whole block)
+            if (!WHOLE && (int)c.n <= (it0 * OPT_THREADS + (int)(threadIdx.x & ~63u)) * 4) return;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float gk = g[k], pk = p[k];
-            if (a.coef) gk = gk * coef;
-            if (a.decoupled) pk = pk * a.decay;
-            else if (a.decay != 0.f) gk = gk + pk * a.decay;
-            const float vk = BITS == 32 ? v[k] : v[k] * v[k];
-            m[k] = m[k] * a.beta1 + gk * a.one_beta1;
-            v[k] = vk * a.beta2 + gk * gk * a.one_beta2;
-            root[k] = sqrtf(v[k]);
-            p[k] = pk - m[k] / (root[k] * f.inv_root_bias2 + a.eps) * f.step_size;
-        }
-        store_pack(pp + i, p, left);
-        if (BITS == 32) {
-            *(f32x4*)((float*)a.m + at + i) = m;
-            *(f32x4*)((float*)a.v + at + i) = v;
-        } else {
-            const int km = scale_exponent(block_top(m)), kv = scale_exponent(block_top(root));
-            uint32_t cm = 0, cv = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t place = (uint32_t)(at + i + k), r = mix32(place + f.key);
-                cm |= encode(m[k], pow2(-km), r & 0xFFFF, false) << (8 * k);
-                cv |= encode(root[k], pow2(-kv), r >> 16, true) << (8 * k);
+            for (int u = 0; u < AHEAD; ++u) {
+                const int i = ((it0 + u) * OPT_THREADS + threadIdx.x) * 4;
+                p[u] = load_four<WHOLE>(pp, i, c);
+                g[u] = load_four<WHOLE>(gp, i, c);
+                if (BITS == 32) {
+                    m[u] = *(const f32x4*)((const float*)a.m + at + i);
+                    v[u] = *(const f32x4*)((const float*)a.v + at + i);
+                } else {
+                    cm[u] = *(const uint32_t*)((const uint8_t*)a.m + at + i);
+                    cv[u] = *(const uint32_t*)((const uint8_t*)a.v + at + i);
+                    sm[u] = a.m_scale[(at + i) / OPT_BLOCK];
+                    sv[u] = a.v_scale[(at + i) / OPT_BLOCK];
+                }
             }
-            *(uint32_t*)((uint8_t*)a.m + at + i) = cm;
-            *(uint32_t*)((uint8_t*)a.v + at + i) = cv;
-            if ((threadIdx.x & 63) == 0) {
-                a.m_scale[(at + i) / OPT_BLOCK] = pow2(km);
-                a.v_scale[(at + i) / OPT_BLOCK] = pow2(kv);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int i = ((it0 + u) * OPT_THREADS + threadIdx.x) * 4;
+                if (BITS == 8) {
+                    m[u] = decode(cm[u], sm[u]);
+                    v[u] = decode(cv[u], sv[u]);
+                }
+                f32x4 root;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float gk = g[u][k], pk = p[u][k];
+                    if (a.coef) gk = gk * coef;
+                    if (a.decoupled) pk = pk * a.decay;
+                    else if (a.decay != 0.f) gk = gk + pk * a.decay;
+                    const float vk = BITS == 32 ? v[u][k] : v[u][k] * v[u][k];
+                    m[u][k] = m[u][k] * a.beta1 + gk * a.one_beta1;
+                    v[u][k] = vk * a.beta2 + gk * gk * a.one_beta2;
+                    root[k] = exact_root(v[u][k]);
+                    p[u][k] = pk - m[u][k] * __builtin_amdgcn_rcpf(root[k] * f.inv_root_bias2 + a.eps) * f.step_size;
+                }
+                if (WHOLE) *(f32x4_loose*)(pp + i) = p[u];
+                else store_pack(pp + i, p[u], (int)c.n - i);
+                if (BITS == 32) {
+                    *(f32x4*)((float*)a.m + at + i) = m[u];
+                    *(f32x4*)((float*)a.v + at + i) = v[u];
+                } else {
+                    const int km = scale_exponent(block_top(m[u])), kv = scale_exponent(block_top(root));
+                    uint32_t em = 0, ev = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t place = (uint32_t)(at + i + k), r = mix32(place + f.key);
+                        em |= (encode(m[u][k], pow2(-km), r & 0xFFFF) | __float_as_uint(m[u][k]) >> 31 << 7) << (8 * k);
+                        const uint32_t code = encode(root[k], pow2(-kv), r >> 16);
+                        ev |= max(code, min(__float_as_uint(root[k]), 1u)) << (8 * k);        // at least 1 unless the root is 0
+                    }
+                    *(uint32_t*)((uint8_t*)a.m + at + i) = em;
+                    *(uint32_t*)((uint8_t*)a.v + at + i) = ev;
+                    if ((threadIdx.x & 63) == 0) {
+                        a.m_scale[(at + i) / OPT_BLOCK] = pow2(km);
+                        a.v_scale[(at + i) / OPT_BLOCK] = pow2(kv);
+                    }
+                }
             }
         }
-    }
+    });
 }
 
-// Splits a list of tensors into launches and calls launch(table, chunks before it).
+static int64_t pieces_of(int64_t n) { return (n + OPT_CHUNK - 1) / OPT_CHUNK; }
+
+// Calls launch(first tensor, tensors, first piece, pieces) for ranges of OPT_TABLE tensors of [begin, end).
 template <typename F>
-static int for_tables(int32_t count, const uint64_t* params, const uint64_t* grads, const int64_t* sizes,
-                      const int64_t* offsets, const int32_t* slots, F&& launch) {
-    OptTable t;
-    t.count = t.chunks = 0;
-    int64_t before = 0;
-    for (int32_t i = 0; i < count; ++i) {
-        const int64_t n = sizes[i];
-        AZ_CHECK_ARG(n >= 0 && n <= (int64_t(1) << 40), "tensor %d has %lld elements", i, (long long)n);
-        if (n == 0) continue;
-        AZ_CHECK_ARG(grads[i] && grads[i] % 4 == 0, "gradient %d is null or not aligned to 4 bytes", i);
-        const int64_t chunks = (n + OPT_CHUNK - 1) / OPT_CHUNK;
-        if (t.count == (uint32_t)OPT_TABLE || (t.count && t.chunks + chunks > 0x7FFFFFFF)) {
-            const int rc = launch(t, before);
+static int for_ranges(int32_t begin, int32_t end, const int64_t* sizes, F&& launch) {
+    int64_t piece = 0;
+    for (int32_t i = 0; i < begin; ++i) piece += pieces_of(sizes[i]);
+    for (int32_t i = begin; i < end; i += OPT_TABLE) {
+        const int32_t k = end - i < OPT_TABLE ? end - i : OPT_TABLE;
+        int64_t n = 0;
+        for (int32_t j = i; j < i + k; ++j) n += pieces_of(sizes[j]);
+        if (n) {
+            const int rc = launch(i, k, piece, (uint32_t)n);
             if (rc != AZ_OK) return rc;
-            before += t.chunks;
-            t.count = t.chunks = 0;
         }
-        t.grad[t.count] = grads[i];
-        t.param[t.count] = params ? params[i] : 0;
-        t.first[t.count] = t.chunks;
-        t.offset[t.count] = offsets ? (uint32_t)(offsets[i] / OPT_BLOCK) : 0;
-        t.slot_tail[t.count] = (slots ? (uint32_t)slots[i] : 0) | (uint32_t)(n - (chunks - 1) * OPT_CHUNK - 1) << 20;
-        ++t.count;
-        t.chunks += (uint32_t)chunks;
+        piece += n;
     }
-    return t.count ? launch(t, before) : AZ_OK;
+    return AZ_OK;
+}
+
+static int check_tensors(const char* what, int32_t count, const int64_t* sizes, const uint64_t* params, const uint64_t* grads, int64_t* pieces) {
+    AZ_CHECK_ARG(count >= 0 && count <= 1 << 20 && (count == 0 || (sizes && grads)), "%s: null table, or %d tensors (up to 2^20)", what, count);
+    *pieces = 0;
+    for (int32_t i = 0; i < count; ++i) {
+        AZ_CHECK_ARG(sizes[i] >= 0 && sizes[i] <= int64_t(1) << 38, "%s: tensor %d has %lld elements", what, i, (long long)sizes[i]);
+        *pieces += pieces_of(sizes[i]);
+        if (!grads[i] || !sizes[i]) continue;
+        AZ_CHECK_ARG(grads[i] % 4 == 0, "%s: gradient %d is not aligned to 4 bytes", what, i);
+        AZ_CHECK_ARG(!params || (params[i] && params[i] % 4 == 0), "%s: parameter %d is null or not aligned to 4 bytes", what, i);
+    }
+    AZ_CHECK_ARG(*pieces <= 0x7FFFFFFF, "%s: too many elements", what);
+    return AZ_OK;
 }
 
 }  // namespace az
 
 using namespace az;
 
-extern "C" int az_grad_sumsq(int32_t count, const uint64_t* grads_host, const int64_t* sizes_host, double* partials_dev,
-                             int64_t n_partials, void* stream) {
-    AZ_CHECK_ARG(count >= 0 && (count == 0 || (grads_host && sizes_host)), "az_grad_sumsq: null table");
-    int64_t need = 0;
-    for (int32_t i = 0; i < count; ++i) need += sizes_host[i] > 0 ? (sizes_host[i] + OPT_CHUNK - 1) / OPT_CHUNK : 0;
-    AZ_CHECK_ARG(n_partials >= need && (need == 0 || partials_dev), "az_grad_sumsq: %lld partial sums needed, room for %lld",
-                 (long long)need, (long long)n_partials);
-    return for_tables(count, nullptr, grads_host, sizes_host, nullptr, nullptr, [&](const OptTable& t, int64_t before) -> int {
-        hipLaunchKernelGGL(k_grad_sumsq, dim3(t.chunks), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, partials_dev + before);
+extern "C" int64_t az_adam_plan(int32_t count, const int64_t* sizes_host, int64_t* offsets_host, az_adam_piece* pieces_host) {
+    if (count < 0 || (count && !sizes_host)) AZ_FAIL(AZ_ERR_ARG, "az_adam_plan: null sizes");
+    int64_t at = 0, piece = 0;
+    for (int32_t i = 0; i < count; ++i) {
+        if (sizes_host[i] < 0 || sizes_host[i] > int64_t(1) << 38) AZ_FAIL(AZ_ERR_ARG, "az_adam_plan: tensor %d has %lld elements", i, (long long)sizes_host[i]);
+        if (offsets_host) offsets_host[i] = at;
+        for (int64_t k = 0; k < pieces_of(sizes_host[i]); ++k, ++piece) {
+            if (!pieces_host) continue;
+            const int64_t left = sizes_host[i] - k * OPT_CHUNK;
+            pieces_host[piece] = {(uint32_t)i, (uint32_t)k, (uint32_t)((at + k * OPT_CHUNK) / OPT_BLOCK), (uint32_t)(left < OPT_CHUNK ? left : OPT_CHUNK)};
+        }
+        at += (sizes_host[i] + OPT_BLOCK - 1) / OPT_BLOCK * OPT_BLOCK;
+    }
+    if (at / OPT_BLOCK > 0xFFFFFFFF) AZ_FAIL(AZ_ERR_ARG, "az_adam_plan: too many elements");
+    if (offsets_host) offsets_host[count] = at;
+    return piece;
+}
+
+extern "C" int az_grad_sumsq(int32_t count, const uint64_t* grads_host, const int64_t* sizes_host, const az_adam_piece* pieces_dev,
+                             double* partials_dev, int64_t n_partials, void* stream) {
+    int64_t pieces;
+    const int rc = check_tensors("az_grad_sumsq", count, sizes_host, nullptr, grads_host, &pieces);
+    if (rc != AZ_OK) return rc;
+    AZ_CHECK_ARG(n_partials == pieces && (pieces == 0 || (partials_dev && pieces_dev)), "az_grad_sumsq: %lld partial sums are written, room for %lld",
+                 (long long)pieces, (long long)n_partials);
+    return for_ranges(0, count, sizes_host, [&](int32_t first, int32_t k, int64_t piece, uint32_t n) -> int {
+        GradTable t;
+        for (int32_t i = 0; i < k; ++i) t.grad[i] = grads_host[first + i];
+        hipLaunchKernelGGL(k_grad_sumsq, dim3(n), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, pieces_dev + piece, (uint32_t)first, partials_dev + piece);
         AZ_HIP(hipGetLastError());
         return AZ_OK;
     });
 }
 
-extern "C" int az_adam_step(const az_adam_config* cfg, int32_t count, const uint64_t* params_host, const uint64_t* grads_host,
-                            const int64_t* sizes_host, const int64_t* offsets_host, const int32_t* slots_host, void* stream) {
+extern "C" int az_adam_step(const az_adam_config* cfg, int32_t count, int32_t begin, int32_t end, const uint64_t* params_host,
+                            const uint64_t* grads_host, const int64_t* sizes_host, void* stream) {
     AZ_CHECK_ARG(cfg, "az_adam_step: null config");
-    if (count == 0) return AZ_OK;
-    AZ_CHECK_ARG(count > 0 && params_host && grads_host && sizes_host && offsets_host && slots_host, "az_adam_step: null table");
+    int64_t pieces;
+    int rc = check_tensors("az_adam_step", count, sizes_host, params_host, grads_host, &pieces);
+    if (rc != AZ_OK) return rc;
+    AZ_CHECK_ARG(0 <= begin && begin <= end && end <= count, "az_adam_step: tensors %d to %d of %d", begin, end, count);
+    if (begin == end) return AZ_OK;
+    AZ_CHECK_ARG(params_host, "az_adam_step: null parameters");
     AZ_CHECK_ARG(cfg->state_bits == 32 || cfg->state_bits == 8, "az_adam_step: moments in %d bits (32 or 8)", cfg->state_bits);
-    AZ_CHECK_ARG(cfg->m_dev && cfg->v_dev && cfg->steps_dev && cfg->scratch_dev, "az_adam_step: null state");
+    AZ_CHECK_ARG(cfg->m_dev && cfg->v_dev && cfg->steps_dev && cfg->scratch_dev && cfg->pieces_dev, "az_adam_step: null state");
     AZ_CHECK_ARG(cfg->state_bits == 32 || (cfg->m_scale_dev && cfg->v_scale_dev), "az_adam_step: 8-bit moments need scales");
     AZ_CHECK_ARG((uintptr_t)cfg->m_dev % 16 == 0 && (uintptr_t)cfg->v_dev % 16 == 0, "az_adam_step: the moments must be 16-byte aligned");
-    AZ_CHECK_ARG(cfg->n_slots > 0 && cfg->n_slots <= 1 << 20, "az_adam_step: %d step counters (1 to 2^20)", cfg->n_slots);
-    AZ_CHECK_ARG(!(cfg->max_norm > 0) || (cfg->n_partials >= 0 && (cfg->n_partials == 0 || cfg->partials_dev)), "az_adam_step: null partial sums");
-    for (int32_t i = 0; i < count; ++i) {
-        AZ_CHECK_ARG(slots_host[i] >= 0 && slots_host[i] < cfg->n_slots, "az_adam_step: step counter %d of %d", slots_host[i], cfg->n_slots);
-        AZ_CHECK_ARG(sizes_host[i] >= 0 && offsets_host[i] >= 0 && offsets_host[i] % OPT_BLOCK == 0 && offsets_host[i] <= cfg->capacity &&
-                         (sizes_host[i] + OPT_BLOCK - 1) / OPT_BLOCK * OPT_BLOCK <= cfg->capacity - offsets_host[i],
-                     "az_adam_step: tensor %d does not fit the moments", i);
-        AZ_CHECK_ARG(sizes_host[i] == 0 || (params_host[i] && params_host[i] % 4 == 0), "parameter %d is null or not aligned to 4 bytes", i);
-    }
+    AZ_CHECK_ARG(!(cfg->max_norm > 0) || (cfg->n_partials == pieces && (pieces == 0 || cfg->partials_dev)),
+                 "az_adam_step: %lld partial sums, %lld wanted", (long long)cfg->n_partials, (long long)pieces);
     float* scratch = (float*)cfg->scratch_dev;            // [0] clipping factor, then the tensors' factors
     OptHyper h;
     h.lr = cfg->lr;
@@ -340,18 +408,25 @@ extern "C" int az_adam_step(const az_adam_config* cfg, int32_t count, const uint
     a.v = cfg->v_dev;
     a.m_scale = cfg->m_scale_dev;
     a.v_scale = cfg->v_scale_dev;
-    for (int32_t at = 0; at < count; at += OPT_SLOTS) {
-        SlotList l;
-        const uint32_t k = (uint32_t)(count - at < OPT_SLOTS ? count - at : OPT_SLOTS);
-        for (uint32_t i = 0; i < k; ++i) l.slot[i] = (uint32_t)slots_host[at + i];
-        hipLaunchKernelGGL(k_adam_begin, dim3(1), dim3(1024), 0, (hipStream_t)stream, l, k, h);
+    for (int32_t at = begin; at < end; at += OPT_MASK * 32) {
+        TensorMask mask = {};
+        const uint32_t k = (uint32_t)(end - at < OPT_MASK * 32 ? end - at : OPT_MASK * 32);
+        for (uint32_t i = 0; i < k; ++i) mask.has_grad[i / 32] |= (grads_host[at + i] && sizes_host[at + i] ? 1u : 0u) << (i % 32);
+        hipLaunchKernelGGL(k_adam_begin, dim3(1), dim3(1024), 0, (hipStream_t)stream, mask, (uint32_t)at, k, h);
         AZ_HIP(hipGetLastError());
     }
-    return for_tables(count, params_host, grads_host, sizes_host, offsets_host, slots_host, [&](const OptTable& t, int64_t) -> int {
+    return for_ranges(begin, end, sizes_host, [&](int32_t first, int32_t k, int64_t piece, uint32_t n) -> int {
+        TensorTable t;
+        for (int32_t i = 0; i < k; ++i) {
+            t.grad[i] = grads_host[first + i];
+            t.param[i] = params_host[first + i];
+        }
+        a.pieces = cfg->pieces_dev + piece;
+        a.first_tensor = (uint32_t)first;
         if (cfg->state_bits == 32)
-            hipLaunchKernelGGL(k_adam<32>, dim3(t.chunks), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, a);
+            hipLaunchKernelGGL(k_adam<32>, dim3(n), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, a);
         else
-            hipLaunchKernelGGL(k_adam<8>, dim3(t.chunks), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, a);
+            hipLaunchKernelGGL(k_adam<8>, dim3(n), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, a);
         AZ_HIP(hipGetLastError());
         return AZ_OK;
     });

@@ -35,6 +35,7 @@ struct Entries {
     decltype(&az_policy_value_loss_ready) loss_ready;
     decltype(&az_policy_value_loss_forward) loss_forward;
     decltype(&az_policy_value_loss_backward) loss_backward;
+    decltype(&az_adam_plan) adam_plan;
     decltype(&az_grad_sumsq) grad_sumsq;
     decltype(&az_adam_step) adam_step;
 } lib;
@@ -343,14 +344,33 @@ struct AdamGroup {
 
 class AdamPlan {
   public:
-    AdamPlan(std::vector<Tensor> params, std::vector<int64_t> offsets, int64_t capacity, int bits, uint64_t seed, Tensor step, Tensor m,
-             Tensor v, MaybeTensor m_scale, MaybeTensor v_scale, Tensor norm)
-        : params_(std::move(params)), offsets_(std::move(offsets)), capacity_(capacity), bits_(bits), seed_(seed), step_(step), m_(m), v_(v),
-          m_scale_(m_scale.value_or(Tensor())), v_scale_(v_scale.value_or(Tensor())), norm_(norm) {
+    // Lays out the moments of the parameters; attach() gives it the buffers.
+    explicit AdamPlan(std::vector<Tensor> params) : params_(std::move(params)), offsets_(params_.size() + 1) {
         for (const Tensor& p : params_) {
+            sizes_.push_back(p.numel());
             strides_.push_back(p.strides().vec());
             places_.push_back(nullptr);
         }
+        const int32_t count = (int32_t)params_.size();
+        const int64_t n = lib.adam_plan(count, sizes_.data(), offsets_.data(), nullptr);
+        check(n < 0 ? (int)n : AZ_OK);
+        Tensor pieces = at::empty({n * (int64_t)sizeof(az_adam_piece)}, at::kByte);
+        lib.adam_plan(count, sizes_.data(), nullptr, (az_adam_piece*)pieces.data_ptr());
+        n_pieces_ = n;
+        pieces_ = pieces.to(params_.at(0).device());
+    }
+
+    std::vector<int64_t> offsets() const { return offsets_; }
+
+    void attach(int bits, uint64_t seed, Tensor step, Tensor m, Tensor v, MaybeTensor m_scale, MaybeTensor v_scale, Tensor norm) {
+        bits_ = bits;
+        seed_ = seed;
+        step_ = step;
+        m_ = m;
+        v_ = v;
+        m_scale_ = held(m_scale);
+        v_scale_ = held(v_scale);
+        norm_ = norm;
     }
 
     // One step over every parameter that has a gradient.
@@ -359,23 +379,21 @@ class AdamPlan {
         const c10::DeviceGuard guard(step_.device());
         void* stream = stream_of(step_);
         const size_t count = params_.size();
-        std::vector<uint64_t> params, grads;
-        std::vector<int64_t> sizes, offsets;
-        std::vector<int32_t> slots;
+        std::vector<uint64_t> params(count), grads(count);
         std::vector<Tensor> copies;                  // gradients brought into their parameter's memory order
-        int64_t partials = 0;
+        bool any = false;
         for (size_t i = 0; i < count; ++i) {
             const Tensor& p = params_[i];
             if (p.data_ptr() != places_[i]) {        // new here, or moved since: it must still fit its moments
-                TORCH_CHECK_VALUE(p.scalar_type() == at::kFloat && p.device() == step_.device(), "a parameter became ", p.scalar_type(), " on ",
-                                  p.device(), " after FusedAdam was built");
+                TORCH_CHECK_VALUE(p.scalar_type() == at::kFloat && p.device() == step_.device() && p.numel() == sizes_[i], "a parameter became ",
+                                  p.scalar_type(), " ", p.sizes(), " on ", p.device(), " after FusedAdam was built");
                 TORCH_CHECK_VALUE(p.dim() == (int64_t)strides_[i].size() && same_places(p, strides_[i]),
                                   "a parameter's strides changed after FusedAdam was built: its moments are in the old order");
+                places_[i] = p.data_ptr();
             }
-            places_[i] = p.data_ptr();
-            Tensor g = p.grad();
-            const int64_t n = p.numel();
-            if (!g.defined() || n == 0) continue;
+            const Tensor& held_grad = p.grad();
+            if (!held_grad.defined() || sizes_[i] == 0) continue;
+            Tensor g = held_grad;
             TORCH_CHECK_VALUE(g.layout() == at::kStrided, "FusedAdam takes dense gradients");
             TORCH_CHECK_VALUE(g.scalar_type() == at::kFloat && g.device() == step_.device() && g.sizes() == p.sizes(),
                               "the gradient of a parameter of shape ", p.sizes(), " is ", g.scalar_type(), " ", g.sizes(), " on ", g.device());
@@ -383,25 +401,19 @@ class AdamPlan {
                 g = at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g);
                 copies.push_back(g);
             }
-            params.push_back((uint64_t)p.data_ptr());
-            grads.push_back((uint64_t)g.data_ptr());
-            sizes.push_back(n);
-            offsets.push_back(offsets_[i]);
-            slots.push_back((int32_t)i);
-            partials += (n + AZ_OPTIM_CHUNK - 1) / AZ_OPTIM_CHUNK;
+            params[i] = (uint64_t)p.data_ptr();
+            grads[i] = (uint64_t)g.data_ptr();
+            any = true;
         }
-        if (slots.empty()) return;
+        if (!any) return;
         const Tensor scratch = floats(4 + 3 * (int64_t)count, step_);
+        const auto pieces = (const az_adam_piece*)pieces_.data_ptr();
         Tensor sums;
         if (max_norm > 0) {
-            sums = at::empty({partials}, step_.options().dtype(at::kDouble));
-            check(lib.grad_sumsq((int32_t)slots.size(), grads.data(), sizes.data(), ptr<double>(sums), partials, stream));
+            sums = at::empty({n_pieces_}, step_.options().dtype(at::kDouble));
+            check(lib.grad_sumsq((int32_t)count, grads.data(), sizes_.data(), pieces, ptr<double>(sums), n_pieces_, stream));
         }
-        size_t at = 0;
         for (const AdamGroup& g : groups) {
-            const size_t from = at;
-            while (at < slots.size() && slots[at] < g.end) ++at;
-            if (at == from) continue;
             az_adam_config c{};
             c.lr = g.lr;
             c.beta1 = g.beta1;
@@ -412,9 +424,8 @@ class AdamPlan {
             c.max_norm = max_norm > 0 ? max_norm : 0.0;
             c.state_bits = bits_;
             c.seed = seed_;
-            c.capacity = capacity_;
-            c.n_partials = sums.defined() ? partials : 0;
-            c.n_slots = (int32_t)count;
+            c.n_partials = sums.defined() ? n_pieces_ : 0;
+            c.pieces_dev = pieces;
             c.m_dev = m_.data_ptr();
             c.v_dev = v_.data_ptr();
             c.m_scale_dev = ptr<float>(m_scale_);
@@ -423,24 +434,25 @@ class AdamPlan {
             c.partials_dev = ptr<double>(sums);
             c.norm_dev = sums.defined() ? ptr<float>(norm_) : nullptr;
             c.scratch_dev = ptr<float>(scratch);
-            check(lib.adam_step(&c, (int32_t)(at - from), params.data() + from, grads.data() + from, sizes.data() + from,
-                                offsets.data() + from, slots.data() + from, stream));
+            check(lib.adam_step(&c, (int32_t)count, (int32_t)g.begin, (int32_t)g.end, params.data(), grads.data(), sizes_.data(), stream));
         }
         // written behind torch's back: whoever watches version counters has to see it
-        for (int32_t i : slots) params_[i].unsafeGetTensorImpl()->bump_version();
+        for (size_t i = 0; i < count; ++i)
+            if (grads[i]) params_[i].unsafeGetTensorImpl()->bump_version();
         for (const Tensor* t : {&step_, &m_, &v_, &m_scale_, &v_scale_})
             if (t->defined()) t->unsafeGetTensorImpl()->bump_version();
     }
 
   private:
     std::vector<Tensor> params_;
-    std::vector<int64_t> offsets_;
-    int64_t capacity_;
-    int bits_;
-    uint64_t seed_;
-    Tensor step_, m_, v_, m_scale_, v_scale_, norm_;
+    std::vector<int64_t> sizes_, offsets_;
     std::vector<std::vector<int64_t>> strides_;
     std::vector<void*> places_;
+    int64_t n_pieces_ = 0;
+    Tensor pieces_;
+    int bits_ = 32;
+    uint64_t seed_ = 0;
+    Tensor step_, m_, v_, m_scale_, v_scale_, norm_;
 };
 
 template <typename F>
@@ -458,6 +470,7 @@ PYBIND11_MODULE(_azops, m) {
         set(lib.loss_ready, a, "az_policy_value_loss_ready");
         set(lib.loss_forward, a, "az_policy_value_loss_forward");
         set(lib.loss_backward, a, "az_policy_value_loss_backward");
+        set(lib.adam_plan, a, "az_adam_plan");
         set(lib.grad_sumsq, a, "az_grad_sumsq");
         set(lib.adam_step, a, "az_adam_step");
         az_error = error.release().ptr();
@@ -465,8 +478,9 @@ PYBIND11_MODULE(_azops, m) {
     m.def("norm", torch::wrap_pybind_function(norm));
     m.def("policy_value_loss", torch::wrap_pybind_function(policy_value_loss));
     py::class_<AdamPlan>(m, "AdamPlan")
-        .def(py::init<std::vector<Tensor>, std::vector<int64_t>, int64_t, int, uint64_t, Tensor, Tensor, Tensor, MaybeTensor,
-                      MaybeTensor, Tensor>())
+        .def(py::init<std::vector<Tensor>>())
+        .def("offsets", &AdamPlan::offsets)
+        .def("attach", &AdamPlan::attach)
         .def("step", [](AdamPlan& self, const std::vector<std::tuple<int64_t, int64_t, double, double, double, double, double, bool>>& groups,
                         double max_norm) {
             std::vector<AdamGroup> g;

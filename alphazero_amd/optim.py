@@ -86,10 +86,8 @@ class FusedAdam(torch.optim.Optimizer):
             if not _dense(p):
                 raise ValueError(f"a parameter of shape {tuple(p.shape)} and strides {p.stride()} does not fill its memory")
         self._params, self._device = params, device
-        self._offsets, total = [], 0
-        for p in params:
-            self._offsets.append(total)
-            total += -(-p.numel() // _PAD) * _PAD
+        self._plan = _lib.torch_ops().AdamPlan(params)
+        *self._offsets, total = self._plan.offsets()
         self._capacity = total
         shape = dict(device=device)
         self._step = torch.zeros(len(params), dtype=torch.float32, **shape)
@@ -108,9 +106,8 @@ class FusedAdam(torch.optim.Optimizer):
             self._groups.append((at, at + k))
             at += k
         m, v = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_rms")
-        self._plan = _lib.torch_ops().AdamPlan(
-            params, self._offsets, total, self.state_bits, self.seed & 0xFFFFFFFF, self._step, self._flat[m], self._flat[v],
-            self._flat.get(m + "_scale"), self._flat.get(v + "_scale"), self.grad_norm)
+        self._plan.attach(self.state_bits, self.seed & 0xFFFFFFFF, self._step, self._flat[m], self._flat[v],
+                          self._flat.get(m + "_scale"), self._flat.get(v + "_scale"), self.grad_norm)
         self._built = True
         self._attach()
 

@@ -393,35 +393,45 @@ int az_policy_value_loss_forward(const az_loss_args* args, void* stream);
 int az_policy_value_loss_backward(const az_loss_args* args, void* stream);
 
 /* One Adam (decoupled == 0: weight decay added to the gradient, torch.optim.Adam of
- * src/parallel_trainer.py:121) or AdamW step over `count` float32 tensors, given as host arrays of
- * device addresses and sizes in elements.  Tensor i's moments start at element offsets_host[i] (a
- * multiple of AZ_OPTIM_PAD) of m_dev / v_dev, which hold `capacity` elements; its step counter is
- * steps_dev[slots_host[i]] (float32, incremented by the call).  A slot appears once.
- * state_bits 32: m and v as float32.  state_bits 8: m and sqrt(v) as e4m3 codes, one power of
- * two per AZ_OPTIM_PAD of them in m_scale_dev / v_scale_dev, rounded at random (a hash of seed,
- * step counter and place).
+ * src/parallel_trainer.py:121) or AdamW step over float32 tensors, given as host arrays of device
+ * addresses and sizes in elements; a gradient of 0 leaves its tensor alone.
+ * az_adam_plan lays out the moments: tensor i's start at element offsets_host[i] (a multiple of
+ * AZ_OPTIM_PAD; offsets_host[count] is the size of all), and it fills one piece per AZ_OPTIM_CHUNK
+ * elements of a tensor; either array may be null.  It returns the number of pieces or a negative
+ * code.  The caller keeps a copy of the pieces in device memory (pieces_dev): they are read by
+ * every call on the same sizes.
+ * az_grad_sumsq writes one partial sum of squares per piece of all `count` tensors.
+ * az_adam_step steps tensors [begin, end) of the `count`: its step counter steps_dev[i] (float32) is
+ * incremented where there is a gradient.  state_bits 32: m and v as float32.  state_bits 8: m and
+ * sqrt(v) as e4m3 codes, one power of two per AZ_OPTIM_PAD of them in m_scale_dev / v_scale_dev,
+ * rounded at random (a hash of seed, step counter and place).
  * max_norm > 0: gradients are scaled by min(1, max_norm / (norm + 1e-6)) on the way in, norm being
- * the root of the sum of partials_dev[0..n_partials) (az_grad_sumsq over every tensor, one partial
- * sum per AZ_OPTIM_CHUNK elements of a tensor); the gradients themselves are not written.
- * scratch_dev: 4 + 3 * n_slots floats. */
+ * the root of the sum of partials_dev; the gradients themselves are not written.
+ * scratch_dev: 4 + 3 * count floats. */
 #define AZ_OPTIM_CHUNK 4096
 #define AZ_OPTIM_PAD 256
+typedef struct {
+    uint32_t tensor, chunk;      /* which tensor, which AZ_OPTIM_CHUNK elements of it */
+    uint32_t offset;             /* its place in the moments, in units of AZ_OPTIM_PAD */
+    uint32_t n;                  /* elements of the piece */
+} az_adam_piece;
 typedef struct {
     double lr, beta1, beta2, eps, weight_decay, max_norm;
     int32_t decoupled, state_bits;
     uint64_t seed;
-    int64_t capacity, n_partials;
-    int32_t n_slots;
-    void *m_dev, *v_dev;
+    int64_t n_partials;
+    const az_adam_piece* pieces_dev;
+    void *m_dev, *v_dev;         /* 16-byte aligned */
     float *m_scale_dev, *v_scale_dev, *steps_dev;
     const double* partials_dev;
     float* norm_dev;             /* receives the norm; may be null */
     float* scratch_dev;
 } az_adam_config;
-int az_grad_sumsq(int32_t count, const uint64_t* grads_host, const int64_t* sizes_host, double* partials_dev,
-                  int64_t n_partials, void* stream);
-int az_adam_step(const az_adam_config* cfg, int32_t count, const uint64_t* params_host, const uint64_t* grads_host,
-                 const int64_t* sizes_host, const int64_t* offsets_host, const int32_t* slots_host, void* stream);
+int64_t az_adam_plan(int32_t count, const int64_t* sizes_host, int64_t* offsets_host, az_adam_piece* pieces_host);
+int az_grad_sumsq(int32_t count, const uint64_t* grads_host, const int64_t* sizes_host, const az_adam_piece* pieces_dev,
+                  double* partials_dev, int64_t n_partials, void* stream);
+int az_adam_step(const az_adam_config* cfg, int32_t count, int32_t begin, int32_t end, const uint64_t* params_host,
+                 const uint64_t* grads_host, const int64_t* sizes_host, void* stream);
 
 #ifdef __cplusplus
 }

@@ -85,34 +85,49 @@ def test_c_entry_of_the_loss_checks_its_arguments(kw, match):
 
 
 def _adam(**kw):
-    a = _lib.AdamConfig(1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, 0, 32, 0, 1024, 0, 2, 64, 64, None, None, 64, None, None, 64)
+    a = _lib.AdamConfig(1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, 0, 32, 0, 0, 64, 64, 64, None, None, 64, None, None, 64)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
 
 
-@pytest.mark.parametrize("kw, size, offset, slot, match", [
-    ({"state_bits": 16}, 10, 0, 0, "moments in 16 bits"), ({"m": None}, 10, 0, 0, "null state"), ({"state_bits": 8}, 10, 0, 0, "scales"),
-    ({"m": 68}, 10, 0, 0, "aligned"), ({"n_slots": 0}, 10, 0, 0, "step counters"), ({}, 10, 0, 2, "step counter 2 of 2"),
-    ({}, 10, 100, 0, "does not fit"), ({}, 1025, 0, 0, "does not fit"), ({}, 800, 256, 0, "does not fit"), ({}, -1, 0, 0, "does not fit"),
-    ({}, 10, -256, 0, "does not fit"), ({"max_norm": 1.0, "n_partials": 1}, 10, 0, 0, "partial sums"),
+@pytest.mark.parametrize("kw, size, begin, end, match", [
+    ({"state_bits": 16}, 10, 0, 1, "moments in 16 bits"), ({"m": None}, 10, 0, 1, "null state"), ({"pieces": None}, 10, 0, 1, "null state"),
+    ({"state_bits": 8}, 10, 0, 1, "scales"), ({"m": 68}, 10, 0, 1, "aligned"), ({}, -1, 0, 1, "-1 elements"), ({}, 1 << 39, 0, 1, "elements"),
+    ({}, 10, 0, 2, "tensors 0 to 2 of 1"), ({}, 10, -1, 1, "tensors -1 to 1"), ({"max_norm": 1.0, "n_partials": 1}, 10, 0, 1, "partial sums"),
+    ({"max_norm": 1.0, "n_partials": 2, "partials": 64}, 10, 0, 1, "2 partial sums, 1 wanted"),
 ])
-def test_c_entry_of_the_step_checks_its_arguments(kw, size, offset, slot, match):
+def test_c_entry_of_the_step_checks_its_arguments(kw, size, begin, end, match):
     L = _lib.lib()
-    p, s, o, i = (C.c_uint64 * 1)(64), (C.c_int64 * 1)(size), (C.c_int64 * 1)(offset), (C.c_int32 * 1)(slot)
-    assert L.az_adam_step(C.byref(_adam(**kw)), 1, p, p, s, o, i, None) == -1
+    p, s = (C.c_uint64 * 1)(64), (C.c_int64 * 1)(size)
+    assert L.az_adam_step(C.byref(_adam(**kw)), 1, begin, end, p, p, s, None) == -1
     assert match.encode() in L.az_last_error()
 
 
 def test_c_entries_refuse_misaligned_tensors_and_short_partials():
     L = _lib.lib()
-    good, odd, s, z, i = (C.c_uint64 * 1)(64), (C.c_uint64 * 1)(66), (C.c_int64 * 1)(5000), (C.c_int64 * 1)(0), (C.c_int32 * 1)(0)
-    assert L.az_grad_sumsq(1, good, s, 64, 1, None) == -1 and b"2 partial sums" in L.az_last_error()
-    assert L.az_grad_sumsq(1, odd, s, 64, 2, None) == -1 and b"aligned" in L.az_last_error()
-    cfg = _adam(capacity=8192)
-    assert L.az_adam_step(C.byref(cfg), 1, odd, good, s, z, i, None) == -1 and b"aligned" in L.az_last_error()
-    assert L.az_adam_step(C.byref(cfg), 0, None, None, None, None, None, None) == 0          # nothing to do is fine
-    assert L.az_grad_sumsq(0, None, None, None, 0, None) == 0
+    good, odd, s = (C.c_uint64 * 1)(64), (C.c_uint64 * 1)(66), (C.c_int64 * 1)(5000)
+    assert L.az_grad_sumsq(1, good, s, 64, 64, 1, None) == -1 and b"2 partial sums" in L.az_last_error()
+    assert L.az_grad_sumsq(1, good, s, None, 64, 2, None) == -1
+    assert L.az_grad_sumsq(1, odd, s, 64, 64, 2, None) == -1 and b"aligned" in L.az_last_error()
+    assert L.az_adam_step(C.byref(_adam()), 1, 0, 1, odd, good, s, None) == -1 and b"aligned" in L.az_last_error()
+    assert L.az_adam_step(C.byref(_adam()), 0, 0, 0, None, None, None, None) == 0          # nothing to do is fine
+    assert L.az_grad_sumsq(0, None, None, None, None, 0, None) == 0
+
+
+def test_plan_of_the_moments():
+    """Every tensor starts at a multiple of the pad, its pieces follow one another, the last one is what is left."""
+    sizes = [1, 0, 256, 4096, 4097, 10000]
+    n, offsets = len(sizes), (C.c_int64 * 7)()
+    L = _lib.lib()
+    count = L.az_adam_plan(n, (C.c_int64 * n)(*sizes), offsets, None)
+    assert count == 1 + 0 + 1 + 1 + 2 + 3
+    assert list(offsets) == [0, 256, 256, 512, 4608, 4608 + 4352, 4608 + 4352 + 10240]
+    pieces = (C.c_uint32 * (4 * count))()
+    assert L.az_adam_plan(n, (C.c_int64 * n)(*sizes), None, pieces) == count
+    got = [tuple(pieces[4 * i:4 * i + 4]) for i in range(count)]
+    assert got == [(0, 0, 0, 1), (2, 0, 1, 256), (3, 0, 2, 4096), (4, 0, 18, 4096), (4, 1, 34, 1), (5, 0, 35, 4096), (5, 1, 51, 4096), (5, 2, 67, 1808)]
+    assert L.az_adam_plan(1, (C.c_int64 * 1)(-5), None, None) == -1 and L.az_adam_plan(-1, None, None, None) == -1
 
 
 def test_eight_bit_moments_survive_a_checkpoint():
