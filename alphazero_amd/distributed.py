@@ -16,7 +16,9 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
+from . import ops
 from .config import Config
+from .optim import FusedAdam
 
 
 def shard_games(total_games: int, rank: int, world: int) -> Tuple[int, int]:
@@ -130,13 +132,33 @@ def sync_batchnorm_buffers(model: torch.nn.Module, weight: float, group=None):
             b.copy_(v)
 
 
-def losses(model, states, target_pis, target_wls):
-    """Soft-target policy cross-entropy + WL cross-entropy (src/parallel_trainer.py:251-260)."""
-    pred_pis, pred_wls = model(states)
+def losses(model, states, target_pis, target_wls, autocast_dtype=None):
+    """Soft-target policy cross-entropy + WL cross-entropy (src/parallel_trainer.py:251-260), by
+    ops.policy_value_loss for a model with fused operators.  autocast_dtype: the forward runs under torch.autocast."""
+    if autocast_dtype is None:
+        pred_pis, pred_wls = model(states)
+    else:
+        with torch.autocast(device_type=states.device.type, dtype=autocast_dtype):
+            pred_pis, pred_wls = model(states)
+    if getattr(model, "fused", False):
+        return ops.policy_value_loss(pred_pis, pred_wls, target_pis, target_wls)
+    if autocast_dtype is not None:
+        pred_pis, pred_wls = pred_pis.float(), pred_wls.float()
     log_probs = F.log_softmax(pred_pis, dim=1)
     loss_pi = -torch.sum(target_pis * log_probs) / target_pis.size(0)
     loss_wl = F.cross_entropy(pred_wls, target_wls)
     return loss_pi + loss_wl, loss_pi, loss_wl
+
+
+def clip_and_step(model, optimizer):
+    """Clip the gradients by their global norm (src/parallel_trainer.py:264-268) and update the weights: one call
+    of FusedAdam, which clips on the way (and leaves .grad as it is), or torch's two."""
+    if isinstance(optimizer, FusedAdam):
+        optimizer.step(max_norm=Config.GRAD_CLIP_NORM if Config.GRAD_CLIP_NORM > 0 else None)
+        return
+    if Config.GRAD_CLIP_NORM > 0:
+        torch.nn.utils.clip_grad_norm_(model.parameters(), Config.GRAD_CLIP_NORM)
+    optimizer.step()
 
 
 def train_step(model, optimizer, states, target_pis, target_wls, group=None, autocast_dtype=None,
@@ -164,12 +186,7 @@ def train_step(model, optimizer, states, target_pis, target_wls, group=None, aut
             searched = torch.backends.cudnn.benchmark
             torch.backends.cudnn.benchmark = True
             try:
-                with torch.autocast(device_type=states.device.type, dtype=autocast_dtype):
-                    pred_pis, pred_wls = model(states)
-                log_probs = F.log_softmax(pred_pis.float(), dim=1)
-                loss_pi = -torch.sum(target_pis * log_probs) / target_pis.size(0)
-                loss_wl = F.cross_entropy(pred_wls.float(), target_wls)
-                loss = loss_pi + loss_wl
+                loss, loss_pi, loss_wl = losses(model, states, target_pis, target_wls, autocast_dtype)
                 loss.backward()
             finally:
                 torch.backends.cudnn.benchmark = searched
@@ -191,9 +208,7 @@ def train_step(model, optimizer, states, target_pis, target_wls, group=None, aut
         allreduce_gradients(model, weight, group)
         with torch.no_grad():
             sync_batchnorm_buffers(model, weight, group)
-    if Config.GRAD_CLIP_NORM > 0:
-        torch.nn.utils.clip_grad_norm_(model.parameters(), Config.GRAD_CLIP_NORM)
-    optimizer.step()
+    clip_and_step(model, optimizer)
     return out if as_tensor else tuple(out.tolist())
 
 
@@ -245,22 +260,12 @@ class GraphedTrainStep:
 
     def _grads(self):
         self.optimizer.zero_grad(set_to_none=False)
-        if self.autocast_dtype is None:
-            loss, loss_pi, loss_wl = losses(self.model, self.states, self.pis, self.wls)
-        else:
-            with torch.autocast(device_type="cuda", dtype=self.autocast_dtype):
-                pred_pis, pred_wls = self.model(self.states)
-            log_probs = F.log_softmax(pred_pis.float(), dim=1)
-            loss_pi = -torch.sum(self.pis * log_probs) / self.n
-            loss_wl = F.cross_entropy(pred_wls.float(), self.wls)
-            loss = loss_pi + loss_wl
+        loss, loss_pi, loss_wl = losses(self.model, self.states, self.pis, self.wls, self.autocast_dtype)
         loss.backward()
         self.sums += torch.stack((loss.detach().float(), loss_pi.detach().float(), loss_wl.detach().float()))
 
     def _update(self):
-        if Config.GRAD_CLIP_NORM > 0:
-            torch.nn.utils.clip_grad_norm_(self.model.parameters(), Config.GRAD_CLIP_NORM)
-        self.optimizer.step()
+        clip_and_step(self.model, self.optimizer)
 
     def _between(self, global_batch):
         if dist.is_available() and dist.is_initialized() and dist.get_world_size(self.group) > 1:

@@ -6,6 +6,11 @@ kernels.
 The torch modules are what the training step differentiates; eval-mode
 inference on a GPU goes through libazamd (`HipInference`), which has no
 fallback: if the library or the GPU is missing it raises.
+
+After `AlphaZeroNet.use_fused_ops()` everything of the network's forward and
+backward pass but its convolutions and linear layers runs in the library's own
+kernels too (`alphazero_amd.ops`): each BatchNorm with the ReLU behind it, and
+the whole end of a residual block (BatchNorm, squeeze-excitation, skip, ReLU).
 """
 import ctypes as C
 
@@ -13,8 +18,21 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, ops
 from .config import Config
+
+
+def _bn(norm):
+    """A BatchNorm2d's state as the fused operators take it."""
+    return norm.running_mean, norm.running_var, norm.num_batches_tracked, norm.training, norm.momentum, norm.eps
+
+
+def _norm_relu(norm, x, fused):
+    """relu(norm(x))."""
+    if not fused:
+        return F.relu(norm(x))
+    mean, var, count, training, momentum, eps = _bn(norm)
+    return ops.norm_act(x, norm.weight, norm.bias, mean, var, count, training, momentum, eps)
 
 
 class SEBlock(nn.Module):
@@ -38,6 +56,8 @@ class SEBlock(nn.Module):
 class SEResidualBlock(nn.Module):
     """conv-bn-relu-conv-bn-SE, skip, relu (src/model.py:56-92)."""
 
+    fused = False       # set by AlphaZeroNet.use_fused_ops
+
     def __init__(self, channels, se_ratio=8):
         super().__init__()
         self.conv1 = nn.Conv2d(channels, channels, kernel_size=3, padding=1, bias=False)
@@ -47,13 +67,18 @@ class SEResidualBlock(nn.Module):
         self.se = SEBlock(channels, se_ratio)
 
     def forward(self, x):
-        out = F.relu(self.bn1(self.conv1(x)))
-        out = self.se(self.bn2(self.conv2(out)))
-        return F.relu(out + x)
+        out = self.conv2(_norm_relu(self.bn1, self.conv1(x), self.fused))
+        if not self.fused:
+            return F.relu(self.se(self.bn2(out)) + x)
+        mean, var, count, training, momentum, eps = _bn(self.bn2)
+        return ops.norm_gate_residual(out, x, self.bn2.weight, self.bn2.bias, mean, var, self.se.fc1.weight, self.se.fc1.bias,
+                                      self.se.fc2.weight, self.se.fc2.bias, count, training, momentum, eps)
 
 
 class AlphaZeroNet(nn.Module):
     """src/model.py:95-195.  forward(x[B,3,8,8]) -> (policy_logits[B,192], wl_logits[B,2])."""
+
+    fused = False       # see use_fused_ops
 
     def __init__(self, num_blocks=Config.RESNET_BLOCKS, num_filters=Config.RESNET_FILTERS,
                  num_input_planes=Config.INPUT_PLANES, num_actions=Config.OUTPUT_ACTIONS,
@@ -76,13 +101,21 @@ class AlphaZeroNet(nn.Module):
         self.value_fc1 = nn.Linear(32 * 8 * 8, 128)
         self.value_fc2 = nn.Linear(128, 2)
 
+    def use_fused_ops(self, on=True):
+        """Norms, gates, skips and ReLUs of the forward and backward pass as the library's fused kernels (GPU only; the
+        same network, with sums in another order), and back.  The parameters and the checkpoint are the same."""
+        self.fused = bool(on)
+        for block in self.residual_tower:
+            block.fused = self.fused
+        return self
+
     def forward(self, x):
-        out = F.relu(self.input_bn(self.input_conv(x)))
+        out = _norm_relu(self.input_bn, self.input_conv(x), self.fused)
         for block in self.residual_tower:
             out = block(out)
-        policy = F.relu(self.policy_bn(self.policy_conv(out)))
+        policy = _norm_relu(self.policy_bn, self.policy_conv(out), self.fused)
         policy_logits = self.policy_fc(policy.reshape(policy.size(0), -1))
-        value = F.relu(self.value_bn(self.value_conv(out)))
+        value = _norm_relu(self.value_bn, self.value_conv(out), self.fused)
         value = F.relu(self.value_fc1(value.reshape(value.size(0), -1)))
         return policy_logits, self.value_fc2(value)
 

@@ -64,7 +64,8 @@ class FusedAdam(torch.optim.Optimizer):
         self.state_bits, self.seed = state_bits, int(seed)
         self._built = False
         # capturable: what torch.optim.Adam calls an optimiser whose step counters are on the GPU
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled=decoupled, capturable=True))
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                                      decoupled_weight_decay=bool(decoupled), capturable=True))
         self._build()
 
     # ------------------------------------------------------------------ layout
@@ -150,7 +151,7 @@ class FusedAdam(torch.optim.Optimizer):
         before = self.param_groups
         super().load_state_dict(state_dict)
         for g, old in zip(self.param_groups, before):
-            g["decoupled"] = g.get("decoupled", old["decoupled"])
+            g.setdefault("decoupled_weight_decay", old["decoupled_weight_decay"])
             g["capturable"] = True
         moments = {k: torch.zeros(self._capacity, device=self._device) for k in ("exp_avg", "exp_avg_sq")}
         with torch.no_grad():
@@ -179,6 +180,6 @@ class FusedAdam(torch.optim.Optimizer):
                 loss = closure()
         if max_norm is not None and not max_norm > 0:
             raise ValueError(f"max_norm must be positive, got {max_norm}")
-        self._plan.step([(*at, g["lr"], *g["betas"], g["eps"], g["weight_decay"], g["decoupled"])
+        self._plan.step([(*at, g["lr"], *g["betas"], g["eps"], g["weight_decay"], g["decoupled_weight_decay"])
                          for at, g in zip(self._groups, self.param_groups)], max_norm or 0.0)
         return loss

@@ -33,6 +33,7 @@ from .config import Config
 from .game import BOARD_SIZE, NUM_ACTIONS, WHITE, BreakthroughGame
 from .mcts import MCTS, Node
 from .model import AlphaZeroNet
+from .optim import FusedAdam
 
 
 def _mirror_permutation() -> np.ndarray:
@@ -321,18 +322,29 @@ class ParallelTrainer:
     (src/parallel_trainer.py:101-476).  `seed` (extra) seeds the device RNG of
     the fused self-play path; `verbose` (extra) enables the progress prints;
     `autocast_dtype` (extra, default None = float32 like the reference) runs the
-    training forward under torch.autocast."""
+    training forward under torch.autocast; `fused_ops` (extra, GPU only) trains with the
+    library's own kernels for everything but convolutions and linear layers: fused
+    norms and block ends, the loss with its gradient, and FusedAdam (clipping and the
+    update of all tensors in three launches), whose moments take `optimizer_bits`
+    (32 or 8) bits.  Checkpoints are the same files either way."""
 
     def __init__(self, model: AlphaZeroNet, device: str = "cpu",
                  num_parallel_games: int = Config.PARALLEL_GAMES,
                  num_simulations: int = Config.MCTS_SIMULATIONS,
                  checkpoint_dir: str = Config.CHECKPOINT_DIR, seed: int = 0, verbose: bool = True,
-                 autocast_dtype=None, graph_step: bool = False):
+                 autocast_dtype=None, graph_step: bool = False, fused_ops: bool = False, optimizer_bits: int = 32):
         self.model = model
         self.device = device
         self.num_parallel_games = num_parallel_games
         self.num_simulations = num_simulations
-        self.optimizer = optim.Adam(model.parameters(), lr=Config.LEARNING_RATE, weight_decay=Config.WEIGHT_DECAY)
+        if optimizer_bits != 32 and not fused_ops:
+            raise ValueError("optimizer_bits is FusedAdam's: it needs fused_ops=True")
+        if fused_ops:
+            self.optimizer = FusedAdam(model.parameters(), lr=Config.LEARNING_RATE, weight_decay=Config.WEIGHT_DECAY,
+                                       state_bits=optimizer_bits, seed=seed)
+            model.use_fused_ops()
+        else:
+            self.optimizer = optim.Adam(model.parameters(), lr=Config.LEARNING_RATE, weight_decay=Config.WEIGHT_DECAY)
         self.scheduler = CosineAnnealingLR(self.optimizer, T_max=Config.LR_SCHEDULER_T_MAX,
                                            eta_min=Config.LR_SCHEDULER_ETA_MIN)
         self.mcts = MCTS(model, num_simulations=num_simulations, device=device)

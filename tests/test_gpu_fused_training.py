@@ -1,0 +1,170 @@
+"""GPU: the training operators together, as the trainer uses them (ParallelTrainer(fused_ops=True)): the network with
+fused norms and block ends, the loss with its gradient, clipping and the update in one call, eager and from captured
+graphs, in float32 and under autocast, with checkpoints that go both ways."""
+import copy
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def examples(n=96, seed=3):
+    rs = np.random.RandomState(seed)
+    pol = rs.rand(n, 192).astype(np.float32)
+    pol /= pol.sum(1, keepdims=True)
+    return (rs.rand(n, 3, 8, 8) > 0.7).astype(np.float32), pol, np.tile(np.array([[1.0, 0.0], [0.0, 1.0]], np.float32), (n // 2, 1))
+
+
+def trainer(tmp_path, tag, blocks=2, filters=32, n=96, **kw):
+    from alphazero_amd.model import AlphaZeroNet
+    from alphazero_amd.parallel_trainer import ExampleArrays, ParallelTrainer
+    torch.manual_seed(11)
+    tr = ParallelTrainer(AlphaZeroNet(num_blocks=blocks, num_filters=filters).cuda(), device="cuda",
+                         checkpoint_dir=str(tmp_path / tag), verbose=False, **kw)
+    tr.add_examples(ExampleArrays(*examples(n)))
+    return tr
+
+
+def learn(tr, epochs=1, batch_size=32):
+    torch.manual_seed(5)
+    return tr.learn(epochs=epochs, batch_size=batch_size)
+
+
+def distance(x, y):
+    """Relative L2 distance of two models' parameters."""
+    a, b = (torch.cat([p.detach().float().reshape(-1) for p in m.parameters()]) for m in (x, y))
+    return float((a - b).norm() / a.norm())
+
+
+@pytest.mark.parametrize("blocks, filters", [(2, 32), (1, 128), (1, 20)])
+def test_fused_network_is_the_network(blocks, filters):
+    """Outputs, gradients of every parameter and running statistics of one training step against the unfused network in
+    float64 on the CPU.  A gradient passes some ten float32 layers of sums with a few thousand terms: 2^-24 * 10 * 64 in the
+    norm (4e-5), rounded up to 1e-4; a ReLU whose argument lies within that of zero may flip once in ten thousand."""
+    from alphazero_amd.distributed import losses
+    from alphazero_amd.model import AlphaZeroNet
+    torch.manual_seed(2)
+    plain = AlphaZeroNet(num_blocks=blocks, num_filters=filters)
+    fused = copy.deepcopy(plain).cuda().use_fused_ops()
+    plain = plain.double()
+    s, p, w = (torch.from_numpy(a[:24]) for a in examples())
+    want = losses(plain.train(), s.double(), p.double(), w.double())
+    got = losses(fused.train(), s.cuda(), p.cuda(), w.cuda())
+    for a, b in zip(got, want):
+        assert abs(float(a.detach()) - float(b.detach())) <= 1e-5 * abs(float(b.detach()))
+    want[0].backward()
+    got[0].backward()
+    for (name, a), b in zip(fused.named_parameters(), plain.parameters()):
+        assert a.grad.shape == b.grad.shape
+        d = float((a.grad.cpu().double() - b.grad).norm())
+        # a gradient that is a difference of nearly nothing is measured by its parameter's size
+        assert d <= 1e-4 * float(b.grad.norm()) + 1e-7 * float(b.detach().norm()), name
+    for (name, a), b in zip(fused.named_buffers(), plain.buffers()):
+        assert float((a.cpu().double() - b.double()).abs().max()) <= 1e-5 * max(1.0, float(b.double().abs().max())), name
+    fused.eval(), plain.eval()
+    with torch.no_grad():
+        for a, b in zip(fused(s.cuda()), plain(s.double())):
+            assert float((a.cpu().double() - b).abs().max()) <= 1e-4 * float(b.abs().max())
+    assert not fused.use_fused_ops(False).fused
+
+
+def test_fused_learn_follows_the_plain_one(tmp_path):
+    """Six steps from the same seeds: the fused trainer's weights stay within what two float32 runs of one training differ
+    by after so few steps (1e-3, the bound of the graphed trainer's test); the losses agree."""
+    plain, fused = trainer(tmp_path, "p"), trainer(tmp_path, "f", fused_ops=True)
+    a, b = learn(plain), learn(fused)
+    for k in a:
+        assert abs(a[k] - b[k]) <= 1e-4 * abs(a[k])
+    assert distance(plain.model, fused.model) < 1e-3
+    assert all(int(x) == int(y) for x, y in zip(plain.model.buffers(), fused.model.buffers()) if not x.is_floating_point())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_fused_learn_from_graphs(tmp_path, bits):
+    """graph_step=True replays the fused step: three eager steps, the capture, and replays with the schedule's next rate."""
+    eager = trainer(tmp_path, "e", fused_ops=True, optimizer_bits=bits)
+    graphed = trainer(tmp_path, "g", fused_ops=True, optimizer_bits=bits, graph_step=True)
+    learn(eager), learn(graphed)
+    step = graphed._graphed[32]
+    assert step.graph_a is not None and step.graph_b is not None and step.steps_seen == 6
+    assert distance(eager.model, graphed.model) < 1e-3
+    assert float(graphed.optimizer.flat_state()["step"].min()) == 6.0
+    before = [p.detach().clone() for p in graphed.model.parameters()]
+    stats = learn(graphed)                                             # another rate: the update is captured again
+    assert np.isfinite(stats["loss"]) and step.steps_seen == 12
+    assert any(not torch.equal(x, y) for x, y in zip(before, graphed.model.parameters()))
+    assert step.lr < 1e-3 and float(graphed.optimizer.flat_state()["step"].max()) == 12.0
+
+
+@pytest.mark.parametrize("layout", [torch.contiguous_format, torch.channels_last], ids=["nchw", "nhwc"])
+def test_fused_learn_under_autocast(tmp_path, layout):
+    """bfloat16 activations, float32 statistics and weights; either layout.  One step's losses against the plain
+    network's under the same autocast: both round every activation to 2^-8 at least once per layer (2e-2)."""
+    plain = trainer(tmp_path, "p", autocast_dtype=torch.bfloat16)
+    fused = trainer(tmp_path, "f", autocast_dtype=torch.bfloat16, fused_ops=True)
+    for tr in (plain, fused):
+        tr.model.to(memory_format=layout)
+    if layout is torch.channels_last:                                   # the optimiser was built for the other order
+        with pytest.raises(ValueError, match="strides changed"):
+            learn(fused, batch_size=192)
+        from alphazero_amd.optim import FusedAdam
+        fused.optimizer = FusedAdam(fused.model.parameters(), lr=1e-3, weight_decay=1e-4)
+    a, b = learn(plain, batch_size=192), learn(fused, batch_size=192)
+    for k in a:
+        assert abs(a[k] - b[k]) <= 2e-2 * abs(a[k])
+    assert all(bool(torch.isfinite(p).all()) for p in fused.model.parameters())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_checkpoints_of_a_fused_trainer(tmp_path, bits):
+    """iteration_N.pt written by a fused trainer loads into a plain one (on the CPU too) and back, and training goes on from
+    the same moments."""
+    from alphazero_amd.model import AlphaZeroNet
+    from alphazero_amd.parallel_trainer import ParallelTrainer
+    fused = trainer(tmp_path, "c", fused_ops=True, optimizer_bits=bits)
+    learn(fused)
+    fused.save_iteration_checkpoint(1)
+    plain = ParallelTrainer(AlphaZeroNet(num_blocks=2, num_filters=32), device="cpu", checkpoint_dir=str(tmp_path / "c"), verbose=False)
+    assert plain.load_iteration_checkpoint(1)
+    state = fused.optimizer.state_dict()["state"]
+    for i, p in enumerate(plain.model.parameters()):
+        st = plain.optimizer.state[p]
+        assert float(st["step"]) == 6.0 and st["step"].device.type == "cpu"
+        assert torch.equal(st["exp_avg"], state[i]["exp_avg"].cpu()) and torch.equal(st["exp_avg_sq"], state[i]["exp_avg_sq"].cpu())
+    plain.save_iteration_checkpoint(2)
+    again = trainer(tmp_path, "c", fused_ops=True, optimizer_bits=bits)
+    assert again.load_iteration_checkpoint(2)
+    for i, st in again.optimizer.state_dict()["state"].items():
+        assert all(torch.equal(st[k], state[i][k]) for k in ("step", "exp_avg", "exp_avg_sq"))
+    assert again.optimizer.param_groups[0]["lr"] == fused.optimizer.param_groups[0]["lr"]
+    assert np.isfinite(learn(again)["loss"])
+
+
+def test_fused_training_refreshes_self_play(tmp_path):
+    """The weights and statistics that the fused step writes move their version counters: the next episodes run on them."""
+    tr = trainer(tmp_path, "s", blocks=1, filters=32, fused_ops=True, num_parallel_games=4, num_simulations=4)
+    tr.execute_parallel_episodes(4)
+    learn(tr)
+    assert tr._weights_changed
+    tr.execute_parallel_episodes(4)
+    assert not tr._weights_changed
+    probe = torch.from_numpy(examples()[0][:4]).cuda()
+    probe[:, 2] = 1
+    probe[:, 1] *= 1 - probe[:, 0]
+    tr.model.eval()
+    with torch.no_grad():
+        want = torch.softmax(tr.model(probe)[0], 1)
+    assert float((tr._selfplay.inference.forward_planes(probe)[0] - want).abs().max()) < 2e-2
+
+
+def test_fused_trainer_refusals(tmp_path):
+    from alphazero_amd.model import AlphaZeroNet
+    from alphazero_amd.parallel_trainer import ParallelTrainer
+    with pytest.raises(ValueError, match="fused_ops=True"):
+        ParallelTrainer(AlphaZeroNet(1, 32), checkpoint_dir=str(tmp_path), verbose=False, optimizer_bits=8)
+    with pytest.raises(ValueError, match="on a GPU"):
+        ParallelTrainer(AlphaZeroNet(1, 32), checkpoint_dir=str(tmp_path), verbose=False, fused_ops=True)
+    with pytest.raises(ValueError, match="GPU tensor"):
+        AlphaZeroNet(1, 32).use_fused_ops()(torch.zeros(2, 3, 8, 8))

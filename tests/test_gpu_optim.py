@@ -225,7 +225,7 @@ def test_parameters_without_gradient_groups_and_empty_ones():
     params = tensors([(10,), (300,), (0,), (7, 7)])
     params[1].grad = None
     params[2].grad = torch.zeros(0, device="cuda")
-    opt = FusedAdam([{"params": params[:2], "lr": 1e-2}, {"params": params[2:], "lr": 1e-3, "weight_decay": 0.5, "decoupled": True}])
+    opt = FusedAdam([{"params": params[:2], "lr": 1e-2}, {"params": params[2:], "lr": 1e-3, "weight_decay": 0.5, "decoupled_weight_decay": True}])
     kept = params[1].detach().clone()
     start = [p.detach().clone() for p in params]
     opt.step(max_norm=1.0)

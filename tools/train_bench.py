@@ -22,6 +22,8 @@ ap.add_argument("--bf16", action="store_true", help="autocast the forward to bfl
 ap.add_argument("--find", action="store_true", help="let MIOpen time its solvers per layer shape (cudnn.benchmark)")
 ap.add_argument("--channels-last", action="store_true", help="keep weights and activations NHWC")
 ap.add_argument("--graph", action="store_true", help="replay full batches from captured HIP graphs (ParallelTrainer(graph_step=True))")
+ap.add_argument("--fused", action="store_true", help="the library's own training operators (ParallelTrainer(fused_ops=True))")
+ap.add_argument("--bits", type=int, default=32, help="bits of the optimiser's moments (8 needs --fused)")
 a = ap.parse_args()
 torch.backends.cudnn.benchmark = a.find
 rs = np.random.RandomState(0)
@@ -34,7 +36,8 @@ model = AlphaZeroNet(num_blocks=a.blocks, num_filters=128).cuda()
 if a.channels_last:
     model = model.to(memory_format=torch.channels_last)
 tr = ParallelTrainer(model, device="cuda", checkpoint_dir=tempfile.mkdtemp(), verbose=False,
-                     autocast_dtype=torch.bfloat16 if a.bf16 else None, graph_step=a.graph)
+                     autocast_dtype=torch.bfloat16 if a.bf16 else None, graph_step=a.graph,
+                     fused_ops=a.fused, optimizer_bits=a.bits)
 tr.add_examples(ExampleArrays(states, pol, wls))
 tr.learn(epochs=1, batch_size=a.batch)            # warm-up (MIOpen kernel selection)
 torch.cuda.synchronize()
@@ -43,5 +46,5 @@ stats = tr.learn(epochs=1, batch_size=a.batch)
 torch.cuda.synchronize()
 dt = time.perf_counter() - t0
 steps = -(-2 * a.examples // a.batch)
-print(f"learn(){' graph' if a.graph else ''}{' bf16' if a.bf16 else ''}: {2 * a.examples} augmented examples, batch {a.batch}, {a.blocks}x128: {dt:.2f} s, "
+print(f"learn(){' graph' if a.graph else ''}{' bf16' if a.bf16 else ''}{' fused' if a.fused else ''}{' 8-bit moments' if a.bits == 8 else ''}: {2 * a.examples} augmented examples, batch {a.batch}, {a.blocks}x128: {dt:.2f} s, "
       f"{steps / dt:.1f} steps/s, {2 * a.examples / dt:.0f} examples/s, loss {stats['loss']:.3f}")
