@@ -694,29 +694,62 @@ __device__ inline void channel_grads(const NormParams& p, int block) {
 // and a weight is loaded once for all of them.  Weights are read along their rows, 16 bytes a lane.
 constexpr int GATE_THREADS = 256;
 
-// out(j, sums) for every row j of w [rows][cols]: the row against the four boards' vectors v.  L lanes to a row; every lane
-// of them gets the sums.
-template <int L, typename F>
-__device__ inline void rows_times(const float* w, int rows, int cols, const f32x4* v, F&& out) {
+// Four weights from p on; FOURS: the rows are multiples of four.
+template <bool FOURS>
+__device__ inline f32x4 four_weights(const float* p, int left) {
+    return FOURS ? *(const f32x4_loose*)p : load_pack(p, left);
+}
+
+template <typename F>
+__device__ inline void with_fours(int cols, F&& f) {
+    if (cols % 4 == 0) f(std::true_type());
+    else f(std::false_type());
+}
+
+// out(j, bias[j] + row j of w [rows][cols] against the four boards' vectors v).  L lanes to a row, ROWS_AHEAD rows' loads
+// under way; every lane of them gets the sums.
+constexpr int ROWS_AHEAD = 4;
+
+template <int L, bool FOURS, typename F>
+__device__ inline void rows_times(const float* w, const float* bias, int rows, int cols, const f32x4* v, F&& out) {
+    constexpr int STEP = GATE_THREADS / L;
     const int lane = threadIdx.x % L;
-    for (int j = threadIdx.x / L; j < rows; j += GATE_THREADS / L) {
-        f32x4 s = 0.f;
-        for (int c = lane * 4; c < cols; c += L * 4) {
-            const f32x4 q = load_pack(w + (size_t)j * cols + c, cols - c);
+    for (int j0 = threadIdx.x / L; j0 < rows; j0 += STEP * ROWS_AHEAD) {
+        f32x4 s[ROWS_AHEAD];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s += q[i] * v[c + i < cols ? c + i : 0];
+        for (int u = 0; u < ROWS_AHEAD; ++u) s[u] = lane == 0 ? bias[j0 + u * STEP < rows ? j0 + u * STEP : j0] : 0.f;
+        for (int c = lane * 4; c < cols; c += L * 4) {
+            f32x4 q[ROWS_AHEAD];
+#pragma unroll
+            for (int u = 0; u < ROWS_AHEAD; ++u) {
+                const int j = j0 + u * STEP;
+                q[u] = four_weights<FOURS>(w + (size_t)(j < rows ? j : j0) * cols + c, cols - c);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 vi = v[FOURS || c + i < cols ? c + i : 0];
+#pragma unroll
+                for (int u = 0; u < ROWS_AHEAD; ++u) s[u] += q[u][i] * vi;
+            }
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[r] = lane_sum<L>(s[r]);
-        out(j, s);
+        for (int u = 0; u < ROWS_AHEAD; ++u) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[u][r] = lane_sum<L>(s[u][r]);
+            const int j = j0 + u * STEP;
+            if (j < rows) out(j, s[u]);
+        }
     }
 }
 
 template <typename F>
-__device__ inline void rows_times(const float* w, int rows, int cols, const f32x4* v, F&& out) {
-    if (cols <= 16) rows_times<4>(w, rows, cols, v, out);
-    else if (cols <= 32) rows_times<8>(w, rows, cols, v, out);
-    else rows_times<16>(w, rows, cols, v, out);
+__device__ inline void rows_times(const float* w, const float* bias, int rows, int cols, const f32x4* v, F&& out) {
+    with_fours(cols, [&](auto fours) {
+        constexpr bool FOURS = decltype(fours)::value;
+        if (cols <= 16) rows_times<4, FOURS>(w, bias, rows, cols, v, out);
+        else if (cols <= 32) rows_times<8, FOURS>(w, bias, rows, cols, v, out);
+        else rows_times<16, FOURS>(w, bias, rows, cols, v, out);
+    });
 }
 
 // out(k, sums) for every column k: the columns of w against v.  A thread takes four columns and every parts-th row; the parts
@@ -730,18 +763,29 @@ __device__ inline void columns_times(const float* w, int rows, int cols, const f
     for (int at = 0; at < fours; at += wide) {
         const int k = (at + x) * 4;
         f32x4 s[4] = {0.f, 0.f, 0.f, 0.f};
-        if (k < cols) {
-#pragma unroll 4
-            for (int j = y; j < rows; j += parts) {
-                const f32x4 q = load_pack(w + (size_t)j * cols + k, cols - k), vj = v[j];
+        if (k < cols)
+            with_fours(cols, [&](auto whole) {
+                // (rows past the end are loaded again and count nothing: a guard on each would make their loads wait in turn)
+                for (int j0 = y; j0 < rows; j0 += parts * ROWS_AHEAD) {
+                    f32x4 q[ROWS_AHEAD];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[i] += q[i] * vj;
-            }
-        }
+                    for (int u = 0; u < ROWS_AHEAD; ++u) {
+                        const int j = j0 + u * parts;
+                        q[u] = four_weights<decltype(whole)::value>(w + (size_t)(j < rows ? j : j0) * cols + k, cols - k);
+                    }
+#pragma unroll
+                    for (int u = 0; u < ROWS_AHEAD; ++u) {
+                        const int j = j0 + u * parts;
+                        const f32x4 vj = v[j < rows ? j : j0] * (j < rows ? 1.f : 0.f);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[i] += q[u][i] * vj;
+                    }
+                }
+            });
 #pragma unroll
         for (int i = 0; i < 4; ++i) part[(y * wide + x) * 4 + i] = s[i];
         __syncthreads();
-        const int share = GATE_THREADS / (wide * 4) > 64 ? 64 : wide * 4 < GATE_THREADS ? GATE_THREADS / (wide * 4) : 1;   // lanes to a sum
+        const int share = wide * 4 < GATE_THREADS ? GATE_THREADS / (wide * 4) : 1;                   // lanes to a sum: 1 to 64
         for (int i = threadIdx.x / share; i < wide * 4; i += GATE_THREADS / share) {
             f32x4 t = 0.f;
             for (int q = threadIdx.x % share; q < parts; q += share) t += part[q * wide * 4 + i];
@@ -767,19 +811,17 @@ __global__ __launch_bounds__(GATE_THREADS) void k_gate_forward(const NormParams 
         q[c] = v;
     }
     __syncthreads();
-    rows_times(p.w1, p.hidden, p.c, q, [&](int k, const f32x4 s) {
-        const float b = p.b1[k];
-        f32x4 on;
+    rows_times(p.w1, p.b1, p.hidden, p.c, q, [&](int k, f32x4 s) {
 #pragma unroll
-        for (int r = 0; r < GATE_ROWS; ++r) on[r] = not_below_zero(s[r] + b);
-        h[k] = on;                                           // every lane of the row writes the same
+        for (int r = 0; r < GATE_ROWS; ++r) s[r] = not_below_zero(s[r]);
+        h[k] = s;                                            // every lane of the row writes the same
     });
     __syncthreads();
     for (int i = threadIdx.x; i < GATE_ROWS * p.hidden; i += GATE_THREADS) {
         const int r = i / p.hidden, k = i % p.hidden;
         if (r < rows) p.h[(n0 + r) * p.hidden + k] = h[k][r];
     }
-    rows_times(p.w2, 2 * p.c, p.hidden, h, [&](int j, const f32x4 s) { e[j] = s + p.b2[j]; });
+    rows_times(p.w2, p.b2, 2 * p.c, p.hidden, h, [&](int j, const f32x4 s) { e[j] = s; });
     __syncthreads();
     for (int c = threadIdx.x; c < p.c; c += GATE_THREADS) {
         const float scale = p.weight[c] * p.inv[c], shift = p.bias[c] - scale * p.mean[c];
@@ -801,45 +843,59 @@ __global__ __launch_bounds__(GATE_THREADS) void k_gate_backward(const NormParams
     f32x4 *de = lds4, *dh = de + 2 * p.c, *part = dh + p.hidden;     // [2c], [hidden], [GATE_THREADS * 4]
     const int64_t n0 = (int64_t)blockIdx.x * GATE_ROWS;
     const int rows = (int)(p.n - n0 < GATE_ROWS ? p.n - n0 : GATE_ROWS);
+    // (a board past the end is read as the first one and not written: a guard on each load would make them wait in turn)
+    const auto board = [&](int r) { return n0 + (r < rows ? r : 0); };
     for (int c = threadIdx.x; c < p.c; c += GATE_THREADS) {
         const float scale = p.weight[c] * p.inv[c], bias = p.bias[c];
-        f32x4 w = 0.f, b = 0.f;
+        f32x4 gate, s1, s2;
+#pragma unroll
+        for (int r = 0; r < GATE_ROWS; ++r) {
+            const int64_t row = board(r) * p.c + c;
+            gate[r] = p.gate[row];
+            s1[r] = p.s1[row];
+            s2[r] = p.s2[row];
+        }
+        const f32x4 w = gate * (1.f - gate) * (scale * s2 + bias * s1);
+        de[c] = w;
+        de[p.c + c] = s1;
 #pragma unroll
         for (int r = 0; r < GATE_ROWS; ++r)
             if (r < rows) {
-                const int64_t row = (n0 + r) * p.c + c;
-                const float gate = p.gate[row];
-                b[r] = p.s1[row];
-                w[r] = gate * (1.f - gate) * (scale * p.s2[row] + bias * b[r]);
                 p.de[(n0 + r) * 2 * p.c + c] = w[r];
-                p.de[(n0 + r) * 2 * p.c + p.c + c] = b[r];
+                p.de[(n0 + r) * 2 * p.c + p.c + c] = s1[r];
             }
-        de[c] = w;
-        de[p.c + c] = b;
     }
     __syncthreads();
     columns_times(p.w2, 2 * p.c, p.hidden, de, part, [&](int k, f32x4 s) {
+        f32x4 h;
 #pragma unroll
-        for (int r = 0; r < GATE_ROWS; ++r)
-            if (r < rows) {
-                const int64_t at = (n0 + r) * p.hidden + k;
-                if (!(p.h[at] > 0.f)) s[r] = 0.f;
-                p.dh[at] = s[r];
-            }
+        for (int r = 0; r < GATE_ROWS; ++r) h[r] = p.h[board(r) * p.hidden + k];
+#pragma unroll
+        for (int r = 0; r < GATE_ROWS; ++r) {
+            if (!(h[r] > 0.f)) s[r] = 0.f;
+            if (r < rows) p.dh[(n0 + r) * p.hidden + k] = s[r];
+        }
         dh[k] = s;
     });
     columns_times(p.w1, p.hidden, p.c, dh, part, [&](int c, const f32x4 s) {
         // this workgroup's share of dy's channel sums
         const float mean = p.mean[c];
+        f32x4 gate, s1, s2, m;
+#pragma unroll
+        for (int r = 0; r < GATE_ROWS; ++r) {
+            const int64_t row = board(r) * p.c + c;
+            gate[r] = p.gate[row];
+            s1[r] = p.s1[row];
+            s2[r] = p.s2[row];
+            m[r] = p.board_mean[row];
+        }
         float a = 0.f, b = 0.f;
 #pragma unroll
         for (int r = 0; r < GATE_ROWS; ++r)
             if (r < rows) {
-                const int64_t row = (n0 + r) * p.c + c;
-                const float gate = p.gate[row];
-                p.dq[row] = s[r];
-                a += gate * p.s1[row] + s[r];
-                b += gate * p.s2[row] + s[r] * (p.board_mean[row] - mean);
+                p.dq[(n0 + r) * p.c + c] = s[r];
+                a += gate[r] * s1[r] + s[r];
+                b += gate[r] * s2[r] + s[r] * (m[r] - mean);
             }
         p.part_a[(size_t)blockIdx.x * p.c + c] = a;
         p.part_b[(size_t)blockIdx.x * p.c + c] = b;
