@@ -921,9 +921,11 @@ __host__ __device__ inline TileShape tile_shape(int m, int k) {
 
 __host__ __device__ inline int weight_tiles(const NormParams& p) { return tile_shape(2 * p.c, p.hidden).tiles + tile_shape(p.hidden, p.c).tiles; }
 
-// Ranges of at least 64 boards (two rounds of a wavefront), and no more than fill the chip a few times.
+// Ranges of at least 64 boards (two rounds of a wavefront), and no more workgroups than twice the compute units: every
+// range is a partial tile more to join.  (At 4096 x 256, 24 tiles: 64 ranges 19.5 us and 7 us more in the pass that joins
+// them, 32 ranges 17.3, 16 ranges 15.8; at 1024 x 128, 12 tiles: 16 ranges 5.0 us, 8 ranges 6.3, 4 ranges 8.4.)
 __host__ __device__ inline int weight_splits(const NormParams& p) {
-    const int64_t most = (p.n + 63) / 64, enough = 2048 / weight_tiles(p);
+    const int64_t most = (p.n + 63) / 64, enough = 512 / weight_tiles(p);
     return (int)(enough < 1 ? 1 : most < enough ? most : enough);
 }
 
@@ -948,23 +950,29 @@ __device__ inline void weight_tile(const NormParams& p, int job) {
         shift[j] = second ? 0.f : p.bias[c] - scale[j] * p.mean[c];
     }
     const int64_t from = p.n * split / splits, to = p.n * (split + 1) / splits;
-    for (int64_t n = from + wave; n < to; n += TILE_WAVES * TILE_BOARDS) {
-        f32x4 a[TILE_BOARDS], b[TILE_BOARDS];
+    const auto sum_boards = [&](auto fours) {
+        constexpr bool FOURS = decltype(fours)::value;
+        // FOURS: a lane past the end of a factor reads its last four; what comes of them is not joined
+        const int ai = FOURS && li > t.m - 4 ? t.m - 4 : li, bj = FOURS && lj > t.k - 4 ? t.k - 4 : lj;
+        for (int64_t n = from + wave; n < to; n += TILE_WAVES * TILE_BOARDS) {
+            f32x4 a[TILE_BOARDS], b[TILE_BOARDS];
 #pragma unroll
-        for (int u = 0; u < TILE_BOARDS; ++u) {
-            const int64_t nu = n + u * TILE_WAVES;
-            const bool in = nu < to;
-            a[u] = load_pack(left + (in ? nu : n) * t.m + li, in ? t.m - li : 0);
-            b[u] = load_pack(right + (in ? nu : n) * t.k + lj, t.k - lj);
+            for (int u = 0; u < TILE_BOARDS; ++u) {
+                const int64_t nu = n + u * TILE_WAVES < to ? n + u * TILE_WAVES : n;
+                a[u] = four_weights<FOURS>(left + nu * t.m + ai, t.m - ai);
+                b[u] = four_weights<FOURS>(right + nu * t.k + bj, t.k - bj);
+            }
+#pragma unroll
+            for (int u = 0; u < TILE_BOARDS; ++u) {
+                const f32x4 w = a[u] * (n + u * TILE_WAVES < to ? 1.f : 0.f), q = b[u] * scale + shift;
+                bias += w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] += w[i] * q;
+            }
         }
-#pragma unroll
-        for (int u = 0; u < TILE_BOARDS; ++u) {
-            const f32x4 q = b[u] * scale + shift;
-            bias += a[u];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] += a[u][i] * q;
-        }
-    }
+    };
+    if (t.m % 4 == 0 && t.k % 4 == 0) sum_boards(std::true_type());
+    else sum_boards(std::false_type());
 #pragma unroll
     for (int i = 0; i < 4; ++i) *(f32x4*)&lds[wave][(lane / 8 * 4 + i) * TILE + lane % 8 * 4] = acc[i];
     if (lane % 8 == 0) *(f32x4*)&lds[wave][TILE * TILE + lane / 8 * 4] = bias;
