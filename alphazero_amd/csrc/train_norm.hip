@@ -59,10 +59,11 @@ __device__ inline float not_below_zero(float v) { return v < 0.f ? 0.f : v; }   
 __device__ void join_weights(const NormParams& p, int block);
 
 // The boards whose sums chunk i holds: p.chunk_boards of them, p.abreast apart, fewer at the end.
-__device__ inline int64_t boards_in_chunk(const NormParams& p, int64_t i) {
-    const int64_t first = i / p.abreast * p.chunk_boards * p.abreast + i % p.abreast;
-    const int64_t k = first < p.n ? (p.n - 1 - first) / p.abreast + 1 : 0;
-    return k < p.chunk_boards ? k : p.chunk_boards;
+__device__ inline uint32_t boards_in_chunk(const NormParams& p, uint32_t i) {
+    const uint32_t n = (uint32_t)p.n, side = (uint32_t)p.abreast, most = (uint32_t)p.chunk_boards;
+    const uint32_t beside = side == 1 ? 0 : i % side, first = (i - beside) * most + beside;
+    const uint32_t k = first >= n ? 0 : side == 1 ? n - first : (n - 1 - first) / side + 1;
+    return k < most ? k : most;
 }
 
 // ---------------------------------------------------------------------------- [n][c][hw]: L lanes to a row
@@ -586,7 +587,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_apply(const T* __res
 
 // ------------------------------------------------------------ per channel: sums over chunks of boards in 64 bits
 constexpr int CHANNELS = 8, LINES = 64;       // a workgroup: 8 neighbouring channels, 64 chunks at a time
-constexpr int IN_FLIGHT = 4;                  // chunks whose loads a thread has under way
+constexpr int IN_FLIGHT = 8;                  // chunks whose loads a thread has under way
 
 // Sums of v over the threads of a channel; thread 0 to CHANNELS - 1 get theirs.
 template <int K>
@@ -637,7 +638,7 @@ __global__ __launch_bounds__(CHANNELS * LINES) void k_channel_stats(const NormPa
     double v[3] = {0, 0, 0};          // sums over the boards: of their means, of the means' squares, of the centred sums
     if (p.training) {
         over_chunks(p, c, [&](int64_t i, float mean, float m2) {
-            const double k = (double)boards_in_chunk(p, i), m = mean;
+            const double k = boards_in_chunk(p, (uint32_t)i), m = mean;
             v[0] += k * m;
             v[1] += k * (m * m);
             v[2] += m2;
