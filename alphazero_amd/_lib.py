@@ -64,13 +64,17 @@ class LossArgs(C.Structure):
                 + [("grads_ready", C.c_int32)])
 
 
+class AdamGroup(C.Structure):
+    _fields_ = ([(k, C.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+                + [("decoupled", C.c_int32), ("end", C.c_int32)])
+
+
 class AdamConfig(C.Structure):
-    _fields_ = ([(k, C.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")]
-                + [("decoupled", C.c_int32), ("state_bits", C.c_int32), ("seed", C.c_uint64), ("n_partials", C.c_int64)]
-                + [(k, C.c_void_p) for k in ("pieces", "m", "v", "m_scale", "v_scale", "steps", "partials", "norm", "scratch")])
+    _fields_ = ([("max_norm", C.c_double), ("seed", C.c_uint64), ("state_bits", C.c_int32)]
+                + [(k, C.c_void_p) for k in ("pieces", "m", "v", "m_scale", "v_scale", "steps", "norm", "scratch")])
 
 
-# name -> (argtypes); every entry point returns int (az_adam_plan: int64)
+# name -> (argtypes); every entry point returns int (az_adam_plan and az_adam_scratch: int64)
 _VP = C.c_void_p
 _SIGNATURES = {
     "az_version": [],
@@ -123,12 +127,12 @@ _SIGNATURES = {
     "az_policy_value_loss_forward": [C.POINTER(LossArgs), _VP],
     "az_policy_value_loss_backward": [C.POINTER(LossArgs), _VP],
     "az_adam_plan": [C.c_int32, _VP, _VP, _VP],
-    "az_grad_sumsq": [C.c_int32, _VP, _VP, _VP, _VP, C.c_int64, _VP],
-    "az_adam_step": [C.POINTER(AdamConfig), C.c_int32, C.c_int32, C.c_int32, _VP, _VP, _VP, _VP],
+    "az_adam_scratch": [C.c_int32],
+    "az_adam_step": [C.POINTER(AdamConfig), C.c_int32, C.POINTER(AdamGroup), C.c_int32, _VP, _VP, _VP, _VP],
 }
 _OPTIONAL = {}
 
-OPTIM_CHUNK, OPTIM_PAD = 4096, 256      # AZ_OPTIM_CHUNK, AZ_OPTIM_PAD
+OPTIM_CHUNK, OPTIM_PAD, OPTIM_GROUPS = 4096, 256, 48      # AZ_OPTIM_CHUNK, AZ_OPTIM_PAD, AZ_OPTIM_GROUPS
 PACKED_SAMPLE_BYTES = 792     # AZ_PACKED_SAMPLE_BYTES
 
 _lib = None
@@ -146,7 +150,7 @@ def lib():
         for name, args in _SIGNATURES.items():
             fn = getattr(L, name)
             fn.argtypes = args
-            fn.restype = C.c_int64 if name == "az_adam_plan" else C.c_int
+            fn.restype = C.c_int64 if name in ("az_adam_plan", "az_adam_scratch") else C.c_int
         for name, args in _OPTIONAL.items():
             if hasattr(L, name):
                 fn = getattr(L, name)
@@ -176,7 +180,7 @@ def torch_ops():
             raise AzError(f"alphazero_amd/_azops.so does not load ({e}): build it with alphazero_amd/csrc/build.sh "
                           "(__graft_entry__.build()).  There is no fallback path.") from e
         names = ("az_last_error", "az_norm_sizes", "az_norm_forward", "az_norm_backward", "az_policy_value_loss_ready", "az_policy_value_loss_forward",
-                 "az_policy_value_loss_backward", "az_adam_plan", "az_grad_sumsq", "az_adam_step")
+                 "az_policy_value_loss_backward", "az_adam_plan", "az_adam_scratch", "az_adam_step")
         _azops.bind({n: C.cast(getattr(L, n), C.c_void_p).value for n in names}, AzError)
         _torch_ops = _azops
     return _torch_ops

@@ -13,6 +13,8 @@
 // Layout: a workgroup takes a piece of OPT_CHUNK elements of one tensor.  Which one is in a table that is made once, in
 // device memory; the tensors' addresses travel in the kernel arguments (OPT_TABLE tensors a launch, so that the default
 // network's 214 are one), nothing is uploaded per step: it can be captured, and tensors may move between steps.
+// Two launches make a step: k_adam_begin (step counters and what follows from them, partial sums of squares) and k_adam,
+// whose workgroups each add the partial sums themselves, in the same order, while their own loads are under way.
 #include <math.h>
 
 #include <type_traits>
@@ -26,7 +28,8 @@ constexpr int OPT_CHUNK = AZ_OPTIM_CHUNK;          // elements of one tensor tha
 constexpr int OPT_BLOCK = AZ_OPTIM_PAD;            // elements that share a scale: one wavefront x 4
 constexpr int OPT_ROUNDS = OPT_CHUNK / (OPT_THREADS * 4);
 constexpr int OPT_TABLE = 240;                     // 16 bytes each: 3.75 of the 4 KB of kernel arguments
-constexpr int OPT_MASK = 896;                      // words: 28,672 tensors a launch of k_adam_begin
+constexpr int OPT_GROUPS = AZ_OPTIM_GROUPS;
+constexpr int OPT_SUMS = 1024;                     // partial sums per OPT_TABLE tensors, at most (256: k_adam_begin 13 us at 20x128, 512: 9.6, 1024: 9.1)
 static_assert(OPT_CHUNK % (OPT_THREADS * 4) == 0 && OPT_BLOCK == 256, "a wavefront covers one block of a moment");
 
 struct GradTable {
@@ -37,24 +40,23 @@ struct TensorTable {
     uint64_t grad[OPT_TABLE], param[OPT_TABLE];
 };
 
-struct TensorMask {
-    uint32_t has_grad[OPT_MASK];
-};
-
 struct StepFactors {                // per tensor, from its step counter
     float step_size, inv_root_bias2;
     uint32_t key;
 };
 
-struct OptHyper {
-    double lr, beta1, beta2, max_norm;
-    const double* partials;
-    uint32_t n_partials;
-    float* norm;                    // |g| out (may be null)
-    float* coef;                    // c out
+struct GroupRates {
+    double lr, beta1, beta2;
+    uint32_t end;                   // first tensor after the group
+};
+
+struct BeginParams {
+    GroupRates group[OPT_GROUPS];
+    const az_adam_piece* pieces;
+    uint32_t first_tensor, tensors, n_pieces, seed_key;
+    double* partials;
     float* steps;
     StepFactors* factors;
-    uint32_t seed_key;
 };
 
 struct AdamParams {
@@ -62,8 +64,11 @@ struct AdamParams {
     int decoupled;
     const az_adam_piece* pieces;
     uint32_t first_tensor;
-    const float* coef;
     const StepFactors* factors;
+    double max_norm;                // 0: no clipping
+    const double* partials;
+    uint32_t n_partials;
+    float* norm;                    // |g| out (may be null)
     void *m, *v;
     float *m_scale, *v_scale;
 };
@@ -80,13 +85,42 @@ __device__ inline f32x4 load_four(const float* p, int i, const az_adam_piece& c)
     return WHOLE ? *(const f32x4_loose*)(p + i) : load_pack(p + i, (int)c.n - i);
 }
 
-// Sum of squares of a piece in 64 bits (the products are exact there): the norm of 8 M gradients whose sizes lie decades
-// apart, and a clipping factor that does not depend on the order of the sum.
-__global__ __launch_bounds__(OPT_THREADS) void k_grad_sumsq(const GradTable t, const az_adam_piece* pieces, uint32_t first_tensor, double* partials) {
-    const az_adam_piece c = pieces[blockIdx.x];
-    const float* g = (const float*)t.grad[c.tensor - first_tensor];
+// The sum of a workgroup's v in all its threads, always in the same order.
+__device__ inline double block_sum(double v) {
+    __shared__ double part[OPT_THREADS / 64];
+    for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = part[0];
+    for (int w = 1; w < OPT_THREADS / 64; ++w) v += part[w];
+    return v;
+}
+
+// The last workgroup: the tensors' step counters and what follows from them.  The others: partial sums of squares, in
+// 64 bits (the products are exact there): the norm of 8 M gradients whose sizes lie decades apart, and a clipping factor
+// that does not depend on the order of the sum.
+__global__ __launch_bounds__(OPT_THREADS) void k_adam_begin(const GradTable t, const BeginParams h) {
+    if (blockIdx.x == gridDim.x - 1) {
+        for (uint32_t i = threadIdx.x; i < h.tensors; i += OPT_THREADS) {
+            if (!t.grad[i]) continue;
+            const uint32_t tensor = h.first_tensor + i;
+            int g = 0;
+            while (h.group[g].end <= tensor) ++g;
+            const float step = h.steps[tensor] + 1.f;
+            h.steps[tensor] = step;
+            StepFactors f;
+            f.step_size = (float)(h.group[g].lr / (1.0 - pow(h.group[g].beta1, (double)step)));
+            f.inv_root_bias2 = 1.f / (float)sqrt(1.0 - pow(h.group[g].beta2, (double)step));
+            f.key = h.seed_key + (uint32_t)step * 0x85EBCA6Bu;
+            h.factors[tensor] = f;
+        }
+        return;
+    }
     double s = 0.0;
-    if (g) {
+    for (uint32_t piece = blockIdx.x; piece < h.n_pieces; piece += gridDim.x - 1) {
+        const az_adam_piece c = h.pieces[piece];
+        const float* g = (const float*)t.grad[c.tensor - h.first_tensor];
+        if (!g) continue;
         g += (size_t)c.chunk * OPT_CHUNK;
         with_whole(c, [&](auto whole) {
             f32x4 v[OPT_ROUNDS];
@@ -98,44 +132,24 @@ __global__ __launch_bounds__(OPT_THREADS) void k_grad_sumsq(const GradTable t, c
                 for (int k = 0; k < 4; ++k) s += (double)v[it][k] * (double)v[it][k];
         });
     }
-    for (int off = 32; off; off >>= 1) s += __shfl_xor(s, off);
-    __shared__ double part[OPT_THREADS / 64];
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < OPT_THREADS / 64; ++w) s += part[w];
-        partials[blockIdx.x] = s;
-    }
+    s = block_sum(s);
+    if (threadIdx.x == 0) h.partials[blockIdx.x] = s;
 }
 
-// One workgroup: the norm and the clipping factor from the partial sums (in a fixed order), and the tensors' step
-// counters with what follows from them.
-__global__ __launch_bounds__(1024) void k_adam_begin(const TensorMask mask, uint32_t first, uint32_t count, OptHyper h) {
-    if (h.coef) {
-        double s = 0.0;
-#pragma unroll 4
-        for (uint32_t i = threadIdx.x; i < h.n_partials; i += 1024) s += h.partials[i];
-        for (int off = 32; off; off >>= 1) s += __shfl_xor(s, off);
-        __shared__ double part[16];
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < 16; ++w) s += part[w];
-            const double norm = sqrt(s), c = h.max_norm / (norm + 1e-6);
-            if (h.norm) *h.norm = (float)norm;
-            *h.coef = (float)(c > 1.0 ? 1.0 : c);      // a NaN stays one
-        }
+// The clipping factor, from all partial sums.
+__device__ inline float clip_factor(const AdamParams& a) {
+    constexpr int EACH = OPT_SUMS / OPT_THREADS;       // of one launch's sums, loaded together
+    double s = 0.0;
+    for (uint32_t i = threadIdx.x; i < a.n_partials; i += OPT_SUMS) {
+        double part[EACH];
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) part[u] = a.partials[i + u * OPT_THREADS < a.n_partials ? i + u * OPT_THREADS : i];
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) s += i + u * OPT_THREADS < a.n_partials ? part[u] : 0.0;
     }
-    for (uint32_t i = threadIdx.x; i < count; i += 1024) {
-        if (!(mask.has_grad[i / 32] >> (i % 32) & 1)) continue;
-        const float t = h.steps[first + i] + 1.f;
-        h.steps[first + i] = t;
-        StepFactors f;
-        f.step_size = (float)(h.lr / (1.0 - pow(h.beta1, (double)t)));
-        f.inv_root_bias2 = 1.f / (float)sqrt(1.0 - pow(h.beta2, (double)t));
-        f.key = h.seed_key + (uint32_t)t * 0x85EBCA6Bu;
-        h.factors[first + i] = f;
-    }
+    const double norm = sqrt(block_sum(s)), c = a.max_norm / (norm + 1e-6);
+    if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = (float)norm;
+    return (float)(c > 1.0 ? 1.0 : c);             // a NaN stays one
 }
 
 // Correctly rounded root of a value that is not denormal: the hardware's, off by at most a last place, and the signs of what
@@ -215,16 +229,21 @@ __device__ inline uint32_t mix32(uint32_t z) {
 template <int BITS>
 __global__ __launch_bounds__(OPT_THREADS) void k_adam(const TensorTable t, const AdamParams a) {
     const az_adam_piece c = a.pieces[blockIdx.x];
+    const bool clip = a.max_norm > 0.0;
     const float* gp = (const float*)t.grad[c.tensor - a.first_tensor];
-    if (!gp) return;
+    if (!gp) {
+        if (clip && blockIdx.x == 0) clip_factor(a);                // the norm is this workgroup's to write
+        return;
+    }
     gp += (size_t)c.chunk * OPT_CHUNK;
     float* pp = (float*)t.param[c.tensor - a.first_tensor] + (size_t)c.chunk * OPT_CHUNK;
     const size_t at = (size_t)c.offset * OPT_BLOCK;                 // the piece's place in the moments
     const StepFactors f = a.factors[c.tensor];
-    const float coef = a.coef ? *a.coef : 1.f;
+    float coef = 1.f;
     with_whole(c, [&](auto whole) {
         constexpr bool WHOLE = decltype(whole)::value;
         constexpr int AHEAD = WHOLE ? OPT_ROUNDS : 1;          // rounds whose loads are under way together
+        if (!WHOLE && clip) coef = clip_factor(a);
 #pragma unroll
         for (int it0 = 0; it0 < OPT_ROUNDS; it0 += AHEAD) {
             f32x4 p[AHEAD], g[AHEAD], m[AHEAD], v[AHEAD];
@@ -247,6 +266,7 @@ __global__ __launch_bounds__(OPT_THREADS) void k_adam(const TensorTable t, const
                     sv[u] = a.v_scale[(at + i) / OPT_BLOCK];
                 }
             }
+            if (WHOLE && clip) coef = clip_factor(a);
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 const int i = ((it0 + u) * OPT_THREADS + threadIdx.x) * 4;
@@ -258,7 +278,7 @@ __global__ __launch_bounds__(OPT_THREADS) void k_adam(const TensorTable t, const
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float gk = g[u][k], pk = p[u][k];
-                    if (a.coef) gk = gk * coef;
+                    if (clip) gk = gk * coef;
                     if (a.decoupled) pk = pk * a.decay;
                     else if (a.decay != 0.f) gk = gk + pk * a.decay;
                     const float vk = BITS == 32 ? v[u][k] : v[u][k] * v[u][k];
@@ -314,29 +334,15 @@ static int for_ranges(int32_t begin, int32_t end, const int64_t* sizes, F&& laun
     return AZ_OK;
 }
 
-static int check_tensors(const char* what, int32_t count, const int64_t* sizes, const uint64_t* params, const uint64_t* grads, int64_t* pieces) {
-    AZ_CHECK_ARG(count >= 0 && count <= 1 << 20 && (count == 0 || (sizes && grads)), "%s: null table, or %d tensors (up to 2^20)", what, count);
-    *pieces = 0;
-    for (int32_t i = 0; i < count; ++i) {
-        AZ_CHECK_ARG(sizes[i] >= 0 && sizes[i] <= int64_t(1) << 38, "%s: tensor %d has %lld elements", what, i, (long long)sizes[i]);
-        *pieces += pieces_of(sizes[i]);
-        if (!grads[i] || !sizes[i]) continue;
-        AZ_CHECK_ARG(grads[i] % 4 == 0, "%s: gradient %d is not aligned to 4 bytes", what, i);
-        AZ_CHECK_ARG(!params || (params[i] && params[i] % 4 == 0), "%s: parameter %d is null or not aligned to 4 bytes", what, i);
-    }
-    AZ_CHECK_ARG(*pieces <= 0x7FFFFFFF, "%s: too many elements", what);
-    return AZ_OK;
-}
-
 }  // namespace az
 
 using namespace az;
 
 extern "C" int64_t az_adam_plan(int32_t count, const int64_t* sizes_host, int64_t* offsets_host, az_adam_piece* pieces_host) {
-    if (count < 0 || (count && !sizes_host)) AZ_FAIL(AZ_ERR_ARG, "az_adam_plan: null sizes");
+    AZ_CHECK_ARG(count >= 0 && (count == 0 || sizes_host), "az_adam_plan: null sizes");
     int64_t at = 0, piece = 0;
     for (int32_t i = 0; i < count; ++i) {
-        if (sizes_host[i] < 0 || sizes_host[i] > int64_t(1) << 38) AZ_FAIL(AZ_ERR_ARG, "az_adam_plan: tensor %d has %lld elements", i, (long long)sizes_host[i]);
+        AZ_CHECK_ARG(sizes_host[i] >= 0 && sizes_host[i] <= int64_t(1) << 38, "az_adam_plan: tensor %d has %lld elements", i, (long long)sizes_host[i]);
         if (offsets_host) offsets_host[i] = at;
         for (int64_t k = 0; k < pieces_of(sizes_host[i]); ++k, ++piece) {
             if (!pieces_host) continue;
@@ -345,89 +351,96 @@ extern "C" int64_t az_adam_plan(int32_t count, const int64_t* sizes_host, int64_
         }
         at += (sizes_host[i] + OPT_BLOCK - 1) / OPT_BLOCK * OPT_BLOCK;
     }
-    if (at / OPT_BLOCK > 0xFFFFFFFF) AZ_FAIL(AZ_ERR_ARG, "az_adam_plan: too many elements");
+    AZ_CHECK_ARG(at / OPT_BLOCK <= 0xFFFFFFFF && piece <= 0x7FFFFFFF, "az_adam_plan: too many elements");
     if (offsets_host) offsets_host[count] = at;
     return piece;
 }
 
-extern "C" int az_grad_sumsq(int32_t count, const uint64_t* grads_host, const int64_t* sizes_host, const az_adam_piece* pieces_dev,
-                             double* partials_dev, int64_t n_partials, void* stream) {
-    int64_t pieces;
-    const int rc = check_tensors("az_grad_sumsq", count, sizes_host, nullptr, grads_host, &pieces);
-    if (rc != AZ_OK) return rc;
-    AZ_CHECK_ARG(n_partials == pieces && (pieces == 0 || (partials_dev && pieces_dev)), "az_grad_sumsq: %lld partial sums are written, room for %lld",
-                 (long long)pieces, (long long)n_partials);
-    return for_ranges(0, count, sizes_host, [&](int32_t first, int32_t k, int64_t piece, uint32_t n) -> int {
-        GradTable t;
-        for (int32_t i = 0; i < k; ++i) t.grad[i] = grads_host[first + i];
-        hipLaunchKernelGGL(k_grad_sumsq, dim3(n), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, pieces_dev + piece, (uint32_t)first, partials_dev + piece);
-        AZ_HIP(hipGetLastError());
-        return AZ_OK;
-    });
+extern "C" int64_t az_adam_scratch(int32_t count) {
+    AZ_CHECK_ARG(count >= 0, "az_adam_scratch: %d tensors", count);
+    return (int64_t)((count + OPT_TABLE - 1) / OPT_TABLE) * OPT_SUMS * sizeof(double) + (int64_t)count * sizeof(StepFactors);
 }
 
-extern "C" int az_adam_step(const az_adam_config* cfg, int32_t count, int32_t begin, int32_t end, const uint64_t* params_host,
+extern "C" int az_adam_step(const az_adam_config* cfg, int32_t n_groups, const az_adam_group* groups, int32_t count, const uint64_t* params_host,
                             const uint64_t* grads_host, const int64_t* sizes_host, void* stream) {
-    AZ_CHECK_ARG(cfg, "az_adam_step: null config");
-    int64_t pieces;
-    int rc = check_tensors("az_adam_step", count, sizes_host, params_host, grads_host, &pieces);
-    if (rc != AZ_OK) return rc;
-    AZ_CHECK_ARG(0 <= begin && begin <= end && end <= count, "az_adam_step: tensors %d to %d of %d", begin, end, count);
-    if (begin == end) return AZ_OK;
-    AZ_CHECK_ARG(params_host, "az_adam_step: null parameters");
+    AZ_CHECK_ARG(cfg && groups && n_groups >= 1 && n_groups <= OPT_GROUPS, "az_adam_step: null config, or %d groups (1 to %d)", n_groups, OPT_GROUPS);
+    AZ_CHECK_ARG(count >= 0 && (count == 0 || (sizes_host && grads_host && params_host)), "az_adam_step: null table");
+    int64_t pieces = 0;
+    for (int32_t i = 0; i < count; ++i) {
+        AZ_CHECK_ARG(sizes_host[i] >= 0 && sizes_host[i] <= int64_t(1) << 38, "az_adam_step: tensor %d has %lld elements", i, (long long)sizes_host[i]);
+        pieces += pieces_of(sizes_host[i]);
+        if (!grads_host[i] || !sizes_host[i]) continue;
+        AZ_CHECK_ARG(grads_host[i] % 4 == 0, "az_adam_step: gradient %d is not aligned to 4 bytes", i);
+        AZ_CHECK_ARG(params_host[i] && params_host[i] % 4 == 0, "az_adam_step: parameter %d is null or not aligned to 4 bytes", i);
+    }
+    for (int32_t g = 0, at = 0; g < n_groups; at = groups[g++].end)
+        AZ_CHECK_ARG(groups[g].end >= at && (g + 1 < n_groups ? groups[g].end <= count : groups[g].end == count),
+                     "az_adam_step: group %d ends at %d of %d tensors", g, groups[g].end, count);
+    if (pieces == 0) return AZ_OK;
+    AZ_CHECK_ARG(pieces <= 0x7FFFFFFF, "az_adam_step: too many elements");
     AZ_CHECK_ARG(cfg->state_bits == 32 || cfg->state_bits == 8, "az_adam_step: moments in %d bits (32 or 8)", cfg->state_bits);
     AZ_CHECK_ARG(cfg->m_dev && cfg->v_dev && cfg->steps_dev && cfg->scratch_dev && cfg->pieces_dev, "az_adam_step: null state");
     AZ_CHECK_ARG(cfg->state_bits == 32 || (cfg->m_scale_dev && cfg->v_scale_dev), "az_adam_step: 8-bit moments need scales");
-    AZ_CHECK_ARG((uintptr_t)cfg->m_dev % 16 == 0 && (uintptr_t)cfg->v_dev % 16 == 0, "az_adam_step: the moments must be 16-byte aligned");
-    AZ_CHECK_ARG(!(cfg->max_norm > 0) || (cfg->n_partials == pieces && (pieces == 0 || cfg->partials_dev)),
-                 "az_adam_step: %lld partial sums, %lld wanted", (long long)cfg->n_partials, (long long)pieces);
-    float* scratch = (float*)cfg->scratch_dev;            // [0] clipping factor, then the tensors' factors
-    OptHyper h;
-    h.lr = cfg->lr;
-    h.beta1 = cfg->beta1;
-    h.beta2 = cfg->beta2;
-    h.max_norm = cfg->max_norm;
-    h.partials = cfg->partials_dev;
-    h.n_partials = (uint32_t)cfg->n_partials;
-    h.norm = cfg->norm_dev;
-    h.coef = cfg->max_norm > 0 ? scratch : nullptr;
-    h.steps = cfg->steps_dev;
-    h.factors = (StepFactors*)(scratch + 4);
-    h.seed_key = (uint32_t)cfg->seed * 0x9E3779B9u;
-    AdamParams a;
-    a.beta1 = (float)cfg->beta1;
-    a.one_beta1 = (float)(1.0 - cfg->beta1);
-    a.beta2 = (float)cfg->beta2;
-    a.one_beta2 = (float)(1.0 - cfg->beta2);
-    a.eps = (float)cfg->eps;
-    a.decoupled = cfg->decoupled != 0;
-    a.decay = a.decoupled ? (float)(1.0 - cfg->lr * cfg->weight_decay) : (float)cfg->weight_decay;
-    a.coef = h.coef;
-    a.factors = h.factors;
-    a.m = cfg->m_dev;
-    a.v = cfg->v_dev;
-    a.m_scale = cfg->m_scale_dev;
-    a.v_scale = cfg->v_scale_dev;
-    for (int32_t at = begin; at < end; at += OPT_MASK * 32) {
-        TensorMask mask = {};
-        const uint32_t k = (uint32_t)(end - at < OPT_MASK * 32 ? end - at : OPT_MASK * 32);
-        for (uint32_t i = 0; i < k; ++i) mask.has_grad[i / 32] |= (grads_host[at + i] && sizes_host[at + i] ? 1u : 0u) << (i % 32);
-        hipLaunchKernelGGL(k_adam_begin, dim3(1), dim3(1024), 0, (hipStream_t)stream, mask, (uint32_t)at, k, h);
+    AZ_CHECK_ARG((uintptr_t)cfg->m_dev % 16 == 0 && (uintptr_t)cfg->v_dev % 16 == 0 && (uintptr_t)cfg->scratch_dev % 16 == 0,
+                 "az_adam_step: moments and scratch memory must be 16-byte aligned");
+    const bool clip = cfg->max_norm > 0;
+    double* partials = (double*)cfg->scratch_dev;         // then the tensors' factors
+    StepFactors* factors = (StepFactors*)(partials + (size_t)((count + OPT_TABLE - 1) / OPT_TABLE) * OPT_SUMS);
+    uint32_t n_partials = 0;
+    int rc = for_ranges(0, count, sizes_host, [&](int32_t first, int32_t k, int64_t piece, uint32_t n) -> int {
+        GradTable t;
+        for (int32_t i = 0; i < k; ++i) t.grad[i] = sizes_host[first + i] ? grads_host[first + i] : 0;
+        BeginParams b;
+        for (int32_t g = 0; g < n_groups; ++g) b.group[g] = {groups[g].lr, groups[g].beta1, groups[g].beta2, (uint32_t)groups[g].end};
+        b.pieces = cfg->pieces_dev + piece;
+        b.first_tensor = (uint32_t)first;
+        b.tensors = (uint32_t)k;
+        b.n_pieces = n;
+        b.seed_key = (uint32_t)cfg->seed * 0x9E3779B9u;
+        b.partials = partials + n_partials;
+        b.steps = cfg->steps_dev;
+        b.factors = factors;
+        const uint32_t sums = !clip ? 0 : n < (uint32_t)OPT_SUMS ? n : OPT_SUMS;
+        hipLaunchKernelGGL(k_adam_begin, dim3(sums + 1), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, b);
         AZ_HIP(hipGetLastError());
-    }
-    return for_ranges(begin, end, sizes_host, [&](int32_t first, int32_t k, int64_t piece, uint32_t n) -> int {
-        TensorTable t;
-        for (int32_t i = 0; i < k; ++i) {
-            t.grad[i] = grads_host[first + i];
-            t.param[i] = params_host[first + i];
-        }
-        a.pieces = cfg->pieces_dev + piece;
-        a.first_tensor = (uint32_t)first;
-        if (cfg->state_bits == 32)
-            hipLaunchKernelGGL(k_adam<32>, dim3(n), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, a);
-        else
-            hipLaunchKernelGGL(k_adam<8>, dim3(n), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, a);
-        AZ_HIP(hipGetLastError());
+        n_partials += sums;
         return AZ_OK;
     });
+    float* norm = cfg->norm_dev;
+    for (int32_t g = 0, begin = 0; g < n_groups && rc == AZ_OK; begin = groups[g++].end) {
+        AdamParams a;
+        a.beta1 = (float)groups[g].beta1;
+        a.one_beta1 = (float)(1.0 - groups[g].beta1);
+        a.beta2 = (float)groups[g].beta2;
+        a.one_beta2 = (float)(1.0 - groups[g].beta2);
+        a.eps = (float)groups[g].eps;
+        a.decoupled = groups[g].decoupled != 0;
+        a.decay = a.decoupled ? (float)(1.0 - groups[g].lr * groups[g].weight_decay) : (float)groups[g].weight_decay;
+        a.factors = factors;
+        a.max_norm = clip ? cfg->max_norm : 0.0;
+        a.partials = partials;
+        a.n_partials = n_partials;
+        a.m = cfg->m_dev;
+        a.v = cfg->v_dev;
+        a.m_scale = cfg->m_scale_dev;
+        a.v_scale = cfg->v_scale_dev;
+        rc = for_ranges(begin, groups[g].end, sizes_host, [&](int32_t first, int32_t k, int64_t piece, uint32_t n) -> int {
+            TensorTable t;
+            for (int32_t i = 0; i < k; ++i) {
+                t.grad[i] = grads_host[first + i];
+                t.param[i] = params_host[first + i];
+            }
+            a.pieces = cfg->pieces_dev + piece;
+            a.first_tensor = (uint32_t)first;
+            a.norm = norm;
+            norm = nullptr;                               // written once
+            if (cfg->state_bits == 32)
+                hipLaunchKernelGGL(k_adam<32>, dim3(n), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, a);
+            else
+                hipLaunchKernelGGL(k_adam<8>, dim3(n), dim3(OPT_THREADS), 0, (hipStream_t)stream, t, a);
+            AZ_HIP(hipGetLastError());
+            return AZ_OK;
+        });
+    }
+    return rc;
 }

@@ -36,7 +36,7 @@ struct Entries {
     decltype(&az_policy_value_loss_forward) loss_forward;
     decltype(&az_policy_value_loss_backward) loss_backward;
     decltype(&az_adam_plan) adam_plan;
-    decltype(&az_grad_sumsq) grad_sumsq;
+    decltype(&az_adam_scratch) adam_scratch;
     decltype(&az_adam_step) adam_step;
 } lib;
 
@@ -336,12 +336,6 @@ bool same_places(const Tensor& a, at::IntArrayRef strides) {
     return true;
 }
 
-struct AdamGroup {
-    int64_t begin, end;
-    double lr, beta1, beta2, eps, weight_decay;
-    bool decoupled;
-};
-
 class AdamPlan {
   public:
     // Lays out the moments of the parameters; attach() gives it the buffers.
@@ -374,7 +368,7 @@ class AdamPlan {
     }
 
     // One step over every parameter that has a gradient.
-    void step(const std::vector<AdamGroup>& groups, double max_norm) {
+    void step(const std::vector<az_adam_group>& groups, double max_norm) {
         const at::NoGradGuard no_grad;
         const c10::DeviceGuard guard(step_.device());
         void* stream = stream_of(step_);
@@ -406,40 +400,24 @@ class AdamPlan {
             any = true;
         }
         if (!any) return;
-        const Tensor scratch = floats(4 + 3 * (int64_t)count, step_);
-        const auto pieces = (const az_adam_piece*)pieces_.data_ptr();
-        Tensor sums;
-        if (max_norm > 0) {
-            sums = at::empty({n_pieces_}, step_.options().dtype(at::kDouble));
-            check(lib.grad_sumsq((int32_t)count, grads.data(), sizes_.data(), pieces, ptr<double>(sums), n_pieces_, stream));
-        }
-        for (const AdamGroup& g : groups) {
-            az_adam_config c{};
-            c.lr = g.lr;
-            c.beta1 = g.beta1;
-            c.beta2 = g.beta2;
-            c.eps = g.eps;
-            c.weight_decay = g.weight_decay;
-            c.decoupled = g.decoupled;
-            c.max_norm = max_norm > 0 ? max_norm : 0.0;
-            c.state_bits = bits_;
-            c.seed = seed_;
-            c.n_partials = sums.defined() ? n_pieces_ : 0;
-            c.pieces_dev = pieces;
-            c.m_dev = m_.data_ptr();
-            c.v_dev = v_.data_ptr();
-            c.m_scale_dev = ptr<float>(m_scale_);
-            c.v_scale_dev = ptr<float>(v_scale_);
-            c.steps_dev = ptr<float>(step_);
-            c.partials_dev = ptr<double>(sums);
-            c.norm_dev = sums.defined() ? ptr<float>(norm_) : nullptr;
-            c.scratch_dev = ptr<float>(scratch);
-            check(lib.adam_step(&c, (int32_t)count, (int32_t)g.begin, (int32_t)g.end, params.data(), grads.data(), sizes_.data(), stream));
-        }
+        const Tensor scratch = bytes(lib.adam_scratch((int32_t)count), step_);
+        az_adam_config c{};
+        c.max_norm = max_norm > 0 ? max_norm : 0.0;
+        c.state_bits = bits_;
+        c.seed = seed_;
+        c.pieces_dev = (const az_adam_piece*)pieces_.data_ptr();
+        c.m_dev = m_.data_ptr();
+        c.v_dev = v_.data_ptr();
+        c.m_scale_dev = ptr<float>(m_scale_);
+        c.v_scale_dev = ptr<float>(v_scale_);
+        c.steps_dev = ptr<float>(step_);
+        c.norm_dev = ptr<float>(norm_);
+        c.scratch_dev = scratch.data_ptr();
+        check(lib.adam_step(&c, (int32_t)groups.size(), groups.data(), (int32_t)count, params.data(), grads.data(), sizes_.data(), stream));
         // written behind torch's back: whoever watches version counters has to see it
         for (size_t i = 0; i < count; ++i)
             if (grads[i]) params_[i].unsafeGetTensorImpl()->bump_version();
-        for (const Tensor* t : {&step_, &m_, &v_, &m_scale_, &v_scale_})
+        for (const Tensor* t : {&step_, &m_, &v_, &m_scale_, &v_scale_, &norm_})
             if (t->defined()) t->unsafeGetTensorImpl()->bump_version();
     }
 
@@ -471,7 +449,7 @@ PYBIND11_MODULE(_azops, m) {
         set(lib.loss_forward, a, "az_policy_value_loss_forward");
         set(lib.loss_backward, a, "az_policy_value_loss_backward");
         set(lib.adam_plan, a, "az_adam_plan");
-        set(lib.grad_sumsq, a, "az_grad_sumsq");
+        set(lib.adam_scratch, a, "az_adam_scratch");
         set(lib.adam_step, a, "az_adam_step");
         az_error = error.release().ptr();
     });
@@ -481,10 +459,10 @@ PYBIND11_MODULE(_azops, m) {
         .def(py::init<std::vector<Tensor>>())
         .def("offsets", &AdamPlan::offsets)
         .def("attach", &AdamPlan::attach)
-        .def("step", [](AdamPlan& self, const std::vector<std::tuple<int64_t, int64_t, double, double, double, double, double, bool>>& groups,
-                        double max_norm) {
-            std::vector<AdamGroup> g;
-            for (const auto& t : groups) g.push_back(std::apply([](auto... v) { return AdamGroup{v...}; }, t));
+        .def("step", [](AdamPlan& self, const std::vector<std::tuple<double, double, double, double, double, bool, int>>& groups,
+                        double max_norm) {          // (lr, beta1, beta2, eps, weight_decay, decoupled, end)
+            std::vector<az_adam_group> g;
+            for (const auto& t : groups) g.push_back(std::apply([](auto... v) { return az_adam_group{v...}; }, t));
             torch::wrap_pybind_function([&] { self.step(g, max_norm); })();
         });
 }

@@ -40,7 +40,7 @@ def _decode(codes, scale):
 
 class FusedAdam(torch.optim.Optimizer):
     """torch.optim.Adam(params, lr, betas, eps, weight_decay), or AdamW with decoupled=True, for float32 parameters on
-    one GPU, as two to four launches for all of them.
+    one GPU, as two launches for all of them (per 240 tensors and parameter group; up to 48 groups).
 
     step(max_norm=x) also clips by the norm over the gradients of all parameters: they are scaled by
     min(1, x / (norm + 1e-6)) on the way into the update (the .grad tensors keep their values; torch's
@@ -77,6 +77,8 @@ class FusedAdam(torch.optim.Optimizer):
     def _build(self):
         params = [p for g in self.param_groups for p in g["params"]]
         device = params[0].device
+        if len(self.param_groups) > _lib.OPTIM_GROUPS:
+            raise ValueError(f"FusedAdam takes up to {_lib.OPTIM_GROUPS} parameter groups, got {len(self.param_groups)}")
         if device.type != "cuda":
             raise ValueError(f"FusedAdam needs parameters on a GPU, got one on {device}")
         for p in params:
@@ -100,12 +102,10 @@ class FusedAdam(torch.optim.Optimizer):
                 self._flat[name] = torch.zeros(total, dtype=torch.uint8, **shape).view(torch.float8_e4m3fn)
                 self._flat[name + "_scale"] = torch.full((total // _PAD,), 2.0 ** -108, **shape)
         self.grad_norm = torch.zeros((), **shape)
-        self._groups = []
-        at = 0
+        self._ends, end = [], 0
         for g in self.param_groups:
-            k = len(g["params"])
-            self._groups.append((at, at + k))
-            at += k
+            end += len(g["params"])
+            self._ends.append(end)
         m, v = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_rms")
         self._plan.attach(self.state_bits, self.seed & 0xFFFFFFFF, self._step, self._flat[m], self._flat[v],
                           self._flat.get(m + "_scale"), self._flat.get(v + "_scale"), self.grad_norm)
@@ -180,6 +180,6 @@ class FusedAdam(torch.optim.Optimizer):
                 loss = closure()
         if max_norm is not None and not max_norm > 0:
             raise ValueError(f"max_norm must be positive, got {max_norm}")
-        self._plan.step([(*at, g["lr"], *g["betas"], g["eps"], g["weight_decay"], g["decoupled_weight_decay"])
-                         for at, g in zip(self._groups, self.param_groups)], max_norm or 0.0)
+        self._plan.step([(g["lr"], *g["betas"], g["eps"], g["weight_decay"], g["decoupled_weight_decay"], end)
+                         for end, g in zip(self._ends, self.param_groups)], max_norm or 0.0)
         return loss

@@ -400,14 +400,15 @@ int az_policy_value_loss_backward(const az_loss_args* args, void* stream);
  * elements of a tensor; either array may be null.  It returns the number of pieces or a negative
  * code.  The caller keeps a copy of the pieces in device memory (pieces_dev): they are read by
  * every call on the same sizes.
- * az_grad_sumsq writes one partial sum of squares per piece of all `count` tensors.
- * az_adam_step steps tensors [begin, end) of the `count`: its step counter steps_dev[i] (float32) is
- * incremented where there is a gradient.  state_bits 32: m and v as float32.  state_bits 8: m and
- * sqrt(v) as e4m3 codes, one power of two per AZ_OPTIM_PAD of them in m_scale_dev / v_scale_dev,
- * rounded at random (a hash of seed, step counter and place).
+ * az_adam_step makes one step: the step counter steps_dev[i] (float32) of every tensor with a
+ * gradient is incremented.  Tensors lie in groups, one behind the other, each with rates of its own.
+ * state_bits 32: m and v as float32.  state_bits 8: m and sqrt(v) as e4m3 codes, one power of two
+ * per AZ_OPTIM_PAD of them in m_scale_dev / v_scale_dev, rounded at random (a hash of seed, step
+ * counter and place).
  * max_norm > 0: gradients are scaled by min(1, max_norm / (norm + 1e-6)) on the way in, norm being
- * the root of the sum of partials_dev; the gradients themselves are not written.
- * scratch_dev: 4 + 3 * count floats. */
+ * that of all gradients (summed in 64 bits); the gradients themselves are not written.
+ * scratch_dev: az_adam_scratch(count) bytes, 16-byte aligned, free again after the call's work. */
+#define AZ_OPTIM_GROUPS 48
 #define AZ_OPTIM_CHUNK 4096
 #define AZ_OPTIM_PAD 256
 typedef struct {
@@ -416,22 +417,24 @@ typedef struct {
     uint32_t n;                  /* elements of the piece */
 } az_adam_piece;
 typedef struct {
-    double lr, beta1, beta2, eps, weight_decay, max_norm;
-    int32_t decoupled, state_bits;
+    double lr, beta1, beta2, eps, weight_decay;
+    int32_t decoupled;
+    int32_t end;                 /* first tensor after the group; the last group ends with the tensors */
+} az_adam_group;
+typedef struct {
+    double max_norm;
     uint64_t seed;
-    int64_t n_partials;
+    int32_t state_bits;
     const az_adam_piece* pieces_dev;
     void *m_dev, *v_dev;         /* 16-byte aligned */
     float *m_scale_dev, *v_scale_dev, *steps_dev;
-    const double* partials_dev;
-    float* norm_dev;             /* receives the norm; may be null */
-    float* scratch_dev;
+    float* norm_dev;             /* receives the norm where max_norm > 0; may be null */
+    void* scratch_dev;
 } az_adam_config;
 int64_t az_adam_plan(int32_t count, const int64_t* sizes_host, int64_t* offsets_host, az_adam_piece* pieces_host);
-int az_grad_sumsq(int32_t count, const uint64_t* grads_host, const int64_t* sizes_host, const az_adam_piece* pieces_dev,
-                  double* partials_dev, int64_t n_partials, void* stream);
-int az_adam_step(const az_adam_config* cfg, int32_t count, int32_t begin, int32_t end, const uint64_t* params_host,
-                 const uint64_t* grads_host, const int64_t* sizes_host, void* stream);
+int64_t az_adam_scratch(int32_t count);
+int az_adam_step(const az_adam_config* cfg, int32_t n_groups, const az_adam_group* groups_host, int32_t count,
+                 const uint64_t* params_host, const uint64_t* grads_host, const int64_t* sizes_host, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,11 +15,12 @@ def test_structures_match_the_header(tmp_path):
     import subprocess
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     src = tmp_path / "sizes.c"
-    src.write_text('#include <stdio.h>\n#include "azamd.h"\nint main(void) { printf("%zu %zu %zu %d %d", sizeof(az_norm_args), '
-                   'sizeof(az_loss_args), sizeof(az_adam_config), AZ_OPTIM_CHUNK, AZ_OPTIM_PAD); return 0; }\n')
+    src.write_text('#include <stdio.h>\n#include "azamd.h"\nint main(void) { printf("%zu %zu %zu %zu %d %d %d", sizeof(az_norm_args), '
+                   'sizeof(az_loss_args), sizeof(az_adam_config), sizeof(az_adam_group), AZ_OPTIM_CHUNK, AZ_OPTIM_PAD, AZ_OPTIM_GROUPS); return 0; }\n')
     subprocess.check_call(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "sizes")])
     got = [int(v) for v in subprocess.check_output([str(tmp_path / "sizes")]).split()]
-    assert got == [C.sizeof(_lib.NormArgs), C.sizeof(_lib.LossArgs), C.sizeof(_lib.AdamConfig), _lib.OPTIM_CHUNK, _lib.OPTIM_PAD]
+    assert got == [C.sizeof(_lib.NormArgs), C.sizeof(_lib.LossArgs), C.sizeof(_lib.AdamConfig), C.sizeof(_lib.AdamGroup), _lib.OPTIM_CHUNK, _lib.OPTIM_PAD,
+                   _lib.OPTIM_GROUPS]
 
 
 def test_host_tensors_are_refused():
@@ -85,34 +86,39 @@ def test_c_entry_of_the_loss_checks_its_arguments(kw, match):
 
 
 def _adam(**kw):
-    a = _lib.AdamConfig(1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, 0, 32, 0, 0, 64, 64, 64, None, None, 64, None, None, 64)
+    a = _lib.AdamConfig(0.0, 0, 32, 64, 64, 64, None, None, 64, None, 64)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
 
 
-@pytest.mark.parametrize("kw, size, begin, end, match", [
-    ({"state_bits": 16}, 10, 0, 1, "moments in 16 bits"), ({"m": None}, 10, 0, 1, "null state"), ({"pieces": None}, 10, 0, 1, "null state"),
-    ({"state_bits": 8}, 10, 0, 1, "scales"), ({"m": 68}, 10, 0, 1, "aligned"), ({}, -1, 0, 1, "-1 elements"), ({}, 1 << 39, 0, 1, "elements"),
-    ({}, 10, 0, 2, "tensors 0 to 2 of 1"), ({}, 10, -1, 1, "tensors -1 to 1"), ({"max_norm": 1.0, "n_partials": 1}, 10, 0, 1, "partial sums"),
-    ({"max_norm": 1.0, "n_partials": 2, "partials": 64}, 10, 0, 1, "2 partial sums, 1 wanted"),
+def _groups(*ends):
+    return (_lib.AdamGroup * len(ends))(*(_lib.AdamGroup(1e-3, 0.9, 0.999, 1e-8, 0.0, 0, e) for e in ends))
+
+
+@pytest.mark.parametrize("kw, size, ends, match", [
+    ({"state_bits": 16}, 10, [1], "moments in 16 bits"), ({"m": None}, 10, [1], "null state"), ({"pieces": None}, 10, [1], "null state"),
+    ({"scratch": None}, 10, [1], "null state"), ({"state_bits": 8}, 10, [1], "scales"), ({"m": 68}, 10, [1], "aligned"),
+    ({"scratch": 72}, 10, [1], "aligned"), ({}, -1, [1], "-1 elements"), ({}, 1 << 39, [1], "elements"), ({}, 10, [2], "group 0 ends at 2 of 1"),
+    ({}, 10, [0], "group 0 ends at 0 of 1"), ({}, 10, [1, 0], "group 1 ends at 0"), ({}, 10, [-1, 1], "group 0 ends at -1"),
 ])
-def test_c_entry_of_the_step_checks_its_arguments(kw, size, begin, end, match):
+def test_c_entry_of_the_step_checks_its_arguments(kw, size, ends, match):
     L = _lib.lib()
     p, s = (C.c_uint64 * 1)(64), (C.c_int64 * 1)(size)
-    assert L.az_adam_step(C.byref(_adam(**kw)), 1, begin, end, p, p, s, None) == -1
+    assert L.az_adam_step(C.byref(_adam(**kw)), len(ends), _groups(*ends), 1, p, p, s, None) == -1
     assert match.encode() in L.az_last_error()
 
 
-def test_c_entries_refuse_misaligned_tensors_and_short_partials():
+def test_c_entry_of_the_step_refuses_misaligned_tensors_and_too_many_groups():
     L = _lib.lib()
     good, odd, s = (C.c_uint64 * 1)(64), (C.c_uint64 * 1)(66), (C.c_int64 * 1)(5000)
-    assert L.az_grad_sumsq(1, good, s, 64, 64, 1, None) == -1 and b"2 partial sums" in L.az_last_error()
-    assert L.az_grad_sumsq(1, good, s, None, 64, 2, None) == -1
-    assert L.az_grad_sumsq(1, odd, s, 64, 64, 2, None) == -1 and b"aligned" in L.az_last_error()
-    assert L.az_adam_step(C.byref(_adam()), 1, 0, 1, odd, good, s, None) == -1 and b"aligned" in L.az_last_error()
-    assert L.az_adam_step(C.byref(_adam()), 0, 0, 0, None, None, None, None) == 0          # nothing to do is fine
-    assert L.az_grad_sumsq(0, None, None, None, None, 0, None) == 0
+    for p, g in ((odd, good), (good, odd)):
+        assert L.az_adam_step(C.byref(_adam()), 1, _groups(1), 1, p, g, s, None) == -1 and b"aligned to 4" in L.az_last_error()
+    many = _groups(*([0] * _lib.OPTIM_GROUPS + [1]))
+    assert L.az_adam_step(C.byref(_adam()), len(many), many, 1, good, good, s, None) == -1 and b"49 groups" in L.az_last_error()
+    assert L.az_adam_step(C.byref(_adam()), 0, _groups(1), 1, good, good, s, None) == -1
+    assert L.az_adam_step(C.byref(_adam()), 1, _groups(0), 0, None, None, None, None) == 0          # nothing to do is fine
+    assert L.az_adam_scratch(0) == 0 and L.az_adam_scratch(241) == 2 * 8192 + 241 * 12 and L.az_adam_scratch(-1) == -1
 
 
 def test_plan_of_the_moments():
