@@ -913,13 +913,12 @@ __global__ __launch_bounds__(GATE_THREADS) void k_gate_backward(const NormParams
     });
 }
 
-// Gradients of the gate's weights: sums over the boards of outer products, as 32 x 32 tiles.  A workgroup takes one tile and
-// one of `splits` ranges of boards, each of its wavefronts every eighth board, a lane 4 x 4 of the tile, four boards' loads
-// in flight.  The bias is the sum of the left factor.  The partial tiles go to the workspace; the last pass's first
-// workgroups add them in order, beside its own work.
-// (One workgroup per tile over all boards, one board in flight, took 62 us at 1024 x 128 and 230 us at 4096 x 256: four times
-// the pass over the activations that follows.)
-constexpr int TILE = 32, TILE_WAVES = CHANNELS * LINES / 64, TILE_BOARDS = 4, TILE_OUT = TILE * TILE + TILE;
+// Gradients of the gate's weights: sums over the boards of outer products, as 32 x 32 tiles on the matrix unit (in
+// float32: two boards an instruction, a lane loads one value of each factor).  A workgroup takes one tile and one of
+// `splits` ranges of boards, its wavefronts two boards in turn, the loads of 16 boards in flight.  The bias is the sum of
+// the left factor.  The partial tiles go to the workspace; the last pass's first workgroups add them in order, beside
+// its own work.
+constexpr int TILE = 32, TILE_WAVES = CHANNELS * LINES / 64, TILE_AHEAD = 8, TILE_OUT = TILE * TILE + TILE;
 
 struct TileShape {
     int m, k, across, tiles;                                         // [m][k] in `tiles` tiles, `across` to a row
@@ -949,44 +948,35 @@ __device__ inline void weight_tile(const NormParams& p, int job) {
     const TileShape t = second ? fc2 : fc1;
     if (!second) tile -= fc2.tiles;
     const int i0 = tile / t.across * TILE, j0 = tile % t.across * TILE;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = i0 + lane / 8 * 4, lj = j0 + lane % 8 * 4;
-    const float *left = second ? p.de : p.dh, *right = second ? p.h : p.board_mean;
-    f32x4 acc[4], bias, scale, shift;                                // fc1's right factor: q = mean * scale + shift
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        acc[j] = 0.f;
-        bias[j] = 0.f;
-        const int c = lj + j < t.k ? lj + j : 0;
-        scale[j] = second ? 1.f : p.weight[c] * p.inv[c];
-        shift[j] = second ? 0.f : p.bias[c] - scale[j] * p.mean[c];
-    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & 31, second_board = lane >> 5;
+    // (a lane past the end of a factor reads its last value; what comes of it is not joined)
+    const int i = i0 + at < t.m ? i0 + at : t.m - 1, j = j0 + at < t.k ? j0 + at : t.k - 1;
+    const float *left = (second ? p.de : p.dh) + i, *right = (second ? p.h : p.board_mean) + j;
+    // fc1's right factor: q = mean * scale + shift
+    const float scale = second ? 1.f : p.weight[j] * p.inv[j], shift = second ? 0.f : p.bias[j] - scale * p.mean[j];
+    typedef float f32x16 __attribute__((ext_vector_type(16)));
+    f32x16 acc = 0.f;
+    float bias = 0.f;
     const int64_t from = p.n * split / splits, to = p.n * (split + 1) / splits;
-    const auto sum_boards = [&](auto fours) {
-        constexpr bool FOURS = decltype(fours)::value;
-        // FOURS: a lane past the end of a factor reads its last four; what comes of them is not joined
-        const int ai = FOURS && li > t.m - 4 ? t.m - 4 : li, bj = FOURS && lj > t.k - 4 ? t.k - 4 : lj;
-        for (int64_t n = from + wave; n < to; n += TILE_WAVES * TILE_BOARDS) {
-            f32x4 a[TILE_BOARDS], b[TILE_BOARDS];
+    for (int64_t n = from + 2 * wave; n < to; n += 2 * TILE_WAVES * TILE_AHEAD) {
+        float a[TILE_AHEAD], b[TILE_AHEAD];
 #pragma unroll
-            for (int u = 0; u < TILE_BOARDS; ++u) {
-                const int64_t nu = n + u * TILE_WAVES < to ? n + u * TILE_WAVES : n;
-                a[u] = four_weights<FOURS>(left + nu * t.m + ai, t.m - ai);
-                b[u] = four_weights<FOURS>(right + nu * t.k + bj, t.k - bj);
-            }
-#pragma unroll
-            for (int u = 0; u < TILE_BOARDS; ++u) {
-                const f32x4 w = a[u] * (n + u * TILE_WAVES < to ? 1.f : 0.f), q = b[u] * scale + shift;
-                bias += w;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] += w[i] * q;
-            }
+        for (int u = 0; u < TILE_AHEAD; ++u) {
+            const int64_t nu = n + 2 * TILE_WAVES * u + second_board, in = nu < to ? nu : from;
+            a[u] = left[in * t.m];
+            b[u] = right[in * t.k];
         }
-    };
-    if (t.m % 4 == 0 && t.k % 4 == 0) sum_boards(std::true_type());
-    else sum_boards(std::false_type());
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *(f32x4*)&lds[wave][(lane / 8 * 4 + i) * TILE + lane % 8 * 4] = acc[i];
-    if (lane % 8 == 0) *(f32x4*)&lds[wave][TILE * TILE + lane / 8 * 4] = bias;
+        for (int u = 0; u < TILE_AHEAD; ++u) {
+            const float w = n + 2 * TILE_WAVES * u + second_board < to ? a[u] : 0.f;
+            bias += w;
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(w, b[u] * scale + shift, acc, 0, 0, 0);
+        }
+    }
+    bias += __shfl_xor(bias, 32);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) lds[wave][(8 * (r / 4) + 4 * second_board + r % 4) * TILE + at] = acc[r];
+    if (lane < TILE) lds[wave][TILE * TILE + lane] = bias;
     __syncthreads();
     float* out = p.partial + ((size_t)split * tiles + job % tiles) * TILE_OUT;
     for (int o = threadIdx.x; o < TILE_OUT; o += TILE_WAVES * 64) {
