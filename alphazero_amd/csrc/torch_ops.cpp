@@ -363,7 +363,6 @@ class AdamPlan {
         for (const Tensor& p : params_) {
             sizes_.push_back(p.numel());
             strides_.push_back(p.strides().vec());
-            places_.push_back(nullptr);
         }
         const int32_t count = (int32_t)params_.size();
         const int64_t n = lib.adam_plan(count, sizes_.data(), offsets_.data(), nullptr);
@@ -398,13 +397,10 @@ class AdamPlan {
         bool any = false;
         for (size_t i = 0; i < count; ++i) {
             const Tensor& p = params_[i];
-            if (p.data_ptr() != places_[i]) {        // new here, or moved since: it must still fit its moments
-                TORCH_CHECK_VALUE(p.scalar_type() == at::kFloat && p.device() == step_.device() && p.numel() == sizes_[i], "a parameter became ",
-                                  p.scalar_type(), " ", p.sizes(), " on ", p.device(), " after FusedAdam was built");
-                TORCH_CHECK_VALUE(p.dim() == (int64_t)strides_[i].size() && same_places(p, strides_[i]),
-                                  "a parameter's strides changed after FusedAdam was built: its moments are in the old order");
-                places_[i] = p.data_ptr();
-            }
+            TORCH_CHECK_VALUE(p.scalar_type() == at::kFloat && p.device() == step_.device() && p.numel() == sizes_[i], "a parameter became ",
+                              p.scalar_type(), " ", p.sizes(), " on ", p.device(), " after FusedAdam was built");
+            TORCH_CHECK_VALUE(p.dim() == (int64_t)strides_[i].size() && same_places(p, strides_[i]),
+                              "a parameter's strides changed after FusedAdam was built: its moments are in the old order");
             const Tensor& held_grad = p.grad();
             if (!held_grad.defined() || sizes_[i] == 0) continue;
             Tensor g = held_grad;
@@ -445,7 +441,6 @@ class AdamPlan {
     std::vector<Tensor> params_;
     std::vector<int64_t> sizes_, offsets_;
     std::vector<std::vector<int64_t>> strides_;
-    std::vector<void*> places_;
     int64_t n_pieces_ = 0;
     Tensor pieces_;
     int bits_ = 32;

@@ -931,9 +931,9 @@ __host__ __device__ inline TileShape tile_shape(int m, int k) {
 
 __host__ __device__ inline int weight_tiles(const NormParams& p) { return tile_shape(2 * p.c, p.hidden).tiles + tile_shape(p.hidden, p.c).tiles; }
 
-// Ranges of at least 64 boards (two rounds of a wavefront), and no more workgroups than twice the compute units: every
-// range is a partial tile more to join.  (At 4096 x 256, 24 tiles: 64 ranges 19.5 us and 7 us more in the pass that joins
-// them, 32 ranges 17.3, 16 ranges 15.8; at 1024 x 128, 12 tiles: 16 ranges 5.0 us, 8 ranges 6.3, 4 ranges 8.4.)
+// Ranges of at least 64 boards, and no more workgroups than twice the compute units: every range is a partial tile more
+// to join.  (At 4096 x 256, 24 tiles: 21 ranges 12.9 us, 10 ranges 16.7; 64 ranges would cost the pass that joins them
+// 7 us more.  At 1024 x 128, 12 tiles: 16 ranges 4.7 us, 8 ranges 5.1.)
 __host__ __device__ inline int weight_splits(const NormParams& p) {
     const int64_t most = (p.n + 63) / 64, enough = 512 / weight_tiles(p);
     return (int)(enough < 1 ? 1 : most < enough ? most : enough);
@@ -1026,7 +1026,8 @@ static void with_lanes(const NormParams& p, F&& f) {
     typedef std::integral_constant<Fit, ONE> One;
     if (p.hw == 8 * V) f(std::integral_constant<int, 8>(), Exact());
     else if (p.hw == 16 * V) f(std::integral_constant<int, 16>(), Exact());
-    else if (p.hw < V || p.nvec > 64) f(std::integral_constant<int, 16>(), std::integral_constant<Fit, LOOP>());
+    else if (p.nvec > 64) f(std::integral_constant<int, 64>(), std::integral_constant<Fit, LOOP>());
+    else if (p.hw < V) f(std::integral_constant<int, 8>(), std::integral_constant<Fit, LOOP>());
     else if (p.nvec <= 8) f(std::integral_constant<int, 8>(), One());
     else if (p.nvec <= 16) f(std::integral_constant<int, 16>(), One());
     else if (p.nvec <= 32) f(std::integral_constant<int, 32>(), One());

@@ -149,6 +149,12 @@ class FusedAdam(torch.optim.Optimizer):
             if g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("FusedAdam has no amsgrad and no maximize")
         before = self.param_groups
+        if [len(g["params"]) for g in state_dict["param_groups"]] == [len(g["params"]) for g in before]:       # else torch refuses it
+            keys = [k for g in state_dict["param_groups"] for k in g["params"]]
+            for key, p in zip(keys, self._params):
+                for name, v in state_dict["state"].get(key, {}).items():
+                    if name in ("exp_avg", "exp_avg_sq") and v.shape != p.shape:
+                        raise ValueError(f"{name} of a parameter of shape {tuple(p.shape)} has shape {tuple(v.shape)}")
         super().load_state_dict(state_dict)
         for g, old in zip(self.param_groups, before):
             g.setdefault("decoupled_weight_decay", old["decoupled_weight_decay"])

@@ -96,6 +96,10 @@ def test_fused_learn_from_graphs(tmp_path, bits):
     assert np.isfinite(stats["loss"]) and step.steps_seen == 12
     assert any(not torch.equal(x, y) for x, y in zip(before, graphed.model.parameters()))
     assert step.lr < 1e-3 and float(graphed.optimizer.flat_state()["step"].max()) == 12.0
+    # another batch size: four full batches of 40 (three eager, one captured) and a ragged one of 32 beside the graphs
+    assert np.isfinite(learn(graphed, batch_size=40)["loss"]) and graphed._graphed[40].steps_seen == 4
+    assert np.isfinite(learn(graphed)["loss"]) and step.steps_seen == 18
+    assert float(graphed.optimizer.flat_state()["step"].min()) == 12.0 + 5 + 6
 
 
 @pytest.mark.parametrize("layout", [torch.contiguous_format, torch.channels_last], ids=["nchw", "nhwc"])

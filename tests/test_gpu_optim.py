@@ -384,3 +384,97 @@ def test_captured_steps_equal_eager_ones():
             assert torch.equal(eager.grad_norm, graphed.grad_norm)
             for name, x in eager.flat_state().items():
                 assert torch.equal(x.view(torch.uint8), graphed.flat_state()[name].view(torch.uint8)), name
+
+
+def test_a_parameter_that_changed_its_shape_in_place_is_refused():
+    """The same address with fewer elements or another order: the moments no longer fit, and nothing is read or written."""
+    from alphazero_amd.optim import FusedAdam
+    for change in (lambda t: t[:5], lambda t: t.t()):
+        p = torch.ones(8, 8, device="cuda", requires_grad=True)
+        p.grad = torch.ones(8, 8, device="cuda")
+        opt = FusedAdam([p])
+        opt.step()
+        p.grad = None
+        p.data = change(p.data)
+        p.grad = torch.ones_like(p)
+        held = p.detach().clone()
+        with pytest.raises(ValueError, match="after FusedAdam was built"):
+            opt.step()
+        assert torch.equal(p.detach(), held)
+
+
+def test_a_checkpoint_of_another_shape_is_refused_whole():
+    from alphazero_amd.optim import FusedAdam
+    a, b = tensors([(4, 6), (5,)]), tensors([(4, 6), (7,)])
+    one, two = FusedAdam(a), FusedAdam(b)
+    one.step(), two.step()
+    kept = {k: v.clone() for k, v in one.flat_state().items()}
+    with pytest.raises(ValueError, match="has shape"):
+        one.load_state_dict(two.state_dict())
+    with pytest.raises(ValueError):
+        one.load_state_dict(FusedAdam(tensors([(4, 6)])).state_dict())
+    one.step()
+    assert all(float(v.min()) == 2.0 for k, v in one.flat_state().items() if k == "step") and kept["step"].tolist() == [1.0, 1.0]
+
+
+def test_groups_with_rates_of_their_own_are_one_call():
+    """Three groups with other betas, decay and rates, clipped by one norm: each as an optimiser of its own that is given the
+    clipped gradients."""
+    from alphazero_amd.optim import FusedAdam
+    shapes = [(300,), (40, 7), (9000,), (3,)]
+    params, alone = tensors(shapes, 12), tensors(shapes, 12)
+    opts = [dict(lr=1e-2, betas=(0.8, 0.9)), dict(lr=1e-3, weight_decay=0.1), dict(lr=3e-4, weight_decay=0.2, decoupled=True, eps=1e-4)]
+    split = [params[:1], params[1:3], params[3:]]
+    together = FusedAdam([{"params": p, **{"decoupled_weight_decay" if k == "decoupled" else k: v for k, v in o.items()}} for p, o in zip(split, opts)])
+    together.step(max_norm=1e-2)
+    norm = math.sqrt(sum(float(p.grad.double().square().sum()) for p in alone))
+    assert abs(float(together.grad_norm) - norm) <= 2 * U * norm
+    c = torch.tensor(1e-2 / (norm + 1e-6), dtype=torch.float32, device="cuda")
+    for p in alone:
+        p.grad *= c
+    for p, o in zip([alone[:1], alone[1:3], alone[3:]], opts):
+        FusedAdam(p, **o).step()
+    assert all(torch.equal(p.detach(), q.detach()) for p, q in zip(params, alone))
+
+
+def test_two_optimisers_and_gradients_that_are_shared():
+    """One gradient tensor for two parameters, and two optimisers whose steps follow one another on two streams."""
+    from alphazero_amd.optim import FusedAdam
+    p, q = tensors([(500,), (500,)], 13)
+    q.grad = p.grad
+    want = [t.detach().clone().requires_grad_(True) for t in (p, q)]
+    for t in want:
+        t.grad = p.grad.clone()
+    a, b = FusedAdam([p], seed=1), FusedAdam([q], seed=1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    a.step(max_norm=1.0)
+    with torch.cuda.stream(side):
+        b.step(max_norm=1.0)
+    torch.cuda.current_stream().wait_stream(side)
+    for t, o in zip(want, (FusedAdam(want[:1]), FusedAdam(want[1:]))):
+        o.step(max_norm=1.0)
+    assert torch.equal(p.detach(), want[0].detach()) and torch.equal(q.detach(), want[1].detach())
+
+
+def test_closure_scheduler_and_scaler():
+    from alphazero_amd.optim import FusedAdam
+    p = torch.ones(100, device="cuda", requires_grad=True)
+    opt = FusedAdam([p], lr=0.1)
+
+    def closure():
+        opt.zero_grad()
+        loss = (p * p).sum()
+        loss.backward()
+        return loss
+    assert float(opt.step(closure)) == 100.0 and abs(float(p.detach()[0]) - 0.9) < 1e-6
+    scaler = torch.amp.GradScaler("cuda", init_scale=1024.0)
+    opt.zero_grad()
+    scaler.scale((p * p).sum()).backward()
+    scaler.step(opt)
+    scaler.update()
+    before = p.detach().clone()
+    opt.zero_grad()
+    scaler.scale((p * p).sum() * math.inf).backward()
+    scaler.step(opt)                                                   # infinite gradients: the step is left out
+    assert torch.equal(p.detach(), before) and float(opt.flat_state()["step"]) == 2.0

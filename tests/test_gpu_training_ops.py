@@ -19,6 +19,7 @@ EPS = 1e-5
 
 def close(got, want, magnitude, k):
     """|got - want| <= k 2^-24 magnitude + the rounding to got's type."""
+    got = got.detach()
     assert got.shape == want.shape and bool(torch.isfinite(got).all())
     info = torch.finfo(got.dtype)
     # below the type's normal range a step no longer shrinks with the value
@@ -313,6 +314,61 @@ def test_norm_refusals():
     g, = torch.autograd.grad(ops.norm_act(leaf, w, b, *s).sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("layout", [torch.contiguous_format, torch.channels_last], ids=["nchw", "nhwc"])
+def test_norms_of_more_than_2_to_the_31_values(layout):
+    """Offsets past 32 bits: with running statistics every board stands for itself, so the first and the last boards of a
+    tensor of 2.3e9 values have to be what they are alone, forward and backward, bit for bit."""
+    from alphazero_amd import ops
+    n, c, h = 4300, 1024, 23
+    x = torch.empty((n, c, h, h), dtype=torch.bfloat16, device="cuda", memory_format=layout)
+    gen = torch.Generator("cuda").manual_seed(3)
+    ends = [slice(0, 2), slice(n - 2, n)]
+    x.zero_()
+    for e in ends:
+        x[e] = torch.randn((2, c, h, h), device="cuda", generator=gen).to(torch.bfloat16)
+    t = norm_inputs(2, c, 4, 4, 8, torch.bfloat16, training=False)
+    stats, gate = (t["running_mean"], t["running_var"]), [t[k] for k in ("fc1_weight", "fc1_bias", "fc2_weight", "fc2_bias")]
+
+    def both(v):
+        leaf = v.detach().requires_grad_(True)
+        out = ops.norm_gate_residual(leaf, v, t["weight"], t["bias"], *stats, *gate, training=False)
+        return out.detach(), torch.autograd.grad(out, leaf, out.detach())[0]
+    assert x.numel() > 2 ** 31
+    whole = both(x)
+    for e in ends:
+        alone = both(x[e].contiguous(memory_format=layout))
+        for a, b in zip(whole, alone):
+            assert torch.equal(a[e], b)
+
+
+def test_norm_graph_used_twice_and_shared_arguments():
+    """A retained graph gives the same gradients again; one tensor as x and residual gets both gradients, one weight in two
+    norms their sum."""
+    from alphazero_amd import ops
+    t = norm_inputs(6, 10, 8, 8, 3, torch.float32, seed=14)
+    x, w = t["x"].clone().requires_grad_(True), t["weight"].clone().requires_grad_(True)
+    stats = torch.zeros(10, device="cuda"), torch.ones(10, device="cuda")
+    gate = [t[k] for k in ("fc1_weight", "fc1_bias", "fc2_weight", "fc2_bias")]
+    out = ops.norm_gate_residual(x, x, w, t["bias"], *stats, *gate)
+    first = torch.autograd.grad(out, (x, w), t["grad"], retain_graph=True)
+    again = torch.autograd.grad(out, (x, w), t["grad"], retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    apart = run_norm({**t, "residual": t["x"]})
+    # (a border of the ReLU may lie elsewhere than in norm_inputs: both runs here have the same one)
+    assert torch.equal(first[0], apart["x"] + apart["residual"]) and torch.equal(first[1], apart["weight"])
+    two = ops.norm_act(ops.norm_act(x, w, t["bias"], *stats), w, t["bias"], *stats)
+    y = ops.norm_act(x, w, t["bias"], *stats).detach().requires_grad_(True)
+    v = w.detach().clone().requires_grad_(True)
+    gy, gv = torch.autograd.grad(ops.norm_act(y, v, t["bias"], *stats), (y, v), t["grad"])
+    inner, = torch.autograd.grad(ops.norm_act(x, w, t["bias"], *stats), w, gy)
+    assert torch.equal(torch.autograd.grad(two, w, t["grad"])[0], inner + gv)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out = ops.norm_act(x, w, t["bias"], *stats)
+        with torch.no_grad():
+            w.mul_(2)
+        out.backward(t["grad"])
 
 
 # ------------------------------------------------------------------------------------------------ the loss
