@@ -9,7 +9,9 @@
 // that they become in 8 bits.  The quotient is a product with the hardware's reciprocal: one last place of the update.
 //
 // What bounds it: memory.  A 32-bit step reads 16 and writes 12 bytes per weight, an 8-bit one 10 and 6; clipping reads
-// the gradients once more.
+// the gradients once more.  Measured: k_adam on the 20x128 network's 8.0 M weights 41 us in 32 bits (5.5 TB/s), 29 us in
+// 8 (4.4 TB/s: the codes' 80 instructions a weight are 20 us of it); on the 28 M of 20x256 in 8 bits 88 us (5.1 TB/s);
+// k_adam_begin 9 us with the norm of 8.0 M gradients, 5 us without.
 // Layout: a workgroup takes a piece of OPT_CHUNK elements of one tensor.  Which one is in a table that is made once, in
 // device memory; the tensors' addresses travel in the kernel arguments (OPT_TABLE tensors a launch, so that the default
 // network's 214 are one), nothing is uploaded per step: it can be captured, and tensors may move between steps.

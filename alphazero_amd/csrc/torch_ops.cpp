@@ -2,8 +2,9 @@
 // C entries of libazamd.so (bound by address, so that a diagnostic build of the library is used where one is loaded).
 //
 // Why this is native: a Python autograd node costs 30 us in the backward pass and 25 us of argument handling per call,
-// and a step over 216 parameters 100 us of list building, where the kernels themselves take 40 to 100 us (measured on the
-// box's host: norm_gate_residual forward + backward 152 us in Python; FusedAdam.step 150 us).
+// and a step over 216 parameters 100 us of list building, where the kernels themselves take 40 to 100 us.  Measured on the
+// host: norm_gate_residual forward + backward 152 us with a Python node, 104 with this one, of which torch's own engine
+// takes some 60 (it hands the node and each of its eight gradients from thread to thread); FusedAdam.step 150 and 25 us.
 #include <mutex>
 
 #include <pybind11/pybind11.h>

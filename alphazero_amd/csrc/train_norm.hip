@@ -14,9 +14,13 @@
 // and the channel sums of dy come from S1, S2, dq and the board means, so grad and x are read twice.
 //
 // What bounds it: memory (the arithmetic is a handful of operations per value).  The plain form reads or writes 7
-// activations, the gated one 10, of which 4 and 6 could not be avoided by any form; whether out > 0 is kept as a byte per
-// 16 bytes of x.  Statistics are taken about a value of the row (its first), then joined as centred sums in 64 bits: no
+// activations, the gated one 10, of which 4 and 6 could not be avoided by any form: x and the gradient are needed again
+// once the batch's sums are known.  Whether out > 0 is kept as a byte per 16 bytes of x.  Statistics are taken about
+// the row's own mean (or, in rows longer than 64 pieces, a value of the row), then joined as centred sums in 64 bits: no
 // difference of large squares anywhere.
+// Measured, forward and backward: at 4096 x 256 x 64 in bfloat16 (134 MB a tensor) 294 us, of which the four passes over
+// activations take 239 (1.34 GB: 5.6 TB/s; a copy of 1 GiB reaches 5.1) and the gate and the channel sums 55; at
+// 1024 x 128 x 64 in float32 83 us (61 and 22); a plain norm at 1024 x 128 x 64 in bfloat16 34 us (26 and 8).
 #include <math.h>
 
 #include <type_traits>
@@ -702,7 +706,9 @@ __device__ inline void channel_grads(const NormParams& p, int block) {
 
 // --------------------------------------------------------------------------------------------- the gate
 // A workgroup takes four boards: their vectors lie in the LDS as [element][board], so one 16-byte read serves four boards
-// and a weight is loaded once for all of them.  Weights are read along their rows, 16 bytes a lane.
+// and a weight is loaded once for all of them.  Weights are read along their rows, 16 bytes a lane.  Four dependent
+// round trips to memory bound it (statistics, fc1, fc2, results): 6.4 us forward and 6.8 us backward at 1024 boards of 128
+// channels and 16 hidden units, 17 us each at 4096 x 256 x 32.
 constexpr int GATE_THREADS = 256;
 
 // Four weights from p on; FOURS: the rows are multiples of four.
