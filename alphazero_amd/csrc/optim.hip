@@ -353,7 +353,7 @@ extern "C" int64_t az_adam_plan(int32_t count, const int64_t* sizes_host, int64_
         }
         at += (sizes_host[i] + OPT_BLOCK - 1) / OPT_BLOCK * OPT_BLOCK;
     }
-    AZ_CHECK_ARG(at / OPT_BLOCK <= 0xFFFFFFFF && piece <= 0x7FFFFFFF, "az_adam_plan: too many elements");
+    AZ_CHECK_ARG(at / OPT_BLOCK <= 0xFFFFFFFF && piece <= MOST_BLOCKS, "az_adam_plan: too many elements");
     if (offsets_host) offsets_host[count] = at;
     return piece;
 }
@@ -379,7 +379,7 @@ extern "C" int az_adam_step(const az_adam_config* cfg, int32_t n_groups, const a
         AZ_CHECK_ARG(groups[g].end >= at && (g + 1 < n_groups ? groups[g].end <= count : groups[g].end == count),
                      "az_adam_step: group %d ends at %d of %d tensors", g, groups[g].end, count);
     if (pieces == 0) return AZ_OK;
-    AZ_CHECK_ARG(pieces <= 0x7FFFFFFF, "az_adam_step: too many elements");
+    AZ_CHECK_ARG(pieces <= MOST_BLOCKS, "az_adam_step: too many elements");
     AZ_CHECK_ARG(cfg->state_bits == 32 || cfg->state_bits == 8, "az_adam_step: moments in %d bits (32 or 8)", cfg->state_bits);
     AZ_CHECK_ARG(cfg->m_dev && cfg->v_dev && cfg->steps_dev && cfg->scratch_dev && cfg->pieces_dev, "az_adam_step: null state");
     AZ_CHECK_ARG(cfg->state_bits == 32 || (cfg->m_scale_dev && cfg->v_scale_dev), "az_adam_step: 8-bit moments need scales");

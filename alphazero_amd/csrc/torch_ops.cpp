@@ -12,10 +12,12 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/azamd.h"
@@ -56,7 +58,6 @@ void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t
 template <typename T>
 T* ptr(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
 
-
 int dtype_code(const Tensor& t) {
     switch (t.scalar_type()) {
         case at::kFloat: return AZ_F32;
@@ -74,6 +75,15 @@ Tensor held(const MaybeTensor& t) { return t ? *t : Tensor(); }
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 Tensor floats(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 
+// `like`, at element `at` of a buffer: a tensor of its own, not a view that autograd knows of (those refuse to be changed in
+// place when a node returns several).
+Tensor part_of(const Tensor& all, int64_t at, at::IntArrayRef sizes, at::IntArrayRef strides) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(all.storage()), all.key_set(), all.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(at);
+    t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides);
+    return t;
+}
+
 // Float tensors like these in one allocation, each at a multiple of 256 bytes: six small gradients cost what one does (1.4 us
 // instead of 8 us of a backward pass that takes 50 us of host time).
 std::vector<Tensor> together(const std::vector<Tensor>& like, const Tensor& device) {
@@ -85,12 +95,8 @@ std::vector<Tensor> together(const std::vector<Tensor>& like, const Tensor& devi
     }
     const Tensor all = floats(total, device);
     std::vector<Tensor> out(like.size());
-    for (size_t i = 0; i < like.size(); ++i) {
-        if (!like[i].defined()) continue;
-        out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(all.storage()), all.key_set(), all.dtype());
-        out[i].unsafeGetTensorImpl()->set_storage_offset(at[i]);
-        out[i].unsafeGetTensorImpl()->set_sizes_and_strides(like[i].sizes(), like[i].strides());
-    }
+    for (size_t i = 0; i < like.size(); ++i)
+        if (like[i].defined()) out[i] = part_of(all, at[i], like[i].sizes(), like[i].strides());
     return out;
 }
 
@@ -101,6 +107,19 @@ variable_list first_derivatives_only(variable_list grads, const char* name) {
         if (g.defined()) g = g.detach().set_requires_grad(true);
     auto node = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " has first derivatives only", (int64_t)grads.size());
     return (*node)(std::move(grads));
+}
+
+// A backward pass under capture that comes to a leaf whose eager graph on the default stream is still alive would accumulate
+// there, on a stream that cannot take part in a capture, and end the process: refused while it is still a forward pass.
+void refuse_eager_graph(std::initializer_list<const Tensor*> inputs) {
+    if (!at::GradMode::is_enabled() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const Tensor* t : inputs) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto stream = node ? node->stream() : std::nullopt;
+        TORCH_CHECK_VALUE(!stream || stream->id() != 0, "a forward pass is captured while an eager graph of the same leaf (shape ",
+                          t->sizes(), ") is alive on the default stream: drop its outputs first, or run it on another stream");
+    }
 }
 
 // ------------------------------------------------------------------------------------------------- norms
@@ -226,17 +245,23 @@ Tensor norm(const Tensor& x, const MaybeTensor& residual, const Tensor& weight, 
             const MaybeTensor& running_mean, const MaybeTensor& running_var, const MaybeTensor& w1,
             const MaybeTensor& b1, const MaybeTensor& w2, const MaybeTensor& b2, const MaybeTensor& num_batches,
             bool training, double momentum, double eps) {
+    TORCH_CHECK_VALUE(residual.has_value() == w1.has_value() && residual.has_value() == b1.has_value() &&
+                          residual.has_value() == w2.has_value() && residual.has_value() == b2.has_value(),
+                      "a gate needs residual, fc1_weight, fc1_bias, fc2_weight and fc2_bias");
     TORCH_CHECK_VALUE(x.is_cuda(), "the fused norms need a GPU tensor, got one on ", x.device());
     TORCH_CHECK_TYPE(dtype_code(x) >= 0, "activations must be float32, bfloat16 or float16, got ", x.scalar_type());
     TORCH_CHECK_VALUE(x.dim() == 4, "activations must have shape [boards, channels, height, width], got ", x.sizes());
     TORCH_CHECK_VALUE(x.numel() > 0, "no values to normalise in shape ", x.sizes());
     const int64_t c = x.size(1);
+    TORCH_CHECK_VALUE(x.size(0) <= INT32_MAX && c <= INT32_MAX && x.size(0) * c <= INT32_MAX && x.numel() / x.size(0) / c <= 1 << 24,
+                      "a norm takes up to 2^31 - 1 boards times channels and 2^24 places, got shape ", x.sizes());
     TORCH_CHECK_VALUE(!training || x.numel() / c > 1, "the batch's statistics need more than one value per channel, got shape ", x.sizes());
     TORCH_CHECK_VALUE(training || (running_mean.has_value() && running_var.has_value()), "evaluation needs running statistics");
     statistic("running_mean", running_mean, {c}, at::kFloat, x);
     statistic("running_var", running_var, {c}, at::kFloat, x);
     statistic("num_batches_tracked", num_batches, {}, at::kLong, x);
     const Tensor w = parameter("weight", weight, {c}, x), b = parameter("bias", bias, {c}, x);
+    refuse_eager_graph({&x, &weight, &bias});
     if (!residual)
         return NormFunction::apply(x, residual, w, b, w1, b1, w2, b2, running_mean, running_var, num_batches, training, momentum, eps);
     TORCH_CHECK_VALUE(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type() && residual->device() == x.device(),
@@ -246,6 +271,7 @@ Tensor norm(const Tensor& x, const MaybeTensor& residual, const Tensor& weight, 
     const int64_t hidden = w1->size(0);
     TORCH_CHECK_VALUE(hidden >= 1 && hidden <= 1024 && c <= 1024, "a gate takes up to 1024 channels and 1 to 1024 hidden units, got ", c,
                       " and ", hidden);
+    refuse_eager_graph({&*residual, &*w1, &*b1, &*w2, &*b2});
     const MaybeTensor p1 = parameter("fc1_weight", *w1, {hidden, c}, x), p2 = parameter("fc1_bias", *b1, {hidden}, x);
     const MaybeTensor p3 = parameter("fc2_weight", *w2, {2 * c, hidden}, x), p4 = parameter("fc2_bias", *b2, {2 * c}, x);
     return NormFunction::apply(x, residual, w, b, p1, p2, p3, p4, running_mean, running_var, num_batches, training, momentum, eps);
@@ -285,7 +311,7 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
         check(lib.loss_forward(&a, stream_of(policy)));
         ctx->save_for_backward({policy, wl, target_pi, target_wl, mask, stats});
         ctx->set_materialize_grads(false);
-        return losses.unbind(0);
+        return {part_of(losses, 0, {}, {}), part_of(losses, 1, {}, {}), part_of(losses, 2, {}, {})};
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -316,6 +342,10 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
             a.dpolicy_dev = out[0].data_ptr();
             a.dwl_dev = out[1].data_ptr();
             check(lib.loss_backward(&a, stream_of(s[0])));
+            if (!grads[0].defined()) {           // a head whose loss is not used gets none (and no 0 times NaN)
+                if (!grads[1].defined()) out[0] = Tensor();
+                if (!grads[2].defined()) out[1] = Tensor();
+            }
         }
         return first_derivatives_only(std::move(out), "policy_value_loss");
     }
@@ -330,6 +360,7 @@ py::tuple policy_value_loss(const Tensor& policy, const Tensor& wl, const Tensor
                       policy.sizes(), " and ", wl.sizes());
     TORCH_CHECK_VALUE(policy.numel() > 0 && wl.numel() > 0, "policy_value_loss of no rows or no classes");
     TORCH_CHECK_VALUE(wl.size(1) <= 4096, "up to 4096 outcomes, got ", wl.size(1));
+    TORCH_CHECK_VALUE(policy.size(0) <= 1 << 28 && policy.size(1) <= 1 << 28, "up to 2^28 rows and actions, got ", policy.sizes());
     const std::tuple<const char*, const Tensor*, const Tensor*> targets[] = {{"target_pis", &target_pi, &policy}, {"target_wls", &target_wl, &wl}};
     for (const auto& [name, t, like] : targets) {
         TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat, name, " must be float32, got ", t->scalar_type());
@@ -342,6 +373,7 @@ py::tuple policy_value_loss(const Tensor& policy, const Tensor& wl, const Tensor
     TORCH_CHECK_VALUE(wl.device() == policy.device() && target_pi.device() == policy.device() && target_wl.device() == policy.device() &&
                           (!mask || mask->device() == policy.device()),
                       "all tensors must be on ", policy.device());
+    refuse_eager_graph({&policy, &wl});
     const auto r = LossFunction::apply(policy.contiguous(), wl.contiguous(), target_pi.contiguous(), target_wl.contiguous(),
                                        mask ? MaybeTensor(mask->contiguous()) : mask,
                                        at::GradMode::is_enabled() && (policy.requires_grad() || wl.requires_grad()));

@@ -5,6 +5,8 @@
 
 namespace az {
 
+constexpr int64_t MOST_BLOCKS = 0xFFFFFF;      // workgroups of 256 threads: a launch has fewer than 2^32 threads
+
 // A load or store of 16 bytes needs only the element's own alignment: the hardware takes unaligned global accesses
 // in one instruction.  So rows of any length and tensors at any offset run through the same wide path.
 template <typename T> struct Pack;

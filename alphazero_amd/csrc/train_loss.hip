@@ -376,6 +376,8 @@ static int loss_entry(const az_loss_args* a, bool backward, void* stream) {
     AZ_CHECK_ARG(a->n >= 1 && a->n <= 1 << 28, "policy/value loss: %lld rows (1 to 2^28)", (long long)a->n);
     AZ_CHECK_ARG(a->actions >= 1 && a->actions <= 1 << 28 && a->outcomes >= 1 && a->outcomes <= 4096,
                  "policy/value loss: %d actions, %d outcomes", a->actions, a->outcomes);
+    AZ_CHECK_ARG((a->actions <= 512 ? (a->n + 3) / 4 : a->n) + a->n / LOSS_THREADS < MOST_BLOCKS,
+                 "policy/value loss: %lld rows of %d actions are more than a launch takes", (long long)a->n, a->actions);
     AZ_CHECK_ARG(a->policy_dev && a->wl_dev && a->target_pi_dev && a->target_wl_dev && a->stats_dev && (uintptr_t)a->stats_dev % 16 == 0,
                  "policy/value loss: null input, or row statistics not aligned to 16 bytes");
     LossParams p;

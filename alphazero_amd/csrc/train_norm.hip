@@ -1143,12 +1143,16 @@ static int norm_params(const az_norm_args* a, NormParams* p, int64_t sizes[3]) {
     AZ_CHECK_ARG(a->hidden >= 0 && (a->hidden == 0 || (a->c <= NORM_MAX_GATED && a->hidden <= NORM_MAX_GATED)),
                  "norm: a gate takes up to %d channels and hidden units (got %d, %d)", NORM_MAX_GATED, a->c, a->hidden);
     const int V = a->dtype == AZ_F32 ? 4 : 8;
+    const int nvec = (int)(((int64_t)(a->channels_last ? a->c : a->hw) + V - 1) / V);
+    const int64_t groups = nvec <= 8 ? 32 : nvec <= 16 ? 16 : nvec <= 32 ? 8 : 4, room = MOST_BLOCKS - 16384;      // (the weights' joins)
+    AZ_CHECK_ARG(a->channels_last ? a->n <= room && a->c <= 1 << 23 : (a->n + 3) / 4 * ((a->c + groups - 1) / groups) <= room && a->c < 1 << 26,
+                 "norm: %lld x %d x %d is more than a launch takes", (long long)a->n, a->c, a->hw);
     const size_t rows = (size_t)a->n * a->c, hidden = (size_t)a->n * a->hidden;
     p->n = a->n;
     p->c = a->c;
     p->hw = a->hw;
     p->hidden = a->hidden;
-    p->nvec = ((a->channels_last ? a->c : a->hw) + V - 1) / V;
+    p->nvec = nvec;
     p->training = a->training != 0;
     p->eps = a->eps;
     p->momentum = a->momentum;

@@ -6,7 +6,8 @@ few launches each.  They need a GPU tensor; there is no CPU fallback.
 Activations and logits: float32, bfloat16 or float16, contiguous or channels-last (other strides are copied).
 Parameters and statistics: float32.  All arithmetic and all sums are float32 or wider, outputs are rounded once.
 The calls run on the current stream of the tensors' device, allocate only through torch and can be captured into
-a HIP graph.  First derivatives only.
+a HIP graph (a forward pass is refused there while an eager graph of the same leaf parameters lives on the default
+stream: torch would accumulate the gradients on that stream).  First derivatives only.
 Arguments are checked, and the autograd nodes written, in csrc/torch_ops.cpp.
 """
 from . import _lib

@@ -1,4 +1,4 @@
-"""Adam and AdamW over all tensors of a model in a few launches (az_grad_sumsq, az_adam_step in include/azamd.h),
+"""Adam and AdamW over all tensors of a model in a few launches (az_adam_plan, az_adam_step in include/azamd.h),
 with gradient clipping by the global norm and moments in 32 bits or in 8.  It needs parameters on a GPU; there is
 no CPU fallback."""
 import torch
@@ -88,6 +88,9 @@ class FusedAdam(torch.optim.Optimizer):
                 raise ValueError(f"all parameters must be on one GPU, got {device} and {p.device}")
             if not _dense(p):
                 raise ValueError(f"a parameter of shape {tuple(p.shape)} and strides {p.stride()} does not fill its memory")
+        spans = sorted((p.data_ptr(), p.data_ptr() + 4 * p.numel()) for p in params if p.numel())
+        if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+            raise ValueError("two parameters share memory: each weight takes one update")
         self._params, self._device = params, device
         self._plan = _lib.torch_ops().AdamPlan(params)
         *self._offsets, total = self._plan.offsets()

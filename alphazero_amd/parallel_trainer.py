@@ -325,7 +325,7 @@ class ParallelTrainer:
     training forward under torch.autocast; `fused_ops` (extra, GPU only) trains with the
     library's own kernels for everything but convolutions and linear layers: fused
     norms and block ends, the loss with its gradient, and FusedAdam (clipping and the
-    update of all tensors in three launches), whose moments take `optimizer_bits`
+    update of all tensors in two launches), whose moments take `optimizer_bits`
     (32 or 8) bits.  Checkpoints are the same files either way."""
 
     def __init__(self, model: AlphaZeroNet, device: str = "cpu",

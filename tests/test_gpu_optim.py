@@ -478,3 +478,12 @@ def test_closure_scheduler_and_scaler():
     scaler.scale((p * p).sum() * math.inf).backward()
     scaler.step(opt)                                                   # infinite gradients: the step is left out
     assert torch.equal(p.detach(), before) and float(opt.flat_state()["step"]) == 2.0
+
+
+def test_parameters_that_share_memory_are_refused():
+    from alphazero_amd.optim import FusedAdam
+    flat = torch.zeros(100, device="cuda")
+    apart = [flat[:50].requires_grad_(True), flat[50:].requires_grad_(True)]
+    FusedAdam(apart)
+    with pytest.raises(ValueError, match="share memory"):
+        FusedAdam([flat[40:60].detach().requires_grad_(True)] + apart)

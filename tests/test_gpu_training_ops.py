@@ -578,3 +578,61 @@ def test_operators_on_a_side_stream_and_in_a_graph():
         got = [v.clone() for v in held]
         reset()
         assert all(torch.equal(a, b.detach()) for a, b in zip(got, work()))
+
+
+def test_losses_are_tensors_of_their_own():
+    """Each of the three may be changed in place (a regulariser added, a factor taken) without touching the others."""
+    from alphazero_amd import ops
+    z, wl, t, tw, _ = loss_inputs(7, 30, torch.float32, False)
+    z.requires_grad_(True)
+    want = [v.detach().clone() for v in ops.policy_value_loss(z, wl, t, tw)]
+    plain, = torch.autograd.grad(ops.policy_value_loss(z, wl, t, tw)[0], z)
+    loss, pi, w = ops.policy_value_loss(z, wl, t, tw)
+    loss += 1.0
+    loss *= 2.0
+    assert torch.equal(loss.detach(), (want[0] + 1.0) * 2.0) and torch.equal(pi.detach(), want[1]) and torch.equal(w.detach(), want[2])
+    assert torch.equal(torch.autograd.grad(loss, z)[0], 2 * plain)
+
+
+def test_a_head_whose_loss_is_not_used_gets_no_gradient():
+    from alphazero_amd import ops
+    for dtype in DTYPES:
+        z, wl, t, tw, _ = loss_inputs(7, 30, dtype, False)
+        wl[0, 0] = math.inf
+        z.requires_grad_(True), wl.requires_grad_(True)
+        _, pi, _ = ops.policy_value_loss(z, wl, t, tw)
+        got = torch.autograd.grad(pi, (z, wl), allow_unused=True)
+        assert got[1] is None and bool(torch.isfinite(got[0]).all())
+        _, _, w = ops.policy_value_loss(z, wl, t, tw)
+        assert torch.autograd.grad(w, (z, wl), allow_unused=True)[0] is None
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    """An eager graph of the same leaves on the default stream: the forward pass says so, before a backward pass could
+    accumulate on a stream that is not part of the capture.  Without it the same capture works."""
+    from alphazero_amd import ops
+    t = norm_inputs(4, 6, 8, 8, 2, torch.float32)
+    z, wl, tp, tw, _ = loss_inputs(4, 30, torch.float32, False)
+    w, z = t["weight"].clone().requires_grad_(True), z.requires_grad_(True)
+    stats = torch.zeros(6, device="cuda"), torch.ones(6, device="cuda")
+    calls = [lambda: ops.norm_act(t["x"], w, t["bias"], *stats), lambda: ops.policy_value_loss(z, wl, tp, tw)[0]]
+    for call in calls:
+        alive = call()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(ValueError, match="eager graph of the same leaf"):
+            with torch.cuda.graph(graph):
+                call()
+        with torch.no_grad():
+            call()                                   # (no graph: nothing to refuse)
+        del alive
+        leaf = w if call is calls[0] else z
+        leaf.grad = None
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call().sum().backward()
+        want, = torch.autograd.grad(call().sum(), leaf)
+        for _ in range(3):
+            leaf.grad.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(leaf.grad, want)

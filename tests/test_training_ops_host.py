@@ -159,3 +159,28 @@ def test_dense_layouts_are_told_apart():
     assert _dense(t) and _dense(t.to(memory_format=torch.channels_last)) and _dense(t.permute(3, 1, 0, 2)) and _dense(t[:, :, :0])
     assert not _dense(t[:, :3]) and not _dense(t[..., ::2]) and not _dense(torch.zeros(1, 4).expand(3, 4))
     assert _dense(torch.zeros(())) and _dense(torch.zeros(1)[:, None].expand(1, 1))
+
+
+@pytest.mark.parametrize("given", [(1, 0, 0, 0, 0), (0, 1, 1, 1, 1), (1, 1, 0, 1, 1), (1, 1, 1, 1, 0)])
+def test_a_gate_in_parts_is_refused(given):
+    x = torch.zeros(2, 4, 3, 3)
+    residual, *gate = [t if on else None for on, t in zip(given, (x, torch.zeros(2, 4), torch.zeros(2), torch.zeros(8, 2), torch.zeros(8)))]
+    with pytest.raises(ValueError, match="a gate needs"):
+        ops.norm_gate_residual(x, residual, torch.ones(4), torch.zeros(4), None, None, *gate)
+
+
+@pytest.mark.parametrize("kw", [{"n": 1 << 24, "channels_last": 1}, {"n": 1 << 26, "c": 2}, {"n": 1 << 22, "c": 100, "hw": 4096},
+                                {"n": 1, "c": 1 << 26}, {"n": 2, "c": (1 << 23) + 1, "channels_last": 1}])
+def test_norms_of_more_workgroups_than_a_launch_takes_are_refused(kw):
+    L = _lib.lib()
+    sizes = (C.c_int64 * 3)()
+    assert L.az_norm_sizes(C.byref(_norm_args(**kw)), sizes) == -1 and b"more than a launch takes" in L.az_last_error()
+    fits = {"n": (1 << 24) - (1 << 15), "channels_last": 1}, {"n": 1 << 22, "c": 100}
+    assert all(L.az_norm_sizes(C.byref(_norm_args(**k)), sizes) == 0 for k in fits)
+
+
+@pytest.mark.parametrize("n, actions", [(1 << 24, 513), (1 << 26, 5)])
+def test_losses_of_more_workgroups_than_a_launch_takes_are_refused(n, actions):
+    L = _lib.lib()
+    a = _lib.LossArgs(n, actions, 2, 0, 64, 64, 64, 64, None, 64, 64)
+    assert L.az_policy_value_loss_forward(C.byref(a), None) == -1 and b"more than a launch takes" in L.az_last_error()
