@@ -708,7 +708,8 @@ __device__ inline void channel_grads(const NormParams& p, int block) {
 // A workgroup takes four boards: their vectors lie in the LDS as [element][board], so one 16-byte read serves four boards
 // and a weight is loaded once for all of them.  Weights are read along their rows, 16 bytes a lane.  Four dependent
 // round trips to memory bound it (statistics, fc1, fc2, results): 6.4 us forward and 6.8 us backward at 1024 boards of 128
-// channels and 16 hidden units, 17 us each at 4096 x 256 x 32.
+// channels and 16 hidden units, 17 us each at 4096 x 256 x 32.  (There, eight boards to a workgroup: 20 and 21 us, half the
+// weights' traffic but half the workgroups to wait for it; eight rows ahead: 21 and 17.)
 constexpr int GATE_THREADS = 256;
 
 // Four weights from p on; FOURS: the rows are multiples of four.

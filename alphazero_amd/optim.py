@@ -12,6 +12,8 @@ def _dense(t):
     """Whether t's elements fill one stretch of memory, in whatever order of dimensions."""
     if t.numel() == 0:
         return True
+    if t.is_contiguous():
+        return True
     expected = 1
     for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
         if stride != expected:
@@ -116,14 +118,14 @@ class FusedAdam(torch.optim.Optimizer):
         self._attach()
 
     def _view(self, flat, i):
-        p, at = self._params[i], self._offsets[i]
-        return flat[at:at + p.numel()].as_strided(p.size(), p.stride())
+        p = self._params[i]
+        return flat.as_strided(p.size(), p.stride(), self._offsets[i])
 
     def _attach(self):
         """self.state as torch.optim.Adam has it: views of the flat buffers."""
         self.state.clear()
-        for i, p in enumerate(self._params):
-            self.state[p] = {"step": self._step[i]}
+        for i, (p, step) in enumerate(zip(self._params, self._step.unbind())):
+            self.state[p] = {"step": step}
             if self.state_bits == 32:
                 self.state[p].update((k, self._view(v, i)) for k, v in self._flat.items())
 

@@ -636,3 +636,63 @@ def test_capture_beside_an_eager_graph_is_refused():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(leaf.grad, want)
+
+
+def test_operators_in_inference_mode_and_beside_each_other_in_threads():
+    """No graph is kept in inference mode, the statistics move all the same; two threads on streams of their own get what one
+    gets."""
+    import threading
+    from alphazero_amd import ops
+    t = norm_inputs(9, 10, 8, 8, 4, torch.float32, seed=5)
+    gate = [t[k] for k in ("fc1_weight", "fc1_bias", "fc2_weight", "fc2_bias")]
+    z, wl, tp, tw, mask = loss_inputs(9, 50, torch.float32, True)
+
+    def work():
+        x, r, logits = (v.detach().clone().requires_grad_(True) for v in (t["x"], t["residual"], z))
+        stats = torch.zeros(10, device="cuda"), torch.ones(10, device="cuda")
+        out = ops.norm_gate_residual(x, r, t["weight"], t["bias"], *stats, *gate)
+        loss = ops.policy_value_loss(logits, wl, tp, tw, mask)[0]
+        return [out, loss] + list(torch.autograd.grad((out, loss), (x, r, logits), (t["grad"], torch.ones_like(loss)))) + list(stats)
+    want = [v.detach() for v in work()]
+    with torch.inference_mode():
+        stats = torch.zeros(10, device="cuda"), torch.ones(10, device="cuda")
+        out = ops.norm_gate_residual(t["x"], t["residual"], t["weight"], t["bias"], *stats, *gate)
+        loss = ops.policy_value_loss(z, wl, tp, tw, mask)[0]
+        assert not out.requires_grad and not loss.requires_grad
+        assert all(torch.equal(a, b) for a, b in zip((out, loss, *stats), (want[0], want[1], *want[-2:])))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run():
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                if not all(torch.equal(a.detach(), b) for a, b in zip(work(), want)):
+                    wrong.append(1)
+    threads = [threading.Thread(target=run) for _ in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
+
+
+@pytest.mark.parametrize("outcomes", [1, 3, 300])
+def test_loss_of_other_outcome_counts_and_mask_bytes(outcomes):
+    """Any number of outcomes; a byte mask counts what is not zero."""
+    from alphazero_amd import ops
+    z, wl, t, tw, mask = loss_inputs(21, 45, torch.float32, True, outcomes=outcomes)
+    z.requires_grad_(True), wl.requires_grad_(True)
+    a = ops.policy_value_loss(z, wl, t, tw, mask)
+    b = ops.policy_value_loss(z, wl, t, tw, mask.to(torch.uint8) * 200)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    logp = torch.log_softmax(wl.detach().double(), 1)
+    want = -(tw.double() * logp).sum(1).mean()
+    # a term of the sum is t (m - z) and T log S: each a few roundings of its magnitude
+    magnitude = float((tw.double().abs() * (wl.detach().double().amax(1, keepdim=True) - wl.detach().double())).sum(1).mean() + math.log(outcomes + 1))
+    assert abs(float(a[2].detach()) - float(want)) <= (outcomes + 16) * 2.0 ** -24 * magnitude
+    g, = torch.autograd.grad(a[2], wl)
+    exact = (logp.exp() * tw.double().sum(1, keepdim=True) - tw.double()) / 21
+    # exp's argument is off by its own rounding, 2^-24 |z - m|, the sum by outcomes roundings
+    spread = float((wl.detach().amax(1) - wl.detach().amin(1)).max())
+    assert float((g.double() - exact).abs().max()) <= (spread + outcomes + 16) * 2.0 ** -24 * 2 / 21 * max(1.0, float(tw.sum(1).max()))
