@@ -342,7 +342,8 @@ int az_engine_selfplay_stats(az_engine* e, az_selfplay_stats* out, void* stream)
  * (w, b) = fc2(relu(fc1(mean over the board of bn(x)))), src/model.py:40-53, 85-92).
  * x, residual, out, grad, dx, dresidual: [n][c][hw], or [n][hw][c] with channels_last != 0.
  * Sizes in bytes of `saved` (kept for the backward pass), of the forward and of the backward
- * workspace: az_norm_sizes.  These buffers are 16-byte aligned. */
+ * workspace: az_norm_sizes.  These buffers are 16-byte aligned.  Refused: n c over 2^31 - 1, hw over 2^24, and what
+ * takes more than 2^24 workgroups (from 2^26 boards on, and from 2^24 with channels last). */
 typedef struct {
     int64_t n;
     int32_t c, hw, hidden;       /* hidden > 0: c <= 1024 and hidden <= 1024 */
@@ -376,7 +377,8 @@ int az_norm_backward(const az_norm_args* args, void* stream);
  * Where az_policy_value_loss_ready answers 1 (float32 and bfloat16, one piece of 16 bytes to 8192
  * actions), the forward call also writes the gradients for an upstream of 1 if dpolicy_dev and dwl_dev
  * are given; a backward call with grads_ready != 0 then only multiplies them, in place, with an
- * upstream that is not 1. */
+ * upstream that is not 1.  Refused: more
+ * than 2^28 actions, 4096 outcomes, or 2^24 workgroups (from 2^24 rows on, 2^26 of up to 512 actions). */
 typedef struct {
     int64_t n;
     int32_t actions, outcomes, dtype;
