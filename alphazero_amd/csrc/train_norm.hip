@@ -15,12 +15,12 @@
 //
 // What bounds it: memory (the arithmetic is a handful of operations per value).  The plain form reads or writes 7
 // activations, the gated one 10, of which 4 and 6 could not be avoided by any form: x and the gradient are needed again
-// once the batch's sums are known.  Whether out > 0 is kept as a byte per 16 bytes of x.  Statistics are taken about
+// once the batch's sums are known.  A plain norm whose channels fit a workgroup's registers needs the 4.  Whether out > 0 is kept as a byte per 16 bytes of x.  Statistics are taken about
 // the row's own mean (or, in rows longer than 64 pieces, a value of the row), then joined as centred sums in 64 bits: no
 // difference of large squares anywhere.
 // Measured, forward and backward: at 4096 x 256 x 64 in bfloat16 (134 MB a tensor) 294 us, of which the four passes over
 // activations take 239 (1.34 GB: 5.6 TB/s; a copy of 1 GiB reaches 5.1) and the gate and the channel sums 55; at
-// 1024 x 128 x 64 in float32 83 us (61 and 22); a plain norm at 1024 x 128 x 64 in bfloat16 34 us (26 and 8).
+// 1024 x 128 x 64 in float32 83 us (61 and 22); a plain norm at 1024 x 128 x 64 in bfloat16 30 us.
 #include <math.h>
 
 #include <type_traits>
@@ -36,8 +36,8 @@ constexpr int NORM_MAX_GATED = 1024;         // their LDS: 16 (3 c + hidden) byt
 struct NormParams {
     int64_t n;
     int c, hw, hidden, nvec;                 // nvec: 16-byte pieces of a row (hw values, or c with channels last)
-    int training;
-    double eps, momentum;
+    int training, by_channel;
+    double eps, momentum, per_count, to_sample;      // the values of a channel: one by their number, number / (number - 1)
     const float *weight, *bias;
     float *running_mean, *running_var;
     int64_t* num_batches;
@@ -134,6 +134,22 @@ struct RowPlace {
     __device__ bool has_piece(const NormParams& p) const { return FIT == EXACT || (int)lane < p.nvec; }
 };
 
+// FULL: the piece is whole.
+template <bool FULL, typename T>
+__device__ inline typename Pack<T>::f32 load_piece(const T* p, int left) { return load_pack(p, FULL ? Pack<T>::V : left); }
+template <bool FULL, typename T>
+__device__ inline void store_piece(T* p, typename Pack<T>::f32 v, int left) { store_pack(p, v, FULL ? Pack<T>::V : left); }
+
+// f(piece, values left in the row, whether it is whole) for the lane's pieces of a long row: the whole ones four at a time,
+// their loads under way together, then the rest of the row.
+template <int L, int V, typename F>
+__device__ inline void over_pieces(const NormParams& p, int lane, F&& f) {
+    const int whole = p.hw / V;
+#pragma unroll 4
+    for (int j = lane; j < whole; j += L) f(j, V, std::true_type());
+    if (whole < p.nvec && lane == whole % L) f(whole, p.hw - whole * V, std::false_type());
+}
+
 template <typename T> __device__ inline typename Pack<T>::raw load_raw(const T* p) { return *(const typename Pack<T>::loose*)p; }
 template <typename T> __device__ inline typename Pack<T>::f32 widen(typename Pack<T>::raw v) { return __builtin_convertvector(v, typename Pack<T>::f32); }
 template <typename T> __device__ inline void store_raw(T* p, typename Pack<T>::f32 v) {
@@ -185,16 +201,15 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_stats(const T* __restrict_
                 const T* xr = x + r.row(p, k) * p.hw;
                 const float first = (float)xr[0];
                 float s = 0.f, ss = 0.f;
-                for (int j = r.lane; j < p.nvec; j += L) {
-                    const int left = p.hw - j * V;
-                    const auto v = load_pack(xr + j * V, left);
+                over_pieces<L, V>(p, r.lane, [&](int j, int left, auto whole) {
+                    const auto v = load_piece<decltype(whole)::value>(xr + j * V, left);
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         const float d = i < left ? v[i] - first : 0.f;
                         s += d;
                         ss += d * d;
                     }
-                }
+                });
                 s = lane_sum<L>(s);
                 ss = lane_sum<L>(ss);
                 const float mean = first + s / hw;
@@ -252,14 +267,14 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_apply(const T* __restrict_
         for (int k = 0; k < BOARDS_AT_ONCE && r.board(k) < p.n; ++k) {
             const size_t row = r.row(p, k), at = row * p.hw;
             const float A = p.A[GATED ? row : r.c], B = p.B[GATED ? row : r.c];
-            for (int j = r.lane; j < p.nvec; j += L) {
-                const int left = p.hw - j * V;
-                auto v = load_pack(x + at + j * V, left) * A + B;
-                if (GATED) v += load_pack(residual + at + j * V, left);
+            over_pieces<L, V>(p, r.lane, [&](int j, int left, auto whole) {
+                constexpr bool FULL = decltype(whole)::value;
+                auto v = load_piece<FULL>(x + at + j * V, left) * A + B;
+                if (GATED) v += load_piece<FULL>(residual + at + j * V, left);
                 const uint32_t bits = relu_bits(v);
-                store_pack(out + at + j * V, v, left);
+                store_piece<FULL>(out + at + j * V, v, left);
                 p.mask[row * p.nvec + j] = (uint8_t)bits;
-            }
+            });
         }
     }
 }
@@ -316,10 +331,10 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_sums(const T* __restr
             for (int k = 0; k < BOARDS_AT_ONCE && r.board(k) < p.n; ++k) {
                 const size_t row = r.row(p, k), at = row * p.hw;
                 float s1 = 0.f, s2 = 0.f;
-                for (int j = r.lane; j < p.nvec; j += L) {
-                    const int left = p.hw - j * V;
-                    const auto v = load_pack(x + at + j * V, left);
-                    auto g = load_pack(grad + at + j * V, left);
+                over_pieces<L, V>(p, r.lane, [&](int j, int left, auto whole) {
+                    constexpr bool FULL = decltype(whole)::value;
+                    const auto v = load_piece<FULL>(x + at + j * V, left);
+                    auto g = load_piece<FULL>(grad + at + j * V, left);
                     const uint32_t bits = p.mask[row * p.nvec + j];
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
@@ -327,8 +342,8 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_sums(const T* __restr
                         s1 += g[i];
                         s2 += g[i] * (v[i] - mean);
                     }
-                    if (GATED) store_pack(dresidual + at + j * V, g, left);
-                }
+                    if (GATED) store_piece<FULL>(dresidual + at + j * V, g, left);
+                });
                 board_sums(k, s1, s2);
             }
         }
@@ -389,18 +404,18 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_apply(const T* __rest
         for (int k = 0; k < BOARDS_AT_ONCE && r.board(k) < p.n; ++k) {
             const size_t row = r.row(p, k), at = row * p.hw;
             const float a = GATED ? ca * p.gate[row] : ca, d = GATED ? cd + per_place * p.dq[row] : cd;
-            for (int j = r.lane; j < p.nvec; j += L) {
-                const int left = p.hw - j * V;
-                const auto v = load_pack(x + at + j * V, left);
-                auto g = load_pack(grad + at + j * V, left);
+            over_pieces<L, V>(p, r.lane, [&](int j, int left, auto whole) {
+                constexpr bool FULL = decltype(whole)::value;
+                const auto v = load_piece<FULL>(x + at + j * V, left);
+                auto g = load_piece<FULL>(grad + at + j * V, left);
                 const uint32_t bits = GATED ? 0 : p.mask[row * p.nvec + j];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     if (!GATED) g[i] = bits >> i & 1 ? g[i] : 0.f;
                     g[i] = g[i] * a + ((v[i] - mean) * b + d);
                 }
-                store_pack(dx + at + j * V, g, left);
-            }
+                store_piece<FULL>(dx + at + j * V, g, left);
+            });
         }
     }
 }
@@ -429,12 +444,6 @@ __device__ inline Lanes lanes_of(const NormParams& p, int wide) {
     l.left = p.c - l.c;
     return l;
 }
-
-// FULL: every piece is whole.
-template <bool FULL, typename T>
-__device__ inline typename Pack<T>::f32 load_piece(const T* p, int left) { return load_pack(p, FULL ? Pack<T>::V : left); }
-template <bool FULL, typename T>
-__device__ inline void store_piece(T* p, typename Pack<T>::f32 v, int left) { store_pack(p, v, FULL ? Pack<T>::V : left); }
 
 // Numbers of the thread's channels, 16 bytes at a time.
 template <typename F>
@@ -1024,6 +1033,213 @@ __global__ __launch_bounds__(CHANNELS * LINES) void k_param_grads(const NormPara
     else weight_tile(p, (int)blockIdx.x - channel_blocks);
 }
 
+// ------------------------------------------------------------- a plain norm, [n][c][hw]: a workgroup to a channel
+// Where a channel's n rows fit a workgroup's registers (8192 pieces of 16 bytes: 1024 boards of 8 x 8 in 16 bits) it is read
+// once, its sums are taken there and the result leaves by the same kernel: one launch each way instead of three, 4
+// activations instead of 7, and no mask (whether out > 0 follows from x again, by the same operations).  Sums are
+// joined in 64 bits; the variance is taken about a first mean, with the remainder's square taken off.
+// Neighbouring channels share cache lines, so a die takes a range of them.
+// Forward and backward, beside the passes of row sums (all their launches): 37 x 48 x 81 in float16 10 us (22), 128 x 128 x 64 in
+// float32 14 (22), 512 x 128 x 64 in float32 24 (31), 8 x 1024 x 361 in float32 16 (39), 1024 x 128 x 64 in bfloat16 30 (34); with
+// two channels, so two workgroups, 1024 x 2 x 64 in bfloat16 takes 21 either way.
+constexpr int CHANNEL_PIECES = 8192;
+
+__device__ inline uint32_t channel_of(uint32_t block, uint32_t c) {
+    const uint32_t die = block % 8, more = c % 8;
+    return die * (c / 8) + (die < more ? die : more) + block / 8;
+}
+
+// The sums of a workgroup's v in all its threads, always in the same order.
+template <int THREADS, int K>
+__device__ inline void add_threads(double (&v)[K]) {
+    __shared__ double red[THREADS / 64][K];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        for (int off = 1; off < 64; off <<= 1) v[k] += __shfl_xor(v[k], off);
+    __syncthreads();                           // of what an earlier call put there, all is read
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int k = 0; k < K; ++k) red[threadIdx.x >> 6][k] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        v[k] = 0.0;
+#pragma unroll 4
+        for (int w = 0; w < THREADS / 64; ++w) v[k] += red[w][k];
+    }
+}
+
+// Makes the compiler forget what it knows of a register: what follows from it is computed again rather than kept (the
+// places of 8 pieces and their widened values would not fit a thread's 128 registers, and went to memory).
+template <typename R>
+__device__ inline void forget(R& r) { asm volatile("" : "+v"(r)); }
+
+template <typename T>
+__device__ inline void forget_raw(typename Pack<T>::raw& r) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 v = __builtin_bit_cast(u32x4, r);
+    forget(v);
+    r = __builtin_bit_cast(typename Pack<T>::raw, v);
+}
+
+// The i-th piece of a thread: where it begins, and its first value that is its own (the last piece of a row is moved back
+// to end with it; a piece past the end has none and reads the first one).
+template <typename T, int THREADS, bool WHOLE>
+struct ChannelPieces {
+    static constexpr int V = Pack<T>::V;
+    uint32_t c, thread, total, stride;
+    float per_row;
+
+    __device__ ChannelPieces(const NormParams& p, uint32_t c) : c(c), thread(threadIdx.x) {
+        total = (uint32_t)p.n * (uint32_t)p.nvec;
+        stride = (uint32_t)p.c * (uint32_t)p.hw;
+        per_row = 1.f / (float)p.nvec;
+    }
+    __device__ bool there(int i) const { return i * THREADS + thread < total; }
+    // The row comes from a product: below 8192 pieces it is off by less than the half that keeps it from the next one.
+    __device__ size_t place(const NormParams& p, int i, int& own) const {
+        const uint32_t piece = there(i) ? i * THREADS + thread : 0, row = (uint32_t)(((float)piece + 0.5f) * per_row);
+        const uint32_t begin = (piece - row * (uint32_t)p.nvec) * V, last = (uint32_t)p.hw - V, off = WHOLE || begin < last ? begin : last;
+        own = there(i) ? (int)(begin - off) : V;
+        return (size_t)row * stride + (c * (uint32_t)p.hw + off);
+    }
+    __device__ size_t place(const NormParams& p, int i) const {
+        int own;
+        return place(p, i, own);
+    }
+    __device__ static bool counts(int own, int k) { return WHOLE ? own == 0 : k >= own; }
+};
+
+// WHOLE: rows are whole pieces.
+template <typename T, int THREADS, int PIECES, bool WHOLE>
+__global__ __launch_bounds__(THREADS) void k_channel_forward(const T* __restrict__ x, T* __restrict__ out, const NormParams p) {
+    constexpr int V = Pack<T>::V;
+    const uint32_t c = channel_of(blockIdx.x, gridDim.x);
+    ChannelPieces<T, THREADS, WHOLE> q(p, c);
+    const float weight = p.weight[c], bias = p.bias[c];
+    typename Pack<T>::raw raw[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) raw[i] = load_raw(x + q.place(p, i));
+    forget(q.thread);
+    double mean, var;
+    if (p.training) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            int own;
+            q.place(p, i, own);
+            const auto v = widen<T>(raw[i]);
+#pragma unroll
+            for (int k = 0; k < V; ++k) s += q.counts(own, k) ? v[k] : 0.f;
+        }
+        double first[1] = {s};
+        add_threads<THREADS>(first);
+        forget(q.thread);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) forget_raw<T>(raw[i]);
+        const float about = (float)(first[0] * p.per_count);
+        float d1 = 0.f, d2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            int own;
+            q.place(p, i, own);
+            const auto v = widen<T>(raw[i]);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float d = q.counts(own, k) ? v[k] - about : 0.f;
+                d1 += d;
+                d2 += d * d;
+            }
+        }
+        double sums[2] = {d1, d2};
+        add_threads<THREADS>(sums);
+        forget(q.thread);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) forget_raw<T>(raw[i]);
+        const double rest = sums[0] * p.per_count;
+        mean = about + rest;
+        var = sums[1] * p.per_count - rest * rest;
+        if (var < 0.0) var = 0.0;              // a NaN stays one
+        if (threadIdx.x == 0) {
+            if (p.running_mean) p.running_mean[c] = (float)((1.0 - p.momentum) * p.running_mean[c] + p.momentum * mean);
+            if (p.running_var) p.running_var[c] = (float)((1.0 - p.momentum) * p.running_var[c] + p.momentum * var * p.to_sample);
+            if (p.num_batches && c == 0) *p.num_batches += 1;
+        }
+    } else {
+        mean = p.running_mean[c];
+        var = p.running_var[c];
+    }
+    // a root in 32 bits, and one step of Newton's in 64: every thread needs it, and a division and a root in 64 bits are slow
+    const double under = var + p.eps, near = rsqrtf((float)under);
+    const float inv = (float)(near * (1.5 - 0.5 * under * near * near)), m = (float)mean, scale = weight * inv;
+    if (threadIdx.x == 0) {
+        p.mean[c] = m;
+        p.inv[c] = inv;
+    }
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        auto v = widen<T>(raw[i]);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = not_below_zero(__builtin_fmaf(v[k] - m, scale, bias));
+        if (q.there(i)) store_raw(out + q.place(p, i), v);
+    }
+}
+
+template <typename T, int THREADS, int PIECES, bool WHOLE>
+__global__ __launch_bounds__(THREADS) void k_channel_backward(const T* __restrict__ x, const T* __restrict__ grad, T* __restrict__ dx,
+                                                              const NormParams p) {
+    constexpr int V = Pack<T>::V;
+    const uint32_t c = channel_of(blockIdx.x, gridDim.x);
+    ChannelPieces<T, THREADS, WHOLE> q(p, c);
+    const float m = p.mean[c], inv = p.inv[c], scale = p.weight[c] * inv, bias = p.bias[c];
+    typename Pack<T>::raw raw[PIECES], gr[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const size_t at = q.place(p, i);
+        raw[i] = load_raw(x + at);
+        gr[i] = load_raw(grad + at);
+    }
+    forget(q.thread);
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        int own;
+        q.place(p, i, own);
+        const auto v = widen<T>(raw[i]);
+        const auto g = widen<T>(gr[i]);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float xc = v[k] - m, gm = q.counts(own, k) && __builtin_fmaf(xc, scale, bias) > 0.f ? g[k] : 0.f;
+            s1 += gm;
+            s2 += gm * xc;
+        }
+    }
+    double sums[2] = {s1, s2};
+    add_threads<THREADS>(sums);
+    forget(q.thread);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        forget_raw<T>(raw[i]);
+        forget_raw<T>(gr[i]);
+    }
+    if (threadIdx.x == 0) {
+        p.dbias[c] = (float)sums[0];
+        p.dweight[c] = (float)(sums[1] * inv);
+    }
+    const float b = p.training ? (float)(-scale * inv * inv * (sums[1] * p.per_count)) : 0.f, d = p.training ? (float)(-scale * (sums[0] * p.per_count)) : 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const auto v = widen<T>(raw[i]);
+        auto g = widen<T>(gr[i]);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float xc = v[k] - m, gm = __builtin_fmaf(xc, scale, bias) > 0.f ? g[k] : 0.f;
+            g[k] = gm * scale + (xc * b + d);
+        }
+        if (q.there(i)) store_raw(dx + q.place(p, i), g);
+    }
+}
+
 // ---------------------------------------------------------------------------------------------- host side
 // f(lanes to a row, how the row fits them)
 template <typename T, typename F>
@@ -1039,6 +1255,25 @@ static void with_lanes(const NormParams& p, F&& f) {
     else if (p.nvec <= 16) f(std::integral_constant<int, 16>(), One());
     else if (p.nvec <= 32) f(std::integral_constant<int, 32>(), One());
     else f(std::integral_constant<int, 64>(), One());
+}
+
+// Whether a workgroup holds a channel.
+static bool by_channel(const az_norm_args* a, int nvec, int V) {
+    return !a->hidden && !a->channels_last && a->hw >= V && a->n * nvec <= CHANNEL_PIECES && a->c < 1 << 22 &&      // (2^32 threads)
+           (int64_t)a->c * a->hw <= 0x7FFFFFFF;
+}
+
+// f(threads, pieces a thread, whether rows are whole pieces)
+template <typename T, typename F>
+static void with_channel(const NormParams& p, F&& f) {
+    const auto whole = [&](auto threads, auto pieces) {
+        if (p.hw % Pack<T>::V == 0) f(threads, pieces, std::true_type());
+        else f(threads, pieces, std::false_type());
+    };
+    const int64_t pieces = p.n * p.nvec;
+    if (pieces <= 1024) whole(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+    else if (pieces <= 4096) whole(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+    else whole(std::integral_constant<int, 1024>(), std::integral_constant<int, 8>());
 }
 
 // f(whether the channels are at least one piece of 16 bytes)
@@ -1066,6 +1301,13 @@ template <typename T, bool GATED>
 static int norm_forward(NormParams p, bool last, const T* x, const T* residual, T* out, hipStream_t s) {
     const int wide = p.nvec < 64 ? p.nvec : 64;
     const dim3 boards((uint32_t)p.n, (p.nvec + wide - 1) / wide), block(NORM_THREADS);
+    if (p.by_channel) {
+        with_channel<T>(p, [&](auto threads, auto pieces, auto whole) {
+            hipLaunchKernelGGL((k_channel_forward<T, decltype(threads)::value, decltype(pieces)::value, decltype(whole)::value>), dim3(p.c), dim3(threads), 0, s, x, out, p);
+        });
+        AZ_HIP(hipGetLastError());
+        return AZ_OK;
+    }
     set_chunks<T>(p, last);
     if (p.training || GATED) {
         if (last) with_pieces<T>(p, [&](auto full) { hipLaunchKernelGGL((k_last_stats<T, decltype(full)::value, GATED>), boards, block, 0, s, x, p, wide); });
@@ -1095,6 +1337,13 @@ template <typename T, bool GATED>
 static int norm_backward(NormParams p, bool last, const T* x, const T* grad, T* dx, T* dresidual, hipStream_t s) {
     const int wide = p.nvec < 64 ? p.nvec : 64;
     const dim3 boards((uint32_t)p.n, (p.nvec + wide - 1) / wide), block(NORM_THREADS);
+    if (p.by_channel) {
+        with_channel<T>(p, [&](auto threads, auto pieces, auto whole) {
+            hipLaunchKernelGGL((k_channel_backward<T, decltype(threads)::value, decltype(pieces)::value, decltype(whole)::value>), dim3(p.c), dim3(threads), 0, s, x, grad, dx, p);
+        });
+        AZ_HIP(hipGetLastError());
+        return AZ_OK;
+    }
     set_chunks<T>(p, last);
     if (last) with_pieces<T>(p, [&](auto full) { hipLaunchKernelGGL((k_last_grad_sums<T, decltype(full)::value, GATED>), boards, block, 0, s, x, grad, dresidual, p, wide); });
     else with_lanes<T>(p, [&](auto L, auto fit) {
@@ -1157,6 +1406,8 @@ static int norm_params(const az_norm_args* a, NormParams* p, int64_t sizes[3]) {
     p->training = a->training != 0;
     p->eps = a->eps;
     p->momentum = a->momentum;
+    p->per_count = 1.0 / ((double)a->n * a->hw);
+    p->to_sample = 1.0 / (1.0 - p->per_count);
     p->weight = a->weight_dev;
     p->bias = a->bias_dev;
     p->running_mean = a->running_mean_dev;
@@ -1176,6 +1427,16 @@ static int norm_params(const az_norm_args* a, NormParams* p, int64_t sizes[3]) {
     p->board_mean = p->gate = p->h = p->s1 = p->s2 = p->de = p->dh = p->dq = p->partial = nullptr;
     p->mean = saved.take<float>(a->c);
     p->inv = saved.take<float>(a->c);
+    p->by_channel = by_channel(a, nvec, V);
+    if (p->by_channel) {                      // nothing else is kept, and no workspace used
+        p->mask = nullptr;
+        p->part_a = p->part_b = p->A = p->B = p->ca = p->cb = p->cd = nullptr;
+        if (sizes) {
+            sizes[0] = (int64_t)saved.used;
+            sizes[1] = sizes[2] = 0;
+        }
+        return AZ_OK;
+    }
     if (a->hidden) {
         p->board_mean = saved.take<float>(rows);
         p->gate = saved.take<float>(rows);
@@ -1207,8 +1468,8 @@ static int norm_params(const az_norm_args* a, NormParams* p, int64_t sizes[3]) {
     return AZ_OK;
 }
 
-static int norm_check(const az_norm_args* a) {
-    AZ_CHECK_ARG(a->x_dev && a->weight_dev && a->bias_dev && a->saved_dev && a->workspace_dev, "norm: null argument");
+static int norm_check(const az_norm_args* a, const NormParams& p) {
+    AZ_CHECK_ARG(a->x_dev && a->weight_dev && a->bias_dev && a->saved_dev && (a->workspace_dev || p.by_channel), "norm: null argument");
     AZ_CHECK_ARG((uintptr_t)a->saved_dev % 16 == 0 && (uintptr_t)a->workspace_dev % 16 == 0, "norm: buffers must be 16-byte aligned");
     AZ_CHECK_ARG(!a->hidden || (a->fc1_weight_dev && a->fc1_bias_dev && a->fc2_weight_dev && a->fc2_bias_dev), "norm: null gate weights");
     return AZ_OK;
@@ -1234,7 +1495,7 @@ extern "C" int az_norm_sizes(const az_norm_args* a, int64_t sizes_host[3]) {
 extern "C" int az_norm_forward(const az_norm_args* a, void* stream) {
     NormParams p;
     int rc = norm_params(a, &p, nullptr);
-    if (rc == AZ_OK) rc = norm_check(a);
+    if (rc == AZ_OK) rc = norm_check(a, p);
     if (rc != AZ_OK) return rc;
     AZ_CHECK_ARG(a->out_dev && (!a->hidden || a->residual_dev), "az_norm_forward: null argument");
     AZ_CHECK_ARG(a->training || (a->running_mean_dev && a->running_var_dev), "az_norm_forward: evaluation without running statistics");
@@ -1248,7 +1509,7 @@ extern "C" int az_norm_forward(const az_norm_args* a, void* stream) {
 extern "C" int az_norm_backward(const az_norm_args* a, void* stream) {
     NormParams p;
     int rc = norm_params(a, &p, nullptr);
-    if (rc == AZ_OK) rc = norm_check(a);
+    if (rc == AZ_OK) rc = norm_check(a, p);
     if (rc != AZ_OK) return rc;
     AZ_CHECK_ARG(a->grad_dev && a->dx_dev && a->dweight_dev && a->dbias_dev, "az_norm_backward: null argument");
     AZ_CHECK_ARG(!a->hidden || (a->dresidual_dev && a->dfc1_weight_dev && a->dfc1_bias_dev && a->dfc2_weight_dev && a->dfc2_bias_dev),

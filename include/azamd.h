@@ -342,7 +342,7 @@ int az_engine_selfplay_stats(az_engine* e, az_selfplay_stats* out, void* stream)
  * (w, b) = fc2(relu(fc1(mean over the board of bn(x)))), src/model.py:40-53, 85-92).
  * x, residual, out, grad, dx, dresidual: [n][c][hw], or [n][hw][c] with channels_last != 0.
  * Sizes in bytes of `saved` (kept for the backward pass), of the forward and of the backward
- * workspace: az_norm_sizes.  These buffers are 16-byte aligned.  Refused: n c over 2^31 - 1, hw over 2^24, and what
+ * workspace: az_norm_sizes (a workspace of 0 bytes may be null).  These buffers are 16-byte aligned.  Refused: n c over 2^31 - 1, hw over 2^24, and what
  * takes more than 2^24 workgroups (from 2^26 boards on, and from 2^24 with channels last). */
 typedef struct {
     int64_t n;

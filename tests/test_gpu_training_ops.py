@@ -696,3 +696,21 @@ def test_loss_of_other_outcome_counts_and_mask_bytes(outcomes):
     # exp's argument is off by its own rounding, 2^-24 |z - m|, the sum by outcomes roundings
     spread = float((wl.detach().amax(1) - wl.detach().amin(1)).max())
     assert float((g.double() - exact).abs().max()) <= (spread + outcomes + 16) * 2.0 ** -24 * 2 / 21 * max(1.0, float(tw.sum(1).max()))
+
+
+@pytest.mark.parametrize("n, c, h, w", [(64, 3, 8, 8), (65, 3, 8, 8), (128, 2, 8, 8), (129, 2, 8, 8), (256, 5, 8, 8), (257, 5, 8, 8), (512, 9, 8, 8),
+                                        (513, 9, 8, 8), (1024, 4, 8, 8), (1025, 4, 8, 8), (390, 17, 9, 9), (391, 17, 9, 9), (745, 2, 9, 9),
+                                        (1200, 6, 2, 2), (2, 3, 120, 151), (3, 2, 40, 53), (40, 8, 30, 31), (1, 2, 181, 190), (5, 9, 1, 4)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_plain_norms_around_what_a_workgroup_holds(n, c, h, w, dtype):
+    """Channels that just fit 1024, 4096 and 8192 pieces of 16 bytes and that just do not, rows that end inside a piece, long ones."""
+    t = norm_inputs(n, c, h, w, 0, dtype, seed=n + h)
+    check_norm(t)
+    if n % 2:
+        check_norm(norm_inputs(n, c, h, w, 0, dtype, seed=n + h + 1, training=False), training=False)
+
+
+@pytest.mark.parametrize("n, c, h, w, hidden", [(2, 3, 120, 151, 2), (3, 2, 40, 53, 2), (6, 4, 23, 12, 3)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gates_over_long_rows(n, c, h, w, hidden, dtype):
+    check_norm(norm_inputs(n, c, h, w, hidden, dtype, seed=n + h))
