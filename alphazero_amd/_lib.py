@@ -128,6 +128,7 @@ _SIGNATURES = {
     "az_policy_value_loss_backward": [C.POINTER(LossArgs), _VP],
     "az_adam_plan": [C.c_int32, _VP, _VP, _VP],
     "az_adam_scratch": [C.c_int32],
+    "az_graph_fill_by_kernels": [_VP, C.POINTER(C.c_int32)],
     "az_adam_step": [C.POINTER(AdamConfig), C.c_int32, C.POINTER(AdamGroup), C.c_int32, _VP, _VP, _VP, _VP],
 }
 _OPTIONAL = {}

@@ -36,6 +36,7 @@ $HIPCC $COMMON -mllvm -amdgpu-mfma-vgpr-form=1 -DAZ_SPLIT_STAMPS=${AZ_SPLIT_STAM
 # (v_accvgpr_*, s_nop 7) after any change to tower16.hip: python tools/tower16_isa_check.py [--agpr].
 $HIPCC $COMMON ${T16_FLAGS--mllvm -amdgpu-mfma-vgpr-form=1} -Rpass-analysis=kernel-resource-usage -c tower16.hip -o $OBJ/tower16.o 2> $OBJ/tower16.remarks & pids+=($!)
 $HIPCC $COMMON -c tower_any.hip -o $OBJ/tower_any.o & pids+=($!)
+$HIPCC $COMMON -c graph.hip -o $OBJ/graph.o & pids+=($!)
 # training operators; the optimiser's arithmetic is rounded operation by operation
 $HIPCC $COMMON -c train_norm.hip -o $OBJ/train_norm.o & pids+=($!)
 $HIPCC $COMMON -c train_loss.hip -o $OBJ/train_loss.o & pids+=($!)

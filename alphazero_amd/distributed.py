@@ -10,13 +10,14 @@ by rank, no collective during self-play):
 Both work on any torch.distributed backend: "nccl" (= RCCL over xGMI) on the
 GPUs, "gloo" on CPU tensors in the tests.
 """
+import ctypes
 from typing import List, Tuple
 
 import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
-from . import ops
+from . import _lib, ops
 from .config import Config
 from .optim import FusedAdam
 
@@ -222,6 +223,17 @@ def make_capturable(optimizer):
                 st["step"] = st["step"].to(p.device)
 
 
+def capture(work):
+    """A HIP graph of work(), which torch captures on a side stream.  Memset nodes, which torch's own calls record (a sum over
+    many rows clears its semaphores), have given wrong results on replays after the first: kernels take their place."""
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        work()
+    _lib.check(_lib.lib().az_graph_fill_by_kernels(graph.raw_cuda_graph(), ctypes.byref(ctypes.c_int32())))
+    graph.instantiate()
+    return graph
+
+
 class GraphedTrainStep:
     """train_step for one fixed slice size, replayed from two captured HIP graphs: (A) zero the
     gradients, forward, losses, backward; (B) gradient clipping and the Adam update.  Between
@@ -299,14 +311,10 @@ class GraphedTrainStep:
                 self.steps_seen += 1
                 return
             if self.graph_a is None:
-                self.graph_a = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(self.graph_a):
-                    self._grads()
+                self.graph_a = capture(self._grads)
             lr = float(self.optimizer.param_groups[0]["lr"])
             if self.graph_b is None or lr != self.lr:
-                self.graph_b = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(self.graph_b):
-                    self._update()
+                self.graph_b = capture(self._update)
                 self.lr = lr
             self.graph_a.replay()
             self._between(global_batch)

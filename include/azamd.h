@@ -438,6 +438,11 @@ int64_t az_adam_scratch(int32_t count);
 int az_adam_step(const az_adam_config* cfg, int32_t n_groups, const az_adam_group* groups_host, int32_t count,
                  const uint64_t* params_host, const uint64_t* grads_host, const int64_t* sizes_host, void* stream);
 
+/* Replaces every memset node of a captured hipGraph_t that is not instantiated yet by a kernel node
+ * that writes the same bytes, and counts them in replaced_host: memset nodes, which library calls
+ * record, have given wrong results on replays after the first. */
+int az_graph_fill_by_kernels(void* graph, int32_t* replaced_host);
+
 #ifdef __cplusplus
 }
 #endif

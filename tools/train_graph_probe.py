@@ -14,6 +14,7 @@ import torch
 import torch.nn.functional as F
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from alphazero_amd.distributed import capture  # noqa: E402
 from alphazero_amd.model import AlphaZeroNet  # noqa: E402
 
 ap = argparse.ArgumentParser()
@@ -61,9 +62,9 @@ for autocast in (False, True):
         for _ in range(5):
             step(m, o, autocast)
     torch.cuda.current_stream().wait_stream(s)
-    g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
-        loss = step(m, o, autocast)
+    held = []
+    g = capture(lambda: held.append(step(m, o, autocast)))
+    loss = held[0]
     for _ in range(3):
         g.replay()
     torch.cuda.synchronize()
