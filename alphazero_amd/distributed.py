@@ -162,6 +162,21 @@ def clip_and_step(model, optimizer):
     optimizer.step()
 
 
+def check_same_rounding(optimizer, device, group=None):
+    """Replicas stay identical only if every rank rounds its moments alike: a FusedAdam's bits and seed are compared over the
+    ranks, once per optimiser, and a difference is a ValueError on all of them."""
+    if not isinstance(optimizer, FusedAdam) or getattr(optimizer, "same_rounding", False):
+        return
+    mine = [optimizer.state_bits, optimizer.seed & 0xFFFFFFFF if optimizer.state_bits == 8 else 0]
+    largest = torch.tensor(mine + [-v for v in mine], dtype=torch.int64, device=device)
+    dist.all_reduce(largest, op=dist.ReduceOp.MAX, group=group)
+    bits, seed, less_bits, less_seed = largest.tolist()
+    if (bits, seed) != (-less_bits, -less_seed):
+        raise ValueError(f"FusedAdam has to be built with the same state_bits and seed on every rank, here they are {optimizer.state_bits} "
+                         f"and {optimizer.seed}, elsewhere others")
+    optimizer.same_rounding = True
+
+
 def train_step(model, optimizer, states, target_pis, target_wls, group=None, autocast_dtype=None,
                global_batch=None, as_tensor=False):
     """One optimisation step on this rank's slice of the batch.  With torch.distributed
@@ -205,6 +220,7 @@ def train_step(model, optimizer, states, target_pis, target_wls, group=None, aut
             total = torch.tensor([mine], dtype=torch.int64, device=states.device)
             dist.all_reduce(total, op=dist.ReduceOp.SUM, group=group)
             global_batch = int(total.item())
+        check_same_rounding(optimizer, states.device, group)
         weight = mine / max(1, global_batch)
         allreduce_gradients(model, weight, group)
         with torch.no_grad():
@@ -281,6 +297,7 @@ class GraphedTrainStep:
 
     def _between(self, global_batch):
         if dist.is_available() and dist.is_initialized() and dist.get_world_size(self.group) > 1:
+            check_same_rounding(self.optimizer, self.states.device, self.group)
             weight = self.n / max(1, global_batch)
             allreduce_gradients(self.model, weight, self.group)
             with torch.no_grad():

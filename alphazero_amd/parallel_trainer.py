@@ -340,8 +340,10 @@ class ParallelTrainer:
         if optimizer_bits != 32 and not fused_ops:
             raise ValueError("optimizer_bits is FusedAdam's: it needs fused_ops=True")
         if fused_ops:
+            # (its own seed for the rounding of 8-bit moments: self-play's differs from rank to rank, and replicas whose
+            # moments are rounded differently part after one step)
             self.optimizer = FusedAdam(model.parameters(), lr=Config.LEARNING_RATE, weight_decay=Config.WEIGHT_DECAY,
-                                       state_bits=optimizer_bits, seed=seed)
+                                       state_bits=optimizer_bits)
             model.use_fused_ops()
         else:
             self.optimizer = optim.Adam(model.parameters(), lr=Config.LEARNING_RATE, weight_decay=Config.WEIGHT_DECAY)
