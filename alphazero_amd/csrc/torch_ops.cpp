@@ -321,7 +321,7 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
         {
             const at::NoGradGuard no_grad;
             az_loss_args a = arguments(s[0], s[1], s[2], s[3], s[4], s[5]);
-            // the forward pass's gradients serve one backward pass (they are scaled in place and belong to whoever gets them)
+            // the forward pass's gradients serve one backward pass (they belong to whoever gets them)
             static std::mutex taking;
             {
                 const std::lock_guard<std::mutex> lock(taking);

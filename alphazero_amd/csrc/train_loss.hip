@@ -8,9 +8,9 @@
 //
 // Where the row fits a workgroup's registers (8192 actions) it is read once: first the maximum, then the sums, then the
 // gradient for an upstream of 1, written by the same kernel.  The backward pass then only looks at the upstream and, if
-// it is 1 (as it is when the loss itself is what backward() starts from), leaves what is there.  In float16 a gradient
-// divided by the rows and not yet multiplied with the program's loss scale would underflow: there, for longer rows and for
-// a second backward pass the gradient is computed from the logits again.
+// it is 1 (as it is when the loss itself is what backward() starts from), leaves what is there.  For another upstream, for
+// longer rows and for a second backward pass the gradient is computed from the logits again, and in float16 always: there one
+// that is divided by the rows and not yet multiplied with the program's loss scale would underflow.
 //
 // What bounds it: memory at large action spaces (k_loss_row at 8192 x 4001 in bfloat16 with a mask: 295 MB in 56 us,
 // 5.2 TB/s), launches at small ones (1024 x 192: 3.6 + 2.8 + 2.2 us).  All sums in 32 bits; rows are added in 64 bits in a
@@ -242,8 +242,9 @@ __global__ __launch_bounds__(LOSS_THREADS) void k_loss_forward(const LossParams 
     }
 }
 
-// Means over the rows: losses = (sum, policy, outcome).
-__global__ __launch_bounds__(1024) void k_loss_sum(const float* loss, int n, float* losses) {
+// Means over the rows: losses = (sum, policy, outcome).  Afterwards the first row's losses say that the gradients that were
+// written are those for an upstream of 1.
+__global__ __launch_bounds__(1024) void k_loss_sum(float* loss, int n, float* losses) {
     double a = 0.0, b = 0.0;
 #pragma unroll 4
     for (int i = threadIdx.x; i < n; i += 1024) {
@@ -268,6 +269,7 @@ __global__ __launch_bounds__(1024) void k_loss_sum(const float* loss, int n, flo
         losses[0] = (float)((a + b) / n);
         losses[1] = (float)(a / n);
         losses[2] = (float)(b / n);
+        loss[0] = loss[n] = 1.f;
     }
 }
 
@@ -275,56 +277,67 @@ __device__ inline float upstream_of(const LossParams& p, int which) {
     return (p.upstream[0] ? *p.upstream[0] : 0.f) + (p.upstream[which] ? *p.upstream[which] : 0.f);
 }
 
-// Gradients for an upstream of 1 are there: multiply them with what it is, in place.
-template <typename T>
-__global__ __launch_bounds__(LOSS_THREADS) void k_loss_scale(const LossParams p) {
-    constexpr int V = Pack<T>::V;
-    const float up = upstream_of(p, 1), up_wl = upstream_of(p, 2);
-    const int64_t stride = (int64_t)gridDim.x * LOSS_THREADS, first = (int64_t)blockIdx.x * LOSS_THREADS + threadIdx.x;
-    if (up != 1.f) {
-        const int64_t n = (int64_t)p.n * p.actions;
-        for (int64_t i = first * V; i < n; i += stride * V) {
-            const int left = n - i < V ? (int)(n - i) : V;
-            store_pack((T*)p.dpolicy + i, load_pack((const T*)p.dpolicy + i, left) * up, left);
-        }
+// Which of V places the mask keeps, of the first `left`: its bytes in one load where all are there.
+template <int V>
+__device__ inline uint32_t legal_bits(const uint8_t* mask, int left) {
+    typedef uint8_t bytes_t __attribute__((ext_vector_type(V)));
+    typedef bytes_t loose_bytes __attribute__((aligned(1)));
+    uint32_t bits = 0;
+    if (mask && left >= V) {
+        const bytes_t legal = *(const loose_bytes*)mask;
+#pragma unroll
+        for (int k = 0; k < V; ++k) bits |= (legal[k] ? 1u : 0u) << k;
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) bits |= (k < left && (!mask || mask[k]) ? 1u : 0u) << k;
     }
-    if (up_wl != 1.f) {
-        const int64_t n = (int64_t)p.n * p.outcomes;
-        for (int64_t i = first; i < n; i += stride) ((T*)p.dwl)[i] = (T)((float)((T*)p.dwl)[i] * up_wl);
-    }
+    return bits;
 }
 
+// The gradients from the logits.  ready: those for an upstream of 1 may be there already, from the forward kernel (the first
+// row's loss, which nothing needs any more, says so for each head): they stay if the upstream is 1.  For another one they are
+// computed anew, not multiplied: a gradient that is rounded already would be rounded twice, and a backward pass that is
+// replayed without its forward pass would multiply what it has multiplied.  (8192 x 4001 in
+// bfloat16 with a mask: 66 us, 4.4 TB/s; the multiplication took 20.)
 template <typename T, int GROUP>
-__global__ __launch_bounds__(LOSS_THREADS) void k_loss_backward(const LossParams p, int policy_blocks) {
+__global__ __launch_bounds__(LOSS_THREADS) void k_loss_backward(const LossParams p, int policy_blocks, int blocks, bool ready) {
     constexpr int V = Pack<T>::V, ROWS = LOSS_THREADS / GROUP;
-    if ((int)blockIdx.x >= policy_blocks) {
-        const int row = ((int)blockIdx.x - policy_blocks) * LOSS_THREADS + threadIdx.x;
-        if (row >= p.n) return;
-        const float up = upstream_of(p, 2) / (float)p.n, m = p.top[(size_t)p.n + row];
-        const float weight = p.inv[(size_t)p.n + row] * p.total[(size_t)p.n + row];
-        for (int i = 0; i < p.outcomes; ++i) {
-            const size_t k = (size_t)row * p.outcomes + i;
-            ((T*)p.dwl)[k] = (T)gradient((float)((const T*)p.wl)[k], p.target_wl[k], m, weight, up);
-        }
-        return;
+    const float up_policy = upstream_of(p, 1), up_wl = upstream_of(p, 2);
+    const bool leave_policy = ready && up_policy == 1.f && p.loss[0] == 1.f, leave_wl = ready && up_wl == 1.f && p.loss[p.n] == 1.f;
+    if (leave_policy && leave_wl) return;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {       // (who reads this meanwhile has an upstream that is not 1)
+        if (up_policy != 1.f) p.loss[0] = 0.f;
+        if (up_wl != 1.f) p.loss[p.n] = 0.f;
     }
-    const int row = blockIdx.x * ROWS + threadIdx.x / GROUP, lane = threadIdx.x % GROUP;
-    if (row >= p.n) return;
-    const float up = upstream_of(p, 1) / (float)p.n, m = p.top[row], weight = p.inv[row] * p.total[row];
-    const size_t at = (size_t)row * p.actions;
-    for (int i = lane * V; i < p.actions; i += GROUP * V) {
-        const int left = p.actions - i;
-        auto z = load_pack((const T*)p.policy + at + i, left);
-#pragma unroll
-        for (int k = 0; k < V; k += 4) {
-            const f32x4 q = load_pack(p.target_pi + at + i + k, left - k);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool keep = k + j < left && (!p.mask || p.mask[at + i + k + j]);
-                z[k + j] = keep ? gradient(z[k + j], q[j], m, weight, up) : 0.f;
+    const int lane = threadIdx.x % GROUP;
+    for (int block = blockIdx.x; block < blocks; block += gridDim.x) {
+        if (block >= policy_blocks) {
+            const int row = (block - policy_blocks) * LOSS_THREADS + threadIdx.x;
+            if (leave_wl || row >= p.n) continue;
+            const float up = up_wl / (float)p.n, m = p.top[(size_t)p.n + row];
+            const float weight = p.inv[(size_t)p.n + row] * p.total[(size_t)p.n + row];
+            for (int i = 0; i < p.outcomes; ++i) {
+                const size_t k = (size_t)row * p.outcomes + i;
+                ((T*)p.dwl)[k] = (T)gradient((float)((const T*)p.wl)[k], p.target_wl[k], m, weight, up);
             }
+            continue;
         }
-        store_pack((T*)p.dpolicy + at + i, z, left);
+        const int row = block * ROWS + threadIdx.x / GROUP;
+        if (leave_policy || row >= p.n) continue;
+        const float up = up_policy / (float)p.n, m = p.top[row], weight = p.inv[row] * p.total[row];
+        const size_t at = (size_t)row * p.actions;
+        for (int i = lane * V; i < p.actions; i += GROUP * V) {
+            const int left = p.actions - i;
+            auto z = load_pack((const T*)p.policy + at + i, left);
+            const uint32_t legal = legal_bits<V>(p.mask ? p.mask + at + i : nullptr, left);
+#pragma unroll
+            for (int k = 0; k < V; k += 4) {
+                const f32x4 q = load_pack(p.target_pi + at + i + k, left - k);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) z[k + j] = legal >> (k + j) & 1 ? gradient(z[k + j], q[j], m, weight, up) : 0.f;
+            }
+            store_pack((T*)p.dpolicy + at + i, z, left);
+        }
     }
 }
 
@@ -348,12 +361,11 @@ static int launch_loss(const LossParams& p, float* losses, bool backward, bool r
     const int group = p.actions <= 1024 ? 64 : LOSS_THREADS;
     const int pb = (p.n + LOSS_THREADS / group - 1) / (LOSS_THREADS / group), ob = (p.n + LOSS_THREADS - 1) / LOSS_THREADS;
     const dim3 grid(pb + ob), block(LOSS_THREADS);
-    if (backward && ready) {
-        const int64_t blocks = ((int64_t)p.n * p.actions + LOSS_THREADS * Pack<T>::V - 1) / (LOSS_THREADS * Pack<T>::V) + ob;
-        hipLaunchKernelGGL((k_loss_scale<T>), dim3((uint32_t)(blocks < 1024 ? blocks : 1024)), block, 0, s, p);
-    } else if (backward) {
-        if (group == 64) hipLaunchKernelGGL((k_loss_backward<T, 64>), grid, block, 0, s, p, pb);
-        else hipLaunchKernelGGL((k_loss_backward<T, LOSS_THREADS>), grid, block, 0, s, p, pb);
+    if (backward) {
+        // (most calls of a ready one find an upstream of 1 and leave: few workgroups, which take several blocks if they have to)
+        const dim3 few(ready && pb + ob > 2048 ? 2048 : pb + ob);
+        if (group == 64) hipLaunchKernelGGL((k_loss_backward<T, 64>), few, block, 0, s, p, pb, pb + ob, ready);
+        else hipLaunchKernelGGL((k_loss_backward<T, LOSS_THREADS>), few, block, 0, s, p, pb, pb + ob, ready);
     } else {
         if (!(p.dpolicy ? launch_row<T, true>(p, s) : launch_row<T, false>(p, s))) {
             if (group == 64) hipLaunchKernelGGL((k_loss_forward<T, 64>), grid, block, 0, s, p, pb);

@@ -376,9 +376,9 @@ int az_norm_backward(const az_norm_args* args, void* stream);
  * read by the backward call.  upstream_dev: gradients of the three losses, null = 0.
  * Where az_policy_value_loss_ready answers 1 (float32 and bfloat16, one piece of 16 bytes to 8192
  * actions), the forward call also writes the gradients for an upstream of 1 if dpolicy_dev and dwl_dev
- * are given; a backward call with grads_ready != 0 then only multiplies them, in place, with an
- * upstream that is not 1.  Refused: more
- * than 2^28 actions, 4096 outcomes, or 2^24 workgroups (from 2^24 rows on, 2^26 of up to 512 actions). */
+ * are given; a backward call with grads_ready != 0 then leaves them where the upstream is 1 and
+ * computes them anew where it is not, however often it is made.  Refused: more than
+ * 2^28 actions, 4096 outcomes, or 2^24 workgroups (from 2^24 rows on, 2^26 of up to 512 actions). */
 typedef struct {
     int64_t n;
     int32_t actions, outcomes, dtype;

@@ -1,0 +1,57 @@
+"""GPU: the training operators where they were wrong once.  Tolerances as in test_gpu_training_ops: k half-steps of float32
+of the magnitudes plus one rounding to the output's type."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from test_gpu_training_ops import DTYPES, close, loss_inputs, loss_reference
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ the loss
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, actions", [(64, 192), (33, 4001), (9, 9000), (4, 5)])
+@pytest.mark.parametrize("up", [1 / 3, 0.7, -3.0])
+def test_loss_gradients_are_rounded_once_whatever_the_upstream(dtype, n, actions, up):
+    """One rounding to the logits' type, as with an upstream of 1 (whose gradient is there already)."""
+    from alphazero_amd import ops
+    z, wl, t, tw, mask = loss_inputs(n, actions, dtype, True, seed=actions)
+    z.requires_grad_(True), wl.requires_grad_(True)
+    loss = ops.policy_value_loss(z, wl, t, tw, mask)[0]
+    got = torch.autograd.grad(loss, (z, wl), torch.full_like(loss, up))
+    _, _, grads, mags = loss_reference(z.detach(), wl.detach(), t, tw, mask, (float(torch.tensor(up)), 0.0, 0.0))
+    for a, b, m in zip(got, grads, mags):
+        close(a, b, m, 64 + -(-actions // 64) + 8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n, actions", [(70, 192), (10000, 600)])
+def test_backward_call_made_again_without_its_forward_call(dtype, n, actions):
+    """As a captured backward pass is replayed: each call gives the gradient of its own upstream, whatever the one before it
+    left, and both heads for themselves."""
+    from alphazero_amd import _lib
+    L = _lib.lib()
+    z, wl, t, tw, _ = loss_inputs(n, actions, dtype, False)
+    losses, stats = torch.zeros(3, device="cuda"), torch.zeros(8 * n, device="cuda")
+    dz, dwl = torch.zeros_like(z), torch.zeros_like(wl)
+    ups = [torch.zeros((), device="cuda") for _ in range(3)]
+    a = _lib.LossArgs(n, actions, 2, {torch.float32: 0, torch.bfloat16: 1}[dtype], z.data_ptr(), wl.data_ptr(), t.data_ptr(), tw.data_ptr(), None,
+                      losses.data_ptr(), stats.data_ptr(), *(u.data_ptr() for u in ups), dz.data_ptr(), dwl.data_ptr())
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert L.az_policy_value_loss_ready(C.byref(a)) == 1
+    for forward in range(2):
+        _lib.check(L.az_policy_value_loss_forward(C.byref(a), stream))
+        for up in ((1.0, 0.0, 0.0), (3.0, 0.0, 0.0), (3.0, 0.0, 0.0), (1.0, 0.0, 0.0), (0.0, 0.5, 1.0), (0.0, 1.0, 0.25), (1.0, 0.0, 0.0)):
+            for u, v in zip(ups, up):
+                u.fill_(v)
+            a.grads_ready = 1
+            _lib.check(L.az_policy_value_loss_backward(C.byref(a), stream))
+            got = dz.clone(), dwl.clone()
+            fresh = torch.zeros_like(z), torch.zeros_like(wl)
+            a.grads_ready, a.dpolicy, a.dwl = 0, fresh[0].data_ptr(), fresh[1].data_ptr()
+            _lib.check(L.az_policy_value_loss_backward(C.byref(a), stream))
+            a.dpolicy, a.dwl = dz.data_ptr(), dwl.data_ptr()
+            assert torch.equal(got[0], fresh[0]) and torch.equal(got[1], fresh[1]), (forward, up)
