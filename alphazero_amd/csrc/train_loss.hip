@@ -67,15 +67,20 @@ __device__ inline RowSum join_lanes(RowSum r) {
     return r;
 }
 
+// 1 / S; 0 where a row keeps nothing, or only logits of minus infinity, and has no target either.
+__device__ inline float inverse(const RowSum& r) { return r.T == 0.f && r.S == 0.f ? 0.f : 1.f / r.S; }
+
 __device__ inline void put_row(const LossParams& p, size_t at, const RowSum& r) {
     p.top[at] = r.m;
-    p.inv[at] = r.T == 0.f && r.S == 0.f ? 0.f : 1.f / r.S;
+    p.inv[at] = inverse(r);
     p.total[at] = r.T;
     p.loss[at] = r.T == 0.f && r.U == 0.f && !(r.S != r.S) ? 0.f : r.T * logf(r.S) + r.U;
 }
 
-// weight: T / S; up: upstream / rows
-__device__ inline float gradient(float z, float t, float m, float weight, float up) { return (__expf(z - m) * weight - t) * up; }
+// weight: T / S; up: upstream / rows.  (Without targets the logits do not matter: z and m may both be minus infinity.)
+__device__ inline float gradient(float z, float t, float m, float weight, float up) {
+    return ((weight == 0.f ? 0.f : __expf(z - m) * weight) - t) * up;
+}
 
 // One outcome row by one thread: two or three classes.
 template <typename T, bool GRAD>
@@ -90,7 +95,7 @@ __device__ void outcome_forward(const LossParams& p, int row) {
     }
     put_row(p, (size_t)p.n + row, r);
     if (GRAD) {
-        const float weight = 1.f / r.S * r.T, up = 1.f / (float)p.n;
+        const float weight = inverse(r) * r.T, up = 1.f / (float)p.n;
         for (int i = 0; i < p.outcomes; ++i) ((T*)p.dwl)[(size_t)row * p.outcomes + i] = (T)gradient((float)z[i], t[i], r.m, weight, up);
     }
 }
@@ -180,7 +185,7 @@ __global__ __launch_bounds__(LOSS_THREADS) void k_loss_row(const LossParams p, i
     if (row >= p.n) return;
     if (lane == 0) put_row(p, row, r);
     if (GRAD) {
-        const float weight = (r.T == 0.f && r.S == 0.f ? 0.f : 1.f / r.S) * r.T, up = 1.f / (float)p.n;
+        const float weight = inverse(r) * r.T, up = 1.f / (float)p.n;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             if ((i * GROUP + lane) * V >= p.actions) break;

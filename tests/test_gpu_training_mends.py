@@ -55,3 +55,27 @@ def test_backward_call_made_again_without_its_forward_call(dtype, n, actions):
             _lib.check(L.az_policy_value_loss_backward(C.byref(a), stream))
             a.dpolicy, a.dwl = dz.data_ptr(), dwl.data_ptr()
             assert torch.equal(got[0], fresh[0]) and torch.equal(got[1], fresh[1]), (forward, up)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("actions", [3, 192, 1500, 9000])
+@pytest.mark.parametrize("masked", [False, True])
+def test_loss_rows_of_minus_infinity_without_targets(dtype, actions, masked):
+    """A row whose kept logits are all minus infinity and whose targets are zero adds nothing, and its gradient is zero: a row
+    without a legal move whose program marks them so.  The other rows are as if it were a row without targets."""
+    from alphazero_amd import ops
+    z, wl, t, tw, mask = loss_inputs(9, actions, dtype, masked, seed=actions)
+    for row in (4, 7):
+        t[row] = 0
+        z[row] = torch.where(mask[row], torch.full_like(z[row], -math.inf), z[row]) if masked else -math.inf
+    wl[5], tw[5] = -math.inf, 0
+    z.requires_grad_(True), wl.requires_grad_(True)
+    for up in (1.0, 0.5):
+        losses = ops.policy_value_loss(z, wl, t, tw, mask)
+        got = torch.autograd.grad(losses[0], (z, wl), torch.full_like(losses[0], up))
+        want, mags, grads, grad_mags = loss_reference(z.detach(), wl.detach(), t, tw, mask, (up, 0.0, 0.0))
+        for a, b, m in zip(losses, want, mags):
+            close(a, b, m, 72 + -(-actions // 64))
+        for a, b, m in zip(got, grads, grad_mags):
+            close(a, torch.nan_to_num(b, nan=0.0), torch.nan_to_num(m, nan=0.0), 72 + -(-actions // 64))
+        assert bool((got[0][[4, 7]] == 0).all()) and bool((got[1][5] == 0).all())
