@@ -37,8 +37,19 @@ struct RowSum {
     float m, S, T, U;
 };
 
+// exp(x) of an x that is not positive, to two last places; what would be below 2^-126 is 0.  2^y of y = x / ln 2 alone is off by
+// |y| half-steps, so the rest of the product is kept and multiplied in.  (The library's expf: k_loss_row at 8192 x 4001 in
+// bfloat16 53.6 us; this one 49.5.)
+__device__ inline float exp_below(float x) {
+    constexpr float INV_LN2 = (float)M_LOG2E, INV_LN2_REST = (float)(M_LOG2E - (double)INV_LN2);
+    x = x < -150.f ? -150.f : x;               // (minus infinity has no rest; a NaN stays one)
+    const float y = x * INV_LN2, rest = __builtin_fmaf(x, INV_LN2_REST, __builtin_fmaf(x, INV_LN2, -y));
+    const float e = __builtin_amdgcn_exp2f(y);
+    return __builtin_fmaf(e, rest * (float)M_LN2, e);
+}
+
 __device__ inline void absorb(RowSum& r, float z, float t) {          // z <= r.m
-    if (z != -INFINITY) r.S += __expf(z - r.m);
+    if (z != -INFINITY) r.S += exp_below(z - r.m);
     r.T += t;
     if (t != 0.f) r.U += t * (z == -INFINITY ? INFINITY : r.m - z);
 }
@@ -46,7 +57,7 @@ __device__ inline void absorb(RowSum& r, float z, float t) {          // z <= r.
 __device__ inline void raise(RowSum& r, float m) {
     if (m > r.m) {
         if (r.m != -INFINITY) {
-            r.S *= __expf(r.m - m);
+            r.S *= exp_below(r.m - m);
             r.U += (m - r.m) * r.T;
         }
         r.m = m;
@@ -79,7 +90,7 @@ __device__ inline void put_row(const LossParams& p, size_t at, const RowSum& r) 
 
 // weight: T / S; up: upstream / rows.  (Without targets the logits do not matter: z and m may both be minus infinity.)
 __device__ inline float gradient(float z, float t, float m, float weight, float up) {
-    return ((weight == 0.f ? 0.f : __expf(z - m) * weight) - t) * up;
+    return ((weight == 0.f ? 0.f : exp_below(z - m) * weight) - t) * up;
 }
 
 // One outcome row by one thread: two or three classes.

@@ -79,3 +79,24 @@ def test_loss_rows_of_minus_infinity_without_targets(dtype, actions, masked):
         for a, b, m in zip(got, grads, grad_mags):
             close(a, torch.nan_to_num(b, nan=0.0), torch.nan_to_num(m, nan=0.0), 72 + -(-actions // 64))
         assert bool((got[0][[4, 7]] == 0).all()) and bool((got[1][5] == 0).all())
+
+
+@pytest.mark.parametrize("actions", [192, 4001, 9000])
+def test_probabilities_of_far_logits(actions):
+    """Logits down to 76 below the largest, without targets of their own: their gradient is exp(z - m) / S * T * (upstream / n),
+    where z - m is exact (a multiple of 2^-3): 8 half-steps for the operations, and for S one for each of a thread's values (8 in
+    a row of up to 512, actions / 256 in longer ones) and 8 for the sum over the threads.  An exponential that multiplies by
+    1 / ln 2 and rounds is off by up to 44 of them there."""
+    from alphazero_amd import ops
+    z = torch.zeros(4, actions, device="cuda")
+    z[:, 1:] = -(torch.arange(1, actions, device="cuda").float() / 8) % 76 - 76
+    t = torch.zeros(4, actions, device="cuda")
+    t[:, 0] = 1
+    z.requires_grad_(True)
+    wl = torch.zeros(4, 2, device="cuda")
+    for up in (1.0, 0.25):
+        loss = ops.policy_value_loss(z, wl, t, torch.full((4, 2), 0.5, device="cuda"))[0]
+        got, = torch.autograd.grad(loss, z, torch.full_like(loss, up))
+        # (on the host: the GPU's own float64 softmax of rows over 1024 is off by 60 of these steps)
+        want = torch.softmax(z.detach().cpu().double(), 1)[:, 1:].cuda() / 4 * up
+        assert float(((got[:, 1:].double() - want).abs() / want).max()) <= (24 + actions // 256) * 2.0 ** -24
