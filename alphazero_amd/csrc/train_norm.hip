@@ -7,7 +7,7 @@
 // Forward: one pass over x takes the mean and the centred sum of squares of every board and channel ("row"); from these
 // come the batch's statistics and the squeeze q, so x is read once more only, for out = relu(A x + B (+ residual)) with
 // A, B per row (gated) or per channel (plain).
-// Backward, with gm = grad where out > 0:  per row S1 = sum gm, S2 = sum gm xc.  The gate's gradients need only these:
+// Backward, with gm = grad where out > 0 (or out is a NaN):  per row S1 = sum gm, S2 = sum gm xc.  The gate's gradients need only these:
 //   dw = sigmoid(w) (1 - sigmoid(w)) (weight / s S2 + bias S1),  db = S1,  dh = (fc2^T (dw, db)) [h > 0],  dq = fc1^T dh
 //   dy = gm sigmoid(w) + dq / hw,   dbias = sum dy,   dweight = sum dy xc / s
 //   dx = weight / s (dy - dbias / m - xc / s dweight / m)  with m = n hw;  dresidual = gm
@@ -224,13 +224,13 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_stats(const T* __restrict_
     }
 }
 
-// relu of v, and which of its values are positive
+// relu of v, and where it lets the gradient through: where the value is positive, or a NaN (as torch's does)
 template <typename F>
 __device__ inline uint32_t relu_bits(F& v) {
     uint32_t bits = 0;
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(F) / 4); ++i) {
-        bits |= (v[i] > 0.f ? 1u : 0u) << i;
+        bits |= (v[i] <= 0.f ? 0u : 1u) << i;
         v[i] = not_below_zero(v[i]);
     }
     return bits;
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_apply(const T* __restrict
         uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            bits |= (v[i] > 0.f ? 1u : 0u) << i;
+            bits |= (v[i] <= 0.f ? 0u : 1u) << i;
             v[i] = not_below_zero(v[i]);
         }
         store_piece<FULL>(out + at, v, l.left);
@@ -899,7 +899,7 @@ __global__ __launch_bounds__(GATE_THREADS) void k_gate_backward(const NormParams
         for (int r = 0; r < GATE_ROWS; ++r) h[r] = p.h[board(r) * p.hidden + k];
 #pragma unroll
         for (int r = 0; r < GATE_ROWS; ++r) {
-            if (!(h[r] > 0.f)) s[r] = 0.f;
+            if (h[r] <= 0.f) s[r] = 0.f;
             if (r < rows) p.dh[(n0 + r) * p.hidden + k] = s[r];
         }
         dh[k] = s;
@@ -1209,7 +1209,7 @@ __global__ __launch_bounds__(THREADS) void k_channel_backward(const T* __restric
         const auto g = widen<T>(gr[i]);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const float xc = v[k] - m, gm = q.counts(own, k) && __builtin_fmaf(xc, scale, bias) > 0.f ? g[k] : 0.f;
+            const float xc = v[k] - m, gm = q.counts(own, k) && !(__builtin_fmaf(xc, scale, bias) <= 0.f) ? g[k] : 0.f;
             s1 += gm;
             s2 += gm * xc;
         }
@@ -1233,7 +1233,7 @@ __global__ __launch_bounds__(THREADS) void k_channel_backward(const T* __restric
         auto g = widen<T>(gr[i]);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const float xc = v[k] - m, gm = __builtin_fmaf(xc, scale, bias) > 0.f ? g[k] : 0.f;
+            const float xc = v[k] - m, gm = __builtin_fmaf(xc, scale, bias) <= 0.f ? 0.f : g[k];
             g[k] = gm * scale + (xc * b + d);
         }
         if (q.there(i)) store_raw(dx + q.place(p, i), g);

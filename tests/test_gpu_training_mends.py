@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_training_ops import DTYPES, close, loss_inputs, loss_reference
+from test_gpu_training_ops import DTYPES, close, loss_inputs, loss_reference, norm_inputs, norm_reference, run_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,36 @@ def test_probabilities_of_far_logits(actions):
         # (on the host: the GPU's own float64 softmax of rows over 1024 is off by 60 of these steps)
         want = torch.softmax(z.detach().cpu().double(), 1)[:, 1:].cuda() / 4 * up
         assert float(((got[:, 1:].double() - want).abs() / want).max()) <= (24 + actions // 256) * 2.0 ** -24
+
+
+# ----------------------------------------------------------------------------------------------- the norms
+LAYOUTS = pytest.mark.parametrize("layout", [torch.contiguous_format, torch.channels_last], ids=["nchw", "nhwc"])
+# one for each way that a row is read: a channel in a workgroup's registers, whole and moved pieces, rounds, less than a piece
+ROWS = [(6, 5, 8, 8), (2100, 3, 8, 8), (1200, 7, 9, 9), (3, 3, 120, 151), (1200, 6, 1, 3), (60, 24, 19, 19)]
+
+
+@pytest.mark.parametrize("n, c, h, w", ROWS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@LAYOUTS
+def test_norms_pass_the_gradient_where_the_output_is_nan(n, c, h, w, dtype, layout):
+    """As torch's ReLU does.  What makes the output NaN without being in a sum is the residual, or a plain norm's bias: every
+    gradient is the one of an output that is far above zero there, bit for bit."""
+    for hidden in (0, 3):
+        t = norm_inputs(n, c, h, w, hidden, dtype, layout, seed=n)
+        runs = []
+        if hidden:
+            t["grad"] = t["grad"].clone(memory_format=torch.preserve_format)
+            t["grad"][:, 1, 0] = 0.01
+        for value in (math.nan, 1e4):
+            u = dict(t)
+            if hidden:
+                u["residual"] = t["residual"].clone(memory_format=torch.preserve_format)
+                u["residual"][:, 1, 0] = value
+            else:
+                u["bias"] = t["bias"].clone()
+                u["bias"][1] = value
+            runs.append(run_norm(u))
+        assert bool(torch.isnan(runs[0]["out"][:, 1, 0]).all())
+        for name in set(runs[0]) - {"out"}:
+            assert torch.equal(runs[0][name], runs[1][name]), (hidden, name)
+        assert not hidden or torch.equal(runs[0]["residual"][:, 1, 0], t["grad"][:, 1, 0])
