@@ -396,7 +396,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_apply(const T* __rest
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 if (!GATED) g[i] = bits[k] >> i & 1 ? g[i] : 0.f;
-                g[i] = g[i] * a + ((v[i] - mean) * b + d);
+                g[i] = g[i] * a + (p.training ? (v[i] - mean) * b + d : d);
             }
             if (r.has_piece(p)) store_raw(dx + r.row(p, k) * p.hw + r.off, g);
         }
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_apply(const T* __rest
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     if (!GATED) g[i] = bits >> i & 1 ? g[i] : 0.f;
-                    g[i] = g[i] * a + ((v[i] - mean) * b + d);
+                    g[i] = g[i] * a + (p.training ? (v[i] - mean) * b + d : d);
                 }
                 store_piece<FULL>(dx + at + j * V, g, left);
             });
@@ -602,7 +602,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_apply(const T* __res
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             if (!GATED) g[i] = bits >> i & 1 ? g[i] : 0.f;
-            g[i] = g[i] * a[i] + ((v[i] - mean[i]) * b[i] + d[i]);
+            g[i] = g[i] * a[i] + (p.training ? (v[i] - mean[i]) * b[i] + d[i] : d[i]);
         }
         store_piece<FULL>(dx + at, g, l.left);
     }
@@ -692,7 +692,8 @@ __global__ __launch_bounds__(CHANNELS * LINES) void k_channel_stats(const NormPa
     if (p.num_batches && p.training && blockIdx.x == 0 && threadIdx.x == 0) *p.num_batches += 1;
 }
 
-// dy's channel sums, and with them what the last pass needs: dx = ca gm (gate) + (x - mean) cb + cd (+ ca dq / hw)
+// dy's channel sums, and with them what the last pass needs: dx = ca gm (gate) + (x - mean) cb + cd (+ ca dq / hw), without
+// cb and cd where the statistics are the running ones (not with zeros: x may be infinite)
 __device__ inline void channel_grads(const NormParams& p, int block) {
     const int c = block * CHANNELS + threadIdx.x % CHANNELS;
     const bool mine = threadIdx.x < CHANNELS && c < p.c;
@@ -1226,7 +1227,7 @@ __global__ __launch_bounds__(THREADS) void k_channel_backward(const T* __restric
         p.dbias[c] = (float)sums[0];
         p.dweight[c] = (float)(sums[1] * inv);
     }
-    const float b = p.training ? (float)(-scale * inv * inv * (sums[1] * p.per_count)) : 0.f, d = p.training ? (float)(-scale * (sums[0] * p.per_count)) : 0.f;
+    const float b = (float)(-scale * inv * inv * (sums[1] * p.per_count)), d = (float)(-scale * (sums[0] * p.per_count));
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
         const auto v = widen<T>(raw[i]);
@@ -1234,7 +1235,7 @@ __global__ __launch_bounds__(THREADS) void k_channel_backward(const T* __restric
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const float xc = v[k] - m, gm = __builtin_fmaf(xc, scale, bias) <= 0.f ? 0.f : g[k];
-            g[k] = gm * scale + (xc * b + d);
+            g[k] = gm * scale + (p.training ? xc * b + d : 0.f);
         }
         if (q.there(i)) store_raw(dx + q.place(p, i), g);
     }

@@ -133,3 +133,25 @@ def test_norms_pass_the_gradient_where_the_output_is_nan(n, c, h, w, dtype, layo
         for name in set(runs[0]) - {"out"}:
             assert torch.equal(runs[0][name], runs[1][name]), (hidden, name)
         assert not hidden or torch.equal(runs[0]["residual"][:, 1, 0], t["grad"][:, 1, 0])
+
+
+@pytest.mark.parametrize("n, c, h, w", ROWS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@LAYOUTS
+def test_norms_with_running_statistics_and_an_infinite_value(n, c, h, w, dtype, layout):
+    """Every value stands for itself there: a gradient of x is weight / s times the one that arrives, infinite or NaN x or not, bit
+    for bit that of a large one, and so are all gradients of the other channels."""
+    t = norm_inputs(n, c, h, w, 0, dtype, layout, seed=n + 1, training=False)
+    t["weight"] = t["weight"].abs() + 0.1
+    t["grad"] = t["grad"].clone(memory_format=torch.preserve_format)
+    t["grad"][:, 1, 0] = 0.01
+    runs = []
+    for value in (1e4, math.inf, math.nan):
+        x = t["x"].clone(memory_format=torch.preserve_format)
+        x[:, 1, 0] = value
+        runs.append(run_norm({**t, "x": x}, training=False))
+    others = [i for i in range(c) if i != 1]
+    for got in runs[1:]:
+        assert not bool(torch.isfinite(got["out"][:, 1, 0]).any())
+        assert torch.equal(got["x"], runs[0]["x"]) and torch.equal(got["bias"], runs[0]["bias"])
+        assert torch.equal(got["weight"][others], runs[0]["weight"][others]) and not bool(torch.isfinite(got["weight"][1]))
