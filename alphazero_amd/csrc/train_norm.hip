@@ -15,9 +15,10 @@
 //
 // What bounds it: memory (the arithmetic is a handful of operations per value).  The plain form reads or writes 7
 // activations, the gated one 10, of which 4 and 6 could not be avoided by any form: x and the gradient are needed again
-// once the batch's sums are known.  A plain norm whose channels fit a workgroup's registers needs the 4.  Whether out > 0 is kept as a byte per 16 bytes of x.  Statistics are taken about
-// the row's own mean (or, in rows longer than 64 pieces, a value of the row), then joined as centred sums in 64 bits: no
-// difference of large squares anywhere.
+// once the batch's sums are known.  A plain norm whose channels fit a workgroup's registers needs the 4.  Whether out > 0 is kept as a byte per 16 bytes of x.  Statistics are means and centred
+// sums of a row (about its own mean, or joined piece by piece in long rows and channels-last), so that no square of a distance
+// from somewhere else is taken off again; over the chunks of boards they are joined in 64 bits, where the squares of the
+// means may be subtracted.
 // Measured, forward and backward: at 4096 x 256 x 64 in bfloat16 (134 MB a tensor) 294 us, of which the four passes over
 // activations take 239 (1.34 GB: 5.6 TB/s; a copy of 1 GiB reaches 5.1) and the gate and the channel sums 55; at
 // 1024 x 128 x 64 in float32 83 us (61 and 22); a plain norm at 1024 x 128 x 64 in bfloat16 30 us.
@@ -156,6 +157,19 @@ template <typename T> __device__ inline void store_raw(T* p, typename Pack<T>::f
     *(typename Pack<T>::loose*)p = __builtin_convertvector(v, typename Pack<T>::raw);
 }
 
+// Mean and centred sum of some values, to which others' are joined: all terms are squares, so nothing cancels whatever the
+// values' order.  (The reciprocal is approximate: a mean that is off by d adds count d^2 only.)
+struct Centred {
+    float mean = 0.f, m2 = 0.f, count = 0.f;
+    __device__ void join(float other, float other_m2, float others) {
+        const float d = other - mean, before = count;
+        count += others;
+        const float share = others * __builtin_amdgcn_rcpf(count);
+        mean += d * share;
+        m2 += other_m2 + d * d * before * share;
+    }
+};
+
 // Mean and centred sum of a board's values, joined to a chunk's.
 struct ChunkStats {
     float mean = 0.f, m2 = 0.f, boards = 0.f;
@@ -200,21 +214,25 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_stats(const T* __restrict_
             for (int k = 0; k < BOARDS_AT_ONCE && r.board(k) < p.n; ++k) {
                 const T* xr = x + r.row(p, k) * p.hw;
                 const float first = (float)xr[0];
-                float s = 0.f, ss = 0.f;
+                Centred own;                 // of the lane's values less the row's first
                 over_pieces<L, V>(p, r.lane, [&](int j, int left, auto whole) {
                     const auto v = load_piece<decltype(whole)::value>(xr + j * V, left);
+                    const float count = (float)(left < V ? left : V);
+                    float s = 0.f, ss = 0.f;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) s += i < left ? v[i] - first : 0.f;
+                    const float mean = s / count;
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        const float d = i < left ? v[i] - first : 0.f;
-                        s += d;
+                        const float d = i < left ? v[i] - first - mean : 0.f;
                         ss += d * d;
                     }
+                    own.join(mean, ss, count);
                 });
-                s = lane_sum<L>(s);
-                ss = lane_sum<L>(ss);
-                const float mean = first + s / hw;
+                const float about = lane_sum<L>(own.count * own.mean) / hw, d = own.mean - about;
+                const float ss = lane_sum<L>(own.m2 + own.count * d * d), mean = first + about;
                 if (GATED && r.lane == 0) p.board_mean[r.row(p, k)] = mean;
-                chunk.join(mean, not_below_zero(ss - s * s / hw), hw);
+                chunk.join(mean, ss, hw);
             }
         }
     }
@@ -459,9 +477,10 @@ __device__ inline F load_channels(const float* p, int left) {
     return r;
 }
 
-// Sums over the places; out(c, a, b) for each of the workgroup's channels.
+// The threads' values of one channel through the LDS; out(c, a, b, stride) for each of the workgroup's channels: thread ty's
+// are a[ty * stride] and b[ty * stride].
 template <int V, typename F, typename Out>
-__device__ inline void add_places(F a, F b, const Lanes& l, const NormParams& p, int wide, Out&& out) {
+__device__ inline void over_places(F a, F b, const Lanes& l, const NormParams& p, int wide, Out&& out) {
     __shared__ float red[2][NORM_THREADS * V];
     if (l.ty < l.step) {
 #pragma unroll
@@ -475,14 +494,21 @@ __device__ inline void add_places(F a, F b, const Lanes& l, const NormParams& p,
     for (int i = threadIdx.x; i < wide * V; i += NORM_THREADS) {
         // channel of the i-th value: the last piece is moved back
         const int piece = c0 + i / V * V, c = (p.c >= V && piece > p.c - V && piece < p.c ? p.c - V : piece) + i % V;
-        if (c >= p.c) continue;
+        if (c < p.c) out(c, red[0] + i, red[1] + i, wide * V);
+    }
+}
+
+// Sums over the places; out(c, a, b) for each of the workgroup's channels.
+template <int V, typename F, typename Out>
+__device__ inline void add_places(F a, F b, const Lanes& l, const NormParams& p, int wide, Out&& out) {
+    over_places<V>(a, b, l, p, wide, [&](int c, const float* u, const float* v, int stride) {
         float s = 0.f, ss = 0.f;
         for (int y = 0; y < l.step; ++y) {
-            s += red[0][y * wide * V + i];
-            ss += red[1][y * wide * V + i];
+            s += u[y * stride];
+            ss += v[y * stride];
         }
         out(c, s, ss);
-    }
+    });
 }
 
 template <typename T, bool FULL, bool GATED>
@@ -491,24 +517,38 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_stats(const T* __restrict
     typedef typename Pack<T>::f32 F;
     const Lanes l = lanes_of<T>(p, wide);
     const T* xb = x + (size_t)blockIdx.x * p.hw * p.c;
-    F s, ss;
+    F mean, m2;                              // of the thread's values less the board's first (one by one as in Centred)
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = ss[i] = 0.f;
+    for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.f;
     if (l.on) {
         const F first = load_piece<FULL>(xb + l.c, l.left);
+        float count = 0.f;
 #pragma unroll 4
         for (int y = l.ty; y < p.hw; y += l.step) {
-            const F d = load_piece<FULL>(xb + (size_t)y * p.c + l.c, l.left) - first;
-            s += d;
-            ss += d * d;
+            const F v = load_piece<FULL>(xb + (size_t)y * p.c + l.c, l.left) - first, d = v - mean;
+            count += 1.f;
+            mean += d * __builtin_amdgcn_rcpf(count);
+            m2 += d * (v - mean);
         }
     }
-    add_places<V>(s, ss, l, p, wide, [&](int c, float a, float b) {
-        const float mean = (float)xb[c] + a / (float)p.hw;
+    const float hw = (float)p.hw, each = (float)(p.hw / l.step);
+    const int more = p.hw % l.step;          // threads with a place more than the others
+    over_places<V>(mean, m2, l, p, wide, [&](int c, const float* means, const float* m2s, int stride) {
+        const auto count = [&](int y) { return y < more ? each + 1.f : each; };
+        float s = 0.f, ss = 0.f;
+#pragma unroll 8
+        for (int y = 0; y < l.step; ++y) s += count(y) * means[y * stride];
+        const float about = s / hw;
+#pragma unroll 8
+        for (int y = 0; y < l.step; ++y) {
+            const float d = means[y * stride] - about;
+            ss += m2s[y * stride] + count(y) * d * d;
+        }
+        const float mean = (float)xb[c] + about;
         const size_t row = (size_t)blockIdx.x * p.c + c;
         if (GATED) p.board_mean[row] = mean;
         p.part_a[row] = mean;
-        p.part_b[row] = not_below_zero(b - a * a / (float)p.hw);
+        p.part_b[row] = ss;
     });
 }
 

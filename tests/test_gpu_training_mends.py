@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_training_ops import DTYPES, close, loss_inputs, loss_reference, norm_inputs, norm_reference, run_norm
+from test_gpu_training_ops import DTYPES, check_norm, close, loss_inputs, loss_reference, norm_inputs, norm_reference, run_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +155,24 @@ def test_norms_with_running_statistics_and_an_infinite_value(n, c, h, w, dtype, 
         assert not bool(torch.isfinite(got["out"][:, 1, 0]).any())
         assert torch.equal(got["x"], runs[0]["x"]) and torch.equal(got["bias"], runs[0]["bias"])
         assert torch.equal(got["weight"][others], runs[0]["weight"][others]) and not bool(torch.isfinite(got["weight"][1]))
+
+
+@pytest.mark.parametrize("n, c, h, w", [(33, 12, 19, 19), (3, 9, 64, 64), (2, 3, 256, 256), (300, 5, 1, 3), (9, 300, 7, 9), (2100, 3, 8, 8), (20, 6, 8, 8)])
+@pytest.mark.parametrize("off", [100.0, 1000.0])
+@LAYOUTS
+def test_norm_statistics_beside_an_outlier_at_the_first_place(n, c, h, w, off, layout):
+    """Each board's first place lies far from the rest.  Centred sums add squares only, so the variance is off by one half-step
+    for each value that a thread adds (a quarter of the places at most) and 64 for the joins: not by the squares of the distances
+    to that place, which are hw times as large together."""
+    for hidden in (0, 2):
+        t = norm_inputs(n, c, h, w, hidden, torch.float32, layout, seed=n)
+        t["x"][:, :, 0, 0] += off
+        # (gradients are compared where the ReLU's border is not near, as in norm_inputs)
+        _, pre, hid = norm_reference(t, True)
+        t["grad"] = (t["grad"] * (pre.abs() > 1e-3 * off)).contiguous(memory_format=layout)
+        if hidden:
+            t["grad"] = (t["grad"] * (hid.abs() > 1e-3).all(1)[:, None, None, None]).contiguous(memory_format=layout)
+        got = check_norm(t)
+        ref, _, _ = norm_reference(t, True)
+        want = ref["running_var"][0]
+        assert float(((got["running_var"] - want).abs() / want).max()) <= (64 + h * w // 4) * 2.0 ** -24, hidden
