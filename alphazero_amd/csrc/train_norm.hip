@@ -5,8 +5,8 @@
 //   y = weight xc / s + bias                                          plain:  out = relu(y)
 //   q = mean_hw y,  h = relu(fc1 q + b1),  (w, b) = fc2 h + b2        gated:  out = relu(y sigmoid(w) + b + residual)
 // Forward: one pass over x takes the mean and the centred sum of squares of every board and channel ("row"); from these
-// come the batch's statistics and the squeeze q, so x is read once more only, for out = relu(A x + B (+ residual)) with
-// A, B per row (gated) or per channel (plain).
+// come the batch's statistics and the squeeze q, so x is read once more only, for out = relu(A xc + B (+ residual)) with
+// A, B per row (gated) or per channel (plain): xc first, so that what mu and x have in common is gone before anything is rounded.
 // Backward, with gm = grad where out > 0 (or out is a NaN):  per row S1 = sum gm, S2 = sum gm xc.  The gate's gradients need only these:
 //   dw = sigmoid(w) (1 - sigmoid(w)) (weight / s S2 + bias S1),  db = S1,  dh = (fc2^T (dw, db)) [h > 0],  dq = fc1^T dh
 //   dy = gm sigmoid(w) + dq / hw,   dbias = sum dy,   dweight = sum dy xc / s
@@ -263,6 +263,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_apply(const T* __restrict_
     if constexpr (FIT != LOOP) {
         typename Pack<T>::raw raw[BOARDS_AT_ONCE], res[BOARDS_AT_ONCE];
         float A[BOARDS_AT_ONCE], B[BOARDS_AT_ONCE];
+        const float mean = p.mean[r.c];
 #pragma unroll
         for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
             const size_t row = r.row(p, k);
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_apply(const T* __restrict_
         for (int k = 0; k < BOARDS_AT_ONCE; ++k) {
             if (r.board(k) >= p.n) return;
             const size_t row = r.row(p, k);
-            auto v = widen<T>(raw[k]) * A[k] + B[k];
+            auto v = (widen<T>(raw[k]) - mean) * A[k] + B[k];
             if (GATED) v += widen<T>(res[k]);
             const uint32_t bits = relu_bits(v);
             store_raw(out + row * p.hw + r.off, v);
@@ -284,10 +285,10 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_apply(const T* __restrict_
     } else {
         for (int k = 0; k < BOARDS_AT_ONCE && r.board(k) < p.n; ++k) {
             const size_t row = r.row(p, k), at = row * p.hw;
-            const float A = p.A[GATED ? row : r.c], B = p.B[GATED ? row : r.c];
+            const float A = p.A[GATED ? row : r.c], B = p.B[GATED ? row : r.c], mean = p.mean[r.c];
             over_pieces<L, V>(p, r.lane, [&](int j, int left, auto whole) {
                 constexpr bool FULL = decltype(whole)::value;
-                auto v = load_piece<FULL>(x + at + j * V, left) * A + B;
+                auto v = (load_piece<FULL>(x + at + j * V, left) - mean) * A + B;
                 if (GATED) v += load_piece<FULL>(residual + at + j * V, left);
                 const uint32_t bits = relu_bits(v);
                 store_piece<FULL>(out + at + j * V, v, left);
@@ -561,12 +562,12 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_apply(const T* __restrict
     if (!l.on) return;
     const uint32_t n = backwards(blockIdx.x, gridDim.x);
     const size_t q = (GATED ? (size_t)n * p.c : 0) + l.c;
-    const F A = load_channels<F>(p.A + q, l.left), B = load_channels<F>(p.B + q, l.left);
+    const F A = load_channels<F>(p.A + q, l.left), B = load_channels<F>(p.B + q, l.left), mean = load_channels<F>(p.mean + l.c, l.left);
     const size_t board = (size_t)n * p.hw;
 #pragma unroll 4
     for (int y = l.ty; y < p.hw; y += l.step) {
         const size_t at = (board + y) * p.c + l.c;
-        F v = load_piece<FULL>(x + at, l.left) * A + B;
+        F v = (load_piece<FULL>(x + at, l.left) - mean) * A + B;
         if (GATED) v += load_piece<FULL>(residual + at, l.left);
         uint32_t bits = 0;
 #pragma unroll
@@ -726,7 +727,7 @@ __global__ __launch_bounds__(CHANNELS * LINES) void k_channel_stats(const NormPa
         p.inv[c] = inv;
         if (!p.hidden) {
             p.A[c] = weight * inv;
-            p.B[c] = bias - weight * inv * m;
+            p.B[c] = bias;
         }
     }
     if (p.num_batches && p.training && blockIdx.x == 0 && threadIdx.x == 0) *p.num_batches += 1;
@@ -892,7 +893,7 @@ __global__ __launch_bounds__(GATE_THREADS) void k_gate_forward(const NormParams 
     rows_times(p.w2, p.b2, 2 * p.c, p.hidden, h, [&](int j, const f32x4 s) { e[j] = s; });
     __syncthreads();
     for (int c = threadIdx.x; c < p.c; c += GATE_THREADS) {
-        const float scale = p.weight[c] * p.inv[c], shift = p.bias[c] - scale * p.mean[c];
+        const float scale = p.weight[c] * p.inv[c], bias = p.bias[c];
         const f32x4 w = e[c], b = e[p.c + c];
 #pragma unroll
         for (int r = 0; r < GATE_ROWS; ++r)
@@ -901,7 +902,7 @@ __global__ __launch_bounds__(GATE_THREADS) void k_gate_forward(const NormParams 
                 const float gate = 1.f / (1.f + expf(-w[r]));
                 p.gate[row] = gate;
                 p.A[row] = scale * gate;
-                p.B[row] = shift * gate + b[r];
+                p.B[row] = bias * gate + b[r];
             }
     }
 }
@@ -1009,8 +1010,8 @@ __device__ inline void weight_tile(const NormParams& p, int job) {
     // (a lane past the end of a factor reads its last value; what comes of it is not joined)
     const int i = i0 + at < t.m ? i0 + at : t.m - 1, j = j0 + at < t.k ? j0 + at : t.k - 1;
     const float *left = (second ? p.de : p.dh) + i, *right = (second ? p.h : p.board_mean) + j;
-    // fc1's right factor: q = mean * scale + shift
-    const float scale = second ? 1.f : p.weight[j] * p.inv[j], shift = second ? 0.f : p.bias[j] - scale * p.mean[j];
+    // fc1's right factor: q = (mean over the board - mean) * scale + shift
+    const float scale = second ? 1.f : p.weight[j] * p.inv[j], shift = second ? 0.f : p.bias[j], mean = second ? 0.f : p.mean[j];
     typedef float f32x16 __attribute__((ext_vector_type(16)));
     f32x16 acc = 0.f;
     float bias = 0.f;
@@ -1027,7 +1028,7 @@ __device__ inline void weight_tile(const NormParams& p, int job) {
         for (int u = 0; u < TILE_AHEAD; ++u) {
             const float w = n + 2 * TILE_WAVES * u + second_board < to ? a[u] : 0.f;
             bias += w;
-            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(w, b[u] * scale + shift, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(w, (b[u] - mean) * scale + shift, acc, 0, 0, 0);
         }
     }
     bias += __shfl_xor(bias, 32);

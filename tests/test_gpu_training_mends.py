@@ -176,3 +176,36 @@ def test_norm_statistics_beside_an_outlier_at_the_first_place(n, c, h, w, off, l
         ref, _, _ = norm_reference(t, True)
         want = ref["running_var"][0]
         assert float(((got["running_var"] - want).abs() / want).max()) <= (64 + h * w // 4) * 2.0 ** -24, hidden
+
+
+@pytest.mark.parametrize("n, c, h, w", ROWS + [(33, 40, 64, 64)])
+@LAYOUTS
+def test_norms_far_from_zero(n, c, h, w, layout):
+    """Values 900 standard deviations from zero.  The mean is held in float32, off by half a step, 2^-15; that times weight / s is
+    what the output may be off by, beside 8 half-steps of what is added up: x - mean is exact.  Behind it stand the means of the
+    n boards, in float32 too: one that is a value of the board plus a small rest is off by up to half a step more, all of them
+    the same way at worst; one that is a sum of 64 to 361 values over 900 by some 1.6 half-steps (one standard deviation: the
+    last additions 1, 1/2, 1/4.. of a half-step's square, and the division), so that n >= 60 of them have a mean within
+    5 * 1.6 / sqrt(n) half-steps, at most 1.  A gate hears of the board's means, which are sums of hw values: 12 steps of 900 each, through the
+    absolute values of its weights."""
+    for hidden in (0, 3):
+        t = norm_inputs(n, c, h, w, hidden, torch.float32, layout, seed=n)
+        t["x"] = (900.0 + torch.randn(n, c, h, w, device="cuda", generator=torch.Generator("cuda").manual_seed(n))).contiguous(memory_format=layout)
+        ref, pre, hid = norm_reference(t, True)
+        keep = pre.abs() > 1e-2
+        if hidden:
+            keep &= (hid.abs() > 1e-2).all(1)[:, None, None, None]
+        t["grad"] = (t["grad"] * keep).contiguous(memory_format=layout)
+        got = check_norm(t)
+        ref, pre, _ = norm_reference(t, True)
+        var = ref["running_var"][0]
+        assert float(((got["running_var"] - var).abs() / var).max()) <= (64 + h * w // 4) * 2.0 ** -24, hidden
+        scale = (t["weight"].double() / (t["x"].double().var((0, 2, 3), correction=0) + 1e-5).sqrt()).abs()
+        bound = (1 + min(1.0, 8 / math.sqrt(n))) * 2.0 ** -15 * scale[:, None, None] + 8 * 2.0 ** -24 * (5 * scale[:, None, None] + t["bias"].double().abs()[:, None, None] + pre.abs())
+        if hidden:
+            q = 12 * 2.0 ** -24 * 900 * scale
+            inner = t["fc1_weight"].double().abs() @ q
+            e = t["fc2_weight"].double().abs() @ inner
+            bound = bound + ((5 * scale + t["bias"].double().abs()) * e[:c] / 4 + e[c:])[:, None, None]
+        worst = float(((got["out"] - ref["out"][0]).abs() / bound).max())
+        assert worst <= 1.0, (hidden, worst)
