@@ -388,7 +388,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_apply(const T* __rest
     }
     const RowPlace<T, L, FIT> r(p, grid, backwards(blockIdx.x - joins, grid.blocks));
     if (!r.on || r.n_first >= p.n) return;
-    const float mean = p.mean[r.c], b = p.cb[r.c], ca = p.ca[r.c], cd = p.cd[r.c], per_place = ca / (float)p.hw;
+    const float mean = p.mean[r.c], inv = p.inv[r.c], b = p.cb[r.c], ca = p.ca[r.c], cd = p.cd[r.c], per_place = ca / (float)p.hw;
     if constexpr (FIT != LOOP) {
         typename Pack<T>::raw raw[BOARDS_AT_ONCE], gr[BOARDS_AT_ONCE];
         float gate[BOARDS_AT_ONCE], dq[BOARDS_AT_ONCE];
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_apply(const T* __rest
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 if (!GATED) g[i] = bits[k] >> i & 1 ? g[i] : 0.f;
-                g[i] = g[i] * a + (p.training ? (v[i] - mean) * b + d : d);
+                g[i] = g[i] * a + (p.training ? (v[i] - mean) * inv * b + d : d);
             }
             if (r.has_piece(p)) store_raw(dx + r.row(p, k) * p.hw + r.off, g);
         }
@@ -431,7 +431,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_row_grad_apply(const T* __rest
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     if (!GATED) g[i] = bits >> i & 1 ? g[i] : 0.f;
-                    g[i] = g[i] * a + (p.training ? (v[i] - mean) * b + d : d);
+                    g[i] = g[i] * a + (p.training ? (v[i] - mean) * inv * b + d : d);
                 }
                 store_piece<FULL>(dx + at + j * V, g, left);
             });
@@ -627,7 +627,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_apply(const T* __res
     const Lanes l = lanes_of<T>(p, wide);
     if (!l.on) return;
     const size_t row = (size_t)n * p.c + l.c;
-    const F mean = load_channels<F>(p.mean + l.c, l.left), b = load_channels<F>(p.cb + l.c, l.left);
+    const F mean = load_channels<F>(p.mean + l.c, l.left), inv = load_channels<F>(p.inv + l.c, l.left), b = load_channels<F>(p.cb + l.c, l.left);
     F a = load_channels<F>(p.ca + l.c, l.left), d = load_channels<F>(p.cd + l.c, l.left);
     if (GATED) {
         d += a * load_channels<F>(p.dq + row, l.left) / (float)p.hw;
@@ -643,7 +643,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_last_grad_apply(const T* __res
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             if (!GATED) g[i] = bits >> i & 1 ? g[i] : 0.f;
-            g[i] = g[i] * a[i] + (p.training ? (v[i] - mean[i]) * b[i] + d[i] : d[i]);
+            g[i] = g[i] * a[i] + (p.training ? (v[i] - mean[i]) * inv[i] * b[i] + d[i] : d[i]);
         }
         store_piece<FULL>(dx + at, g, l.left);
     }
@@ -733,7 +733,7 @@ __global__ __launch_bounds__(CHANNELS * LINES) void k_channel_stats(const NormPa
     if (p.num_batches && p.training && blockIdx.x == 0 && threadIdx.x == 0) *p.num_batches += 1;
 }
 
-// dy's channel sums, and with them what the last pass needs: dx = ca gm (gate) + (x - mean) cb + cd (+ ca dq / hw), without
+// dy's channel sums, and with them what the last pass needs: dx = ca gm (gate) + xc / s cb + cd (+ ca dq / hw), without
 // cb and cd where the statistics are the running ones (not with zeros: x may be infinite)
 __device__ inline void channel_grads(const NormParams& p, int block) {
     const int c = block * CHANNELS + threadIdx.x % CHANNELS;
@@ -750,7 +750,7 @@ __device__ inline void channel_grads(const NormParams& p, int block) {
         p.dbias[c] = (float)v[0];
         p.dweight[c] = (float)(v[1] * inv);
         p.ca[c] = a;
-        p.cb[c] = p.training ? (float)(-a * inv * inv * (v[1] / count)) : 0.f;
+        p.cb[c] = p.training ? (float)(-a * (v[1] * inv / count)) : 0.f;
         p.cd[c] = p.training ? (float)(-a * (v[0] / count)) : 0.f;
     }
 }
@@ -1152,6 +1152,14 @@ struct ChannelPieces {
     __device__ static bool counts(int own, int k) { return WHOLE ? own == 0 : k >= own; }
 };
 
+// 1 / sqrt(v): a root in 32 bits, and one step of Newton's in 64 (every thread needs it, and a division and a root in 64 bits
+// are slow); those where 32 bits do not hold the number (an eps of zero and a tiny variance, zero, infinity).
+__device__ inline float inverse_root(double v) {
+    if (!(v > 1e-36 && v < 1e36)) return (float)(1.0 / sqrt(v));
+    const double near = rsqrtf((float)v);
+    return (float)(near * (1.5 - 0.5 * v * near * near));
+}
+
 // WHOLE: rows are whole pieces.
 template <typename T, int THREADS, int PIECES, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void k_channel_forward(const T* __restrict__ x, T* __restrict__ out, const NormParams p) {
@@ -1211,9 +1219,7 @@ __global__ __launch_bounds__(THREADS) void k_channel_forward(const T* __restrict
         mean = p.running_mean[c];
         var = p.running_var[c];
     }
-    // a root in 32 bits, and one step of Newton's in 64: every thread needs it, and a division and a root in 64 bits are slow
-    const double under = var + p.eps, near = rsqrtf((float)under);
-    const float inv = (float)(near * (1.5 - 0.5 * under * near * near)), m = (float)mean, scale = weight * inv;
+    const float inv = inverse_root(var + p.eps), m = (float)mean, scale = weight * inv;
     if (threadIdx.x == 0) {
         p.mean[c] = m;
         p.inv[c] = inv;
@@ -1268,7 +1274,7 @@ __global__ __launch_bounds__(THREADS) void k_channel_backward(const T* __restric
         p.dbias[c] = (float)sums[0];
         p.dweight[c] = (float)(sums[1] * inv);
     }
-    const float b = (float)(-scale * inv * inv * (sums[1] * p.per_count)), d = (float)(-scale * (sums[0] * p.per_count));
+    const float b = (float)(-scale * (sums[1] * inv * p.per_count)), d = (float)(-scale * (sums[0] * p.per_count));
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
         const auto v = widen<T>(raw[i]);
@@ -1276,7 +1282,7 @@ __global__ __launch_bounds__(THREADS) void k_channel_backward(const T* __restric
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const float xc = v[k] - m, gm = __builtin_fmaf(xc, scale, bias) <= 0.f ? 0.f : g[k];
-            g[k] = gm * scale + (p.training ? xc * b + d : 0.f);
+            g[k] = gm * scale + (p.training ? xc * inv * b + d : 0.f);
         }
         if (q.there(i)) store_raw(dx + q.place(p, i), g);
     }

@@ -209,3 +209,31 @@ def test_norms_far_from_zero(n, c, h, w, layout):
             bound = bound + ((5 * scale + t["bias"].double().abs()) * e[:c] / 4 + e[c:])[:, None, None]
         worst = float(((got["out"] - ref["out"][0]).abs() / bound).max())
         assert worst <= 1.0, (hidden, worst)
+
+
+@pytest.mark.parametrize("var", [2.0 ** -132, 2.0 ** -120, 2.0 ** 126, math.inf, 0.0])
+@LAYOUTS
+def test_norms_of_variances_at_the_ends_of_the_range(var, layout):
+    """eps = 0 is allowed.  With running statistics out = relu(weight x / sqrt(var) + bias) is 8 operations; a variance of zero
+    makes x / 0, an infinite one leaves the bias.  With the batch's own, squares below 2^-126 keep 2^-149 of their size."""
+    from alphazero_amd import ops
+    gen = torch.Generator("cuda").manual_seed(4)
+    unit = torch.randn(20, 6, 8, 8, device="cuda", generator=gen)
+    w, b = torch.rand(6, device="cuda", generator=gen) + 0.5, torch.randn(6, device="cuda", generator=gen)
+    size = math.sqrt(var) if 0 < var < math.inf else 1.0
+    x = (unit * size).contiguous(memory_format=layout).requires_grad_(True)
+    mean, held = torch.zeros(6, device="cuda"), torch.full((6,), var, device="cuda")
+    out = ops.norm_act(x, w, b, mean, held, training=False, eps=0.0)
+    ch = lambda v: v.double().view(1, 6, 1, 1)                            # noqa: E731
+    y = x.detach().double() / math.sqrt(var) if var else x.detach().double() * math.inf
+    want = torch.relu(ch(w) * y + ch(b))
+    near = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(out), near)
+    assert bool(((out - want).abs() <= 8 * 2.0 ** -24 * (ch(w) * y.abs() + ch(b).abs()))[near].all())
+    if 0 < var < 1:
+        out = ops.norm_act(x, w, b, None, None, training=True, eps=0.0)
+        grad, = torch.autograd.grad(out, x, torch.full_like(out, 0.25))
+        v, m = torch.var_mean(x.detach().double(), (0, 2, 3), correction=0)
+        want = torch.relu(ch(w) * (x.detach().double() - ch(m)) / ch(v).sqrt() + ch(b))
+        assert float((out - want).abs().max()) <= (64 + 64) * 2.0 ** -24 * 10 + 2.0 ** -149 / var * 5
+        assert bool(torch.isfinite(grad).all())
