@@ -5,12 +5,12 @@
 //   g = c g (+ wd p: weight decay in the gradient)        m = b1 m + (1 - b1) g        v = b2 v + (1 - b2) g^2
 //   p = p (- lr wd p: decoupled decay) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // Every operation on the moments is rounded on its own to 32 bits (this file is built without contraction, the root is
-// correctly rounded), so they are the same numbers as the same operations in elementary tensor code, and so are the codes
-// that they become in 8 bits.  The quotient is a product with the hardware's reciprocal: one last place of the update.
+// correctly rounded, denormals too), so they are the same numbers as the same operations in elementary tensor code, and so are
+// the codes that they become in 8 bits.  The quotient is a product with the hardware's reciprocal: one last place of the update.
 //
 // What bounds it: memory.  A 32-bit step reads 16 and writes 12 bytes per weight, an 8-bit one 10 and 6; clipping reads
-// the gradients once more.  Measured: k_adam on the 20x128 network's 8.0 M weights 41 us in 32 bits (5.5 TB/s), 29 us in
-// 8 (4.4 TB/s: the codes' 80 instructions a weight are 20 us of it); on the 28 M of 20x256 in 8 bits 88 us (5.1 TB/s);
+// the gradients once more.  Measured: k_adam on the 20x128 network's 8.0 M weights 41 us in 32 bits (5.5 TB/s), 30 us in
+// 8 (4.3 TB/s; the codes' 80 instructions a weight are 20 us of it); on the 28 M of 20x256 in 8 bits 88 us (5.1 TB/s);
 // k_adam_begin 9 us with the norm of 8.0 M gradients, 5 us without.
 // Layout: a workgroup takes a piece of OPT_CHUNK elements of one tensor.  Which one is in a table that is made once, in
 // device memory; the tensors' addresses travel in the kernel arguments (OPT_TABLE tensors a launch, so that the default
@@ -154,16 +154,6 @@ __device__ inline float clip_factor(const AdamParams& a) {
     return (float)(c > 1.0 ? 1.0 : c);             // a NaN stays one
 }
 
-// Correctly rounded root of a value that is not denormal: the hardware's, off by at most a last place, and the signs of what
-// is left of v beside its two neighbours.
-__device__ inline float exact_root(float v) {
-    const float r = __builtin_amdgcn_sqrtf(v), below = __uint_as_float(__float_as_uint(r) - 1), above = __uint_as_float(__float_as_uint(r) + 1);
-    float best = r;
-    if (__builtin_fmaf(-below, r, v) <= 0.f) best = below;
-    if (__builtin_fmaf(-above, r, v) > 0.f) best = above;
-    return best;                       // (0 and infinity: the neighbours' remainders are NaN or zero)
-}
-
 // ---- moments in 8 bits -------------------------------------------------------------------------------------------
 // 256 values share a power of two that puts their largest in (224, 448]; each is an e4m3 code times it: 3 bits of
 // mantissa over 17 binades, both directions of the scaling exact.  m is held as itself, v as its root: the root is what
@@ -222,6 +212,7 @@ __device__ inline f32x4 decode(uint32_t codes, float scale) {
     return r;
 }
 
+// (A published mix of 32 bits with little bias, C. Wellons 2018: two rounds of xor-shift and multiply.)
 __device__ inline uint32_t mix32(uint32_t z) {
     z = (z ^ (z >> 16)) * 0x7FEB352Du;
     z = (z ^ (z >> 15)) * 0x846CA68Bu;
@@ -286,7 +277,7 @@ __global__ __launch_bounds__(OPT_THREADS) void k_adam(const TensorTable t, const
                     const float vk = BITS == 32 ? v[u][k] : v[u][k] * v[u][k];
                     m[u][k] = m[u][k] * a.beta1 + gk * a.one_beta1;
                     v[u][k] = vk * a.beta2 + gk * gk * a.one_beta2;
-                    root[k] = exact_root(v[u][k]);
+                    root[k] = sqrtf(v[u][k]);
                     p[u][k] = pk - m[u][k] * __builtin_amdgcn_rcpf(root[k] * f.inv_root_bias2 + a.eps) * f.step_size;
                 }
                 if (WHOLE) *(f32x4_loose*)(pp + i) = p[u];

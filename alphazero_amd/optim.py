@@ -53,7 +53,7 @@ class FusedAdam(torch.optim.Optimizer):
     Replicas of a model have to be given one seed (alphazero_amd.distributed.train_step checks that).
 
     state_dict() is torch.optim.Adam's: per parameter step, exp_avg, exp_avg_sq (float32, also with 8-bit moments, which
-    a load restores exactly), so checkpoints go both ways.  Step counters live on the GPU; a step can be captured into
+    a load restores exactly: exp_avg all of it, sqrt(v) from 2^-63 on, where its square is a normal float32), so checkpoints go both ways.  Step counters live on the GPU; a step can be captured into
     a HIP graph (learning rate and the other hyper-parameters are constants of the capture).  amsgrad, maximize,
     sparse gradients and parameter groups added after construction are refused."""
 

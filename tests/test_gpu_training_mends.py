@@ -237,3 +237,58 @@ def test_norms_of_variances_at_the_ends_of_the_range(var, layout):
         want = torch.relu(ch(w) * (x.detach().double() - ch(m)) / ch(v).sqrt() + ch(b))
         assert float((out - want).abs().max()) <= (64 + 64) * 2.0 ** -24 * 10 + 2.0 ** -149 / var * 5
         assert bool(torch.isfinite(grad).all())
+
+
+# ------------------------------------------------------------------------------------------- the optimiser
+def test_moments_of_tiny_gradients_are_those_of_elementary_operations():
+    """Every operation on the moments is one of torch's, correctly rounded, down to the smallest float32: v between 1e-45 and
+    1e-31 and its root, which shows in the codes that the root becomes.  8 bits with a random part of zero round down, so the
+    codes of a root that is a last place too small would be others: the held roots are compared with those of the same
+    operations on the host, at values whose root is a code."""
+    from alphazero_amd.optim import FusedAdam
+    # m = 0.1 g; one step from zero with beta2 = 0 and beta1 = 0: v = g * g, root = sqrt(g * g)
+    g = torch.cat([torch.logspace(-22.4, -15, 3000, dtype=torch.float64).float(), torch.tensor([2.0 ** -k for k in range(52, 75)])]).cuda()
+    p = torch.zeros_like(g).requires_grad_(True)
+    p.grad = g.clone()
+    opt = FusedAdam([p], lr=1.0, betas=(0.0, 0.0), eps=0.0)
+    opt.step()
+    v = g.cpu() * g.cpu() * torch.tensor(1.0)
+    assert torch.equal(opt.state[p]["exp_avg_sq"].cpu(), v)
+    # p = - m / root, the quotient by the hardware's reciprocal: two last places and the product's
+    root = v.double().sqrt().float()
+    live = root > 0
+    want = -(g.cpu().double() / root.double())
+    assert bool(((p.detach().cpu().double() - want).abs() <= 4 * 2.0 ** -24 * want.abs())[live].all())
+
+
+def test_codes_of_tiny_roots():
+    """In 8 bits: a root that is exactly a code stays that code whatever the random part; blocks of 2^-40 to 2^-63 times the e4m3
+    values 8 to 15 and 128 to 240, whose squares are exact in float32."""
+    from alphazero_amd.optim import FusedAdam, _decode
+    values = torch.cat([torch.arange(8, 16), torch.arange(8, 16) * 16]).double()
+    for k in range(40, 64):
+        g = (values * 2.0 ** -k).float().repeat(16).cuda()
+        p = torch.zeros_like(g).requires_grad_(True)
+        p.grad = g.clone()
+        opt = FusedAdam([p], lr=0.0, betas=(0.0, 0.0), state_bits=8)
+        opt.step()
+        held = opt.flat_state()
+        assert torch.equal(_decode(held["exp_rms"], held["exp_rms_scale"])[:256], g), k
+        assert torch.equal(_decode(held["exp_avg"], held["exp_avg_scale"])[:256], g), k
+
+
+def test_update_without_eps_does_not_depend_on_the_scale():
+    """m / sqrt(v) of gradients times a power of two: every operation is the same one, bit for bit, as long as v is a normal
+    number, 2^-124 to 2^-4 here."""
+    from alphazero_amd.optim import FusedAdam
+    gen = torch.Generator("cuda").manual_seed(6)
+    g = torch.randn(20000, device="cuda", generator=gen).abs().clamp(min=0.01) * 2.0 ** -54
+    results = []
+    for power in (0, 20, 50):
+        p = torch.zeros_like(g).requires_grad_(True)
+        opt = FusedAdam([p], lr=1.0, betas=(0.5, 0.25), eps=0.0)
+        for factor in (1.0, -0.375, 3.0):
+            p.grad = g * (factor * 2.0 ** power)
+            opt.step()
+        results.append(p.detach())
+    assert torch.equal(results[0], results[2]) and torch.equal(results[1], results[2])
