@@ -142,12 +142,16 @@ class FusedAdam(torch.optim.Optimizer):
         raise TypeError("FusedAdam is not copied or pickled as a whole: use state_dict()")
 
     def state_dict(self):
+        """As torch.optim.Adam writes it by default, wherever it is read: the step counters on the host, and no group that says
+        they are on the GPU (an Adam of parameters elsewhere would not step)."""
         sd = super().state_dict()
+        sd["param_groups"] = [dict(g, capturable=False) for g in sd["param_groups"]]
+        steps = self._step.cpu().unbind()
         if self.state_bits == 8:
             m = _decode(self._flat["exp_avg"], self._flat["exp_avg_scale"])
             v = _decode(self._flat["exp_rms"], self._flat["exp_rms_scale"]).square()
-            sd["state"] = {i: {"step": self._step[i], "exp_avg": self._view(m, i), "exp_avg_sq": self._view(v, i)}
-                           for i in range(len(self._params))}
+            sd["state"] = {i: {"exp_avg": self._view(m, i), "exp_avg_sq": self._view(v, i)} for i in range(len(self._params))}
+        sd["state"] = {i: {**st, "step": steps[i]} for i, st in sd["state"].items()}
         return sd
 
     def load_state_dict(self, state_dict):

@@ -292,3 +292,35 @@ def test_update_without_eps_does_not_depend_on_the_scale():
             opt.step()
         results.append(p.detach())
     assert torch.equal(results[0], results[2]) and torch.equal(results[1], results[2])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_checkpoint_goes_on_on_the_host(bits):
+    """state_dict() into a torch.optim.Adam of parameters on the CPU, which steps, and back; without the trainer's own handling."""
+    import io
+    from alphazero_amd.optim import FusedAdam
+    gen = torch.Generator("cuda").manual_seed(7)
+    p = torch.randn(300, device="cuda", generator=gen).requires_grad_(True)
+    p.grad = torch.randn(300, device="cuda", generator=gen)
+    opt = FusedAdam([p], lr=1e-2, state_bits=bits)
+    opt.step()
+    file = io.BytesIO()
+    torch.save(opt.state_dict(), file)
+    file.seek(0)
+    q = p.detach().cpu().requires_grad_(True)
+    host = torch.optim.Adam([q], lr=1.0)
+    host.load_state_dict(torch.load(file, map_location="cpu", weights_only=True))
+    q.grad = p.grad.cpu()
+    host.step()
+    kept = {k: v.clone() for k, v in opt.state_dict()["state"][0].items()}
+    opt.step()
+    assert float((p.detach().cpu() - q.detach()).abs().max()) < 1e-6
+    assert float(host.state[q]["step"]) == 2.0 and float(kept["step"]) == 1.0
+    opt.load_state_dict(host.state_dict())
+    assert float(opt.flat_state()["step"]) == 2.0 and opt.param_groups[0]["capturable"]
+    graph = torch.cuda.CUDAGraph()                                      # still steps from a graph
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float(opt.flat_state()["step"]) == 3.0
