@@ -51,6 +51,8 @@ class FusedAdam(torch.optim.Optimizer):
     state_bits=32 keeps the moments in float32.  state_bits=8 keeps m and sqrt(v) as e4m3 codes with one power of two
     per 256, rounded at random (reproducibly: by `seed`, the step and the place): 2 bytes per weight instead of 8.
     Replicas of a model have to be given one seed (alphazero_amd.distributed.train_step checks that).
+    Weights whose gradients stay within four decades of the largest of their 256 get the updates of 32 bits to about 1 %
+    on average; further below v is held too large (no smaller than (4e-6)^2 of the block's largest) and the update is smaller.
 
     state_dict() is torch.optim.Adam's: per parameter step, exp_avg, exp_avg_sq (float32, also with 8-bit moments, which
     a load restores exactly: exp_avg all of it, sqrt(v) from 2^-63 on, where its square is a normal float32), so checkpoints go both ways.  Step counters live on the GPU; a step can be captured into
