@@ -348,3 +348,31 @@ def test_updates_in_8_bits_follow_those_in_32():
         at = decade == k
         assert 1.02 <= float(held[at].mean() / v[at].mean()) <= 1.06, k
         assert 0.99 <= float(p8.detach()[at].mean() / p32.detach()[at].mean()) <= 1.03, k
+
+
+@pytest.mark.parametrize("n, c, h, w, hidden", [(2, 1, 1, 1, 0), (1, 5, 1, 2, 0), (7, 130, 1, 1, 0), (7, 130, 1, 1, 16), (2, 40, 2, 2, 3), (3, 9, 1, 1, 2)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@LAYOUTS
+def test_norms_of_a_few_16_bit_values(n, c, h, w, hidden, dtype, layout):
+    check_norm(norm_inputs(n, c, h, w, hidden, dtype, layout, seed=n + c))
+
+
+@pytest.mark.parametrize("n, c, h, w", ROWS)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@LAYOUTS
+def test_what_is_not_finite_stays_in_its_channel(n, c, h, w, bad, layout):
+    """Every pass: a channel with a NaN or an infinity has NaN statistics, outputs and gradients; the others are what they are
+    without it, bit for bit.  Behind a gate every board hears of it."""
+    t = norm_inputs(n, c, h, w, 0, torch.float32, layout, seed=n)
+    clean = run_norm(t)
+    x = t["x"].clone(memory_format=torch.preserve_format)
+    x[n // 2, 1, 0, w // 2] = bad
+    got = run_norm({**t, "x": x})
+    others = [i for i in range(c) if i != 1]
+    for name in ("out", "x"):
+        assert bool(torch.isnan(got[name][:, 1]).all()) and torch.equal(got[name][:, others], clean[name][:, others]), name
+    for name in ("weight", "bias", "running_mean", "running_var"):
+        assert torch.equal(got[name][others], clean[name][others]), name
+    assert math.isnan(float(got["running_var"][1])) and not math.isfinite(float(got["running_mean"][1]))
+    gated = run_norm({**norm_inputs(n, c, h, w, 2, torch.float32, layout, seed=n), "x": x})
+    assert bool(torch.isnan(gated["out"]).all()) and bool(torch.isnan(gated["fc1_weight"]).all())
