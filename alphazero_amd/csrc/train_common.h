@@ -50,7 +50,7 @@ __device__ inline void store_pack(T* p, typename Pack<T>::f32 v, int left) {
     }
 }
 
-// Sum over L neighbouring lanes (L = 4, 8, 16 or 64), the result in all of them.  Inside 16 lanes the partner's value
+// Sum over L neighbouring lanes (L = 4, 8, 16, 32 or 64), the result in all of them.  Inside 16 lanes the partner's value
 // comes through the DPP operand of an add (quad permutes, then mirrors of 8 and 16: the halves are uniform by then).
 template <int L>
 __device__ inline float lane_sum(float v) {

@@ -13,15 +13,16 @@
 //   dx = weight / s (dy - dbias / m - xc / s dweight / m)  with m = n hw;  dresidual = gm
 // and the channel sums of dy come from S1, S2, dq and the board means, so grad and x are read twice.
 //
-// What bounds it: memory (the arithmetic is a handful of operations per value).  The plain form reads or writes 7
-// activations, the gated one 10, of which 4 and 6 could not be avoided by any form: x and the gradient are needed again
-// once the batch's sums are known.  A plain norm whose channels fit a workgroup's registers needs the 4.  Whether out > 0 is kept as a byte per 16 bytes of x.  Statistics are means and centred
-// sums of a row (about its own mean, or joined piece by piece in long rows and channels-last), so that no square of a distance
-// from somewhere else is taken off again; over the chunks of boards they are joined in 64 bits, where the squares of the
-// means may be subtracted.
-// Measured, forward and backward: at 4096 x 256 x 64 in bfloat16 (134 MB a tensor) 294 us, of which the four passes over
-// activations take 239 (1.34 GB: 5.6 TB/s; a copy of 1 GiB reaches 5.1) and the gate and the channel sums 55; at
-// 1024 x 128 x 64 in float32 83 us (61 and 22); a plain norm at 1024 x 128 x 64 in bfloat16 30 us.
+// What bounds it: memory (the arithmetic is a handful of operations per value).  Both directions together, the plain form reads
+// or writes 8 activations and the gated one 10: x and the gradient are needed again once the batch's sums are known.  A
+// plain norm whose channels fit a workgroup's registers takes 5, each tensor once a direction (4 and 6 are the different tensors
+// there are; x belongs to two calls).  The passes keep whether out > 0 as a byte per 16 bytes of x.
+// Statistics are means and centred sums of a row (about its own mean, or joined piece by piece in long rows and
+// channels-last), so that no square of a distance from somewhere else is taken off again; over the chunks of boards they are
+// joined in 64 bits, where the squares of the means may be subtracted.
+// Measured, forward and backward: at 4096 x 256 x 64 in bfloat16 (134 MB a tensor) 296 us, of which the four passes over
+// activations take 240 (1.34 GB: 5.6 TB/s; a copy of 1 GiB reaches 5.1) and the gate and the channel sums 57; at
+// 1024 x 128 x 64 in float32 83 us (61 and 22); a plain norm at 1024 x 128 x 64 in bfloat16 31 us.
 #include <math.h>
 
 #include <type_traits>
@@ -1077,8 +1078,8 @@ __global__ __launch_bounds__(CHANNELS * LINES) void k_param_grads(const NormPara
 
 // ------------------------------------------------------------- a plain norm, [n][c][hw]: a workgroup to a channel
 // Where a channel's n rows fit a workgroup's registers (8192 pieces of 16 bytes: 1024 boards of 8 x 8 in 16 bits) it is read
-// once, its sums are taken there and the result leaves by the same kernel: one launch each way instead of three, 4
-// activations instead of 7, and no mask (whether out > 0 follows from x again, by the same operations).  Sums are
+// once, its sums are taken there and the result leaves by the same kernel: one launch each way instead of three, 5
+// activations instead of 8, and no mask (whether out > 0 follows from x again, by the same operations).  Sums are
 // joined in 64 bits; the variance is taken about a first mean, with the remainder's square taken off.
 // Neighbouring channels share cache lines, so a die takes a range of them.
 // Forward and backward, beside the passes of row sums (all their launches): 37 x 48 x 81 in float16 10 us (22), 128 x 128 x 64 in
