@@ -63,6 +63,11 @@ static int fill_by_kernels(hipGraph_t graph, int32_t* replaced) {
         std::vector<hipGraphNode_t> to(behind);
         if (behind) AZ_HIP(hipGraphNodeGetDependentNodes(node, to.data(), &behind));
         hipGraphNode_t fill;
+        if (m.elementSize == 1 && m.height == 1 && (uintptr_t)m.dst % 4 == 0 && m.width % 4 == 0) {      // by words
+            m.elementSize = 4;
+            m.width /= 4;
+            m.value = (m.value & 0xFF) * 0x01010101u;
+        }
         if (m.elementSize == 1) AZ_HIP(add_fill<uint8_t>(&fill, graph, from, m));
         else if (m.elementSize == 2) AZ_HIP(add_fill<uint16_t>(&fill, graph, from, m));
         else AZ_HIP(add_fill<uint32_t>(&fill, graph, from, m));

@@ -87,7 +87,7 @@ def test_memset_nodes_are_replaced_where_they_stand():
         assert torch.equal(got, out)
 
 
-@pytest.mark.parametrize("width, height, pitch, size, value", [(1, 1, 1, 1, 7), (1000, 1, 1000, 1, 255), (333, 1, 0, 4, 0xDEADBEEF),
+@pytest.mark.parametrize("width, height, pitch, size, value", [(1, 1, 1, 1, 7), (1000, 1, 1000, 1, 255), (1001, 1, 0, 1, 0x7F), (64, 1, 0, 1, 0xAB), (333, 1, 0, 4, 0xDEADBEEF),
                                                                (77, 1, 0, 2, 0xBEEF), (10, 5, 64, 1, 3), (3, 7, 20, 4, 1), (1 << 20, 1, 0, 4, 2)])
 def test_every_form_of_a_memset_node(width, height, pitch, size, value):
     """A graph made by hand: what the replacing kernel writes, and nothing else, by bytes."""
